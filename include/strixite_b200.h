@@ -59,6 +59,17 @@ typedef struct strix_qmix_view {
     int64_t E, N, K, G;
 } strix_qmix_view;
 
+/* A matrix [N, K] in 8-bit floating point (e4m3, one byte each, row-major, 16-byte aligned) with one FP32 scale per block of
+ * 128 x 128: value = q[n, k] * scale[n / 128, k / 128]; scale is [ceil(N / 128), ceil(K / 128)], the last blocks may be partial.
+ * A stack of E experts of n rows each is [E * n, K] with scale [E * ceil(n / 128), ceil(K / 128)]: blocks start anew with every
+ * expert. Rows of activations in this format ("FP8 rows") are q [M, K] with one scale per (row, 128 columns), [M, ceil(K / 128)].
+ * No counterpart in the reference (its 8-bit format is an integer one): it is the form in which FP8 checkpoints ship. */
+typedef struct strix_fp8view {
+    const uint8_t *q;
+    const float *scale;
+    int64_t N, K;
+} strix_fp8view;
+
 const char *strix_last_error(void);
 /* Library identity: "strixite_b200 <version> sm_100a". */
 const char *strix_version(void);
@@ -103,6 +114,19 @@ int strix_moe_shared_add_inject(void *y, const void *s, const float *gate_logit,
                                 int64_t N, uint32_t gate_index, void *x, const float *w_in, int64_t H, int act,
                                 uint32_t *err, void *stream);
 
+/* Routing by scores (no counterpart in the reference, whose router is the softmax top-k above): s = softmax (score 0) or sigmoid
+ * (score 1) of the logits [M, E] (row stride ld); c = s + bias (FP32 [E] or NULL: a balance bias takes part in the choice only). The
+ * experts form n_group groups of E / n_group neighbours; a group's value is its largest c (group_top 1) or the sum of its two
+ * largest (2); the topk_group largest groups stay open and the k largest c among their experts are the picks. Ties go to the lower
+ * index; the order is that of the 64-bit values of c. coef = s of the picks, divided by their sum when renorm (picks whose scores
+ * all underflow to zero keep 0), times route_scale. ids, coef [M, A] in descending c, A = k (+ 1 with the shared slot, which is
+ * filled as moe_router does). n_group <= 32 divides E <= 1024; k <= min(32, topk_group * E / n_group). A non-finite logit or bias
+ * fails the token: ids -1, coef NaN, err = {1, token, expert}. */
+int strix_moe_router_scored(const void *logits, int64_t ld, int64_t M, int64_t E, int64_t k, int score, const float *bias,
+                            int64_t n_group, int64_t topk_group, int64_t group_top, int renorm, float route_scale,
+                            const void *shared_logit, int64_t shared_ld, int32_t shared_id, int32_t *ids, float *coef, int act,
+                            uint32_t *err, void *stream);
+
 /* ---- dense projections ----------------------------------------------------------------------------------------- */
 
 /* strixite kernels/linear_q4.hpp:26-30 linear_q4 (with out_act), linear_q5.hpp:14-15, linear_q6.hpp:14-15,
@@ -128,10 +152,26 @@ int strix_linear_bf16w_wmma(const void *x, const uint16_t *w, void *y, int64_t M
 int strix_linear_f32w(const void *x, const float *w, void *y, int64_t M, int64_t N, int64_t K, int act, int out_act,
                       void *stream);
 
+/* y[M, N] = dequant(xq, xs) * dequant(W)^T in 8-bit floating point on the tensor cores (strix_fp8view): per 128-column block
+ * FP32 sums of exact products, scaled and summed in FP32, one rounding to out_act (F32 or BF16). Any M and N; K % 16 == 0.
+ * No counterpart in the reference. */
+int strix_linear_fp8(const uint8_t *xq, const float *xs, const strix_fp8view *w, void *y, int64_t M, int out_act, void *stream);
+
 /* ---- elementwise ----------------------------------------------------------------------------------------------- */
 
 /* strixite kernels/swiglu.hpp:21 swiglu. */
 int strix_swiglu(const void *gu, void *h, int64_t rows, int64_t I, int act, void *stream);
+/* swiglu with the result as FP8 rows (strix_fp8view): h = silu(gate) * up in FP32, per (row, 128 columns) scale = max(amax |h|,
+ * 2^-100) / 448 and q = e4m3(h / scale), round to nearest even. gu [rows, 2I] -> q [rows, I], scale [rows, ceil(I / 128)].
+ * I % 16 == 0. No counterpart in the reference. */
+int strix_swiglu_fp8(const void *gu, uint8_t *q, float *scale, int64_t rows, int64_t I, int act, void *stream);
+/* The norm in front of the layer with the residual's addition: x_out = x + y rounded to act (y and x_out NULL: x as it is; x_out may be
+ * x or y), h = x_out * g / sqrt(mean(x_out^2) + eps) from the stored values, g = w (FP32 [d]) or 1 + w when centered. h [M, d] in the
+ * activation dtype (or NULL), and the unrounded h as FP8 rows q, scale as strix_swiglu_fp8 makes them (or both NULL). A NaN makes its
+ * whole row NaN; an infinity (or an FP32 sum of squares that overflows to one) makes h 0, and NaN where x_out is infinite; a block with
+ * a NaN is NaN in every code and in its scale. d % 16 == 0, d <= 16384. No counterpart in the reference's MoE path. */
+int strix_residual_rmsnorm_fp8(const void *x, const void *y, const float *w, int centered, float eps, int64_t M, int64_t d,
+                               void *x_out, void *h, uint8_t *q, float *scale, int act, void *stream);
 /* strixite kernels/residual.hpp:17 residual_add. */
 int strix_residual_add(void *x, const void *y, int64_t n, int act, void *stream);
 /* strixite kernels/hc.hpp:52-55 hc_inject: x[t, s*N + n] = fma(w_in[t, s], y[t, n], x[t, s*N + n]), x [M, H*N]. */
@@ -245,6 +285,17 @@ int strix_linear_qmix_experts_gather_grouped(const void *x, const strix_qmix_vie
 int strix_linear_qmix_experts_combine_grouped(const void *h, const strix_qmix_view *w, const int32_t *ids,
                                               const float *coef, const void *ws, size_t ws_bytes, float *partial,
                                               int64_t M, int64_t A, void *y, int act, int math, void *stream);
+
+/* The grouped pair in 8-bit floating point (strix_fp8view stacks of E experts): gather y[slot, :] = W[ids[slot]] * row slot / A of
+ * the FP8 rows xq [M, K], xs, in slot order [M * A, N]; combine partial[slot, :] = W[ids[slot]] * FP8 row slot of hq [M * A, K], hs,
+ * then y[m, :] = sum over a ascending of coef * partial, one rounding. Slots with an invalid id keep their rows of y (gather) and make
+ * their token's row NaN (combine). ws: moe_group_routes of the same ids. partial: M * A * N floats. K % 16 == 0, any N.
+ * No counterpart in the reference. */
+int strix_linear_fp8_experts_gather_grouped(const uint8_t *xq, const float *xs, const strix_fp8view *w, int64_t E, const void *ws,
+                                            size_t ws_bytes, int64_t M, int64_t A, void *y, int out_act, void *stream);
+int strix_linear_fp8_experts_combine_grouped(const uint8_t *hq, const float *hs, const strix_fp8view *w, int64_t E,
+                                             const int32_t *ids, const float *coef, const void *ws, size_t ws_bytes,
+                                             float *partial, int64_t M, int64_t A, void *y, int act, void *stream);
 
 /* ---- the MoE sublayer as one object ----------------------------------------------------------------------------
  * The per-layer driver of strixite runtime/qwen4exp.cpp:1126-1186 (Qwen4ExpSession::forward's MoE block, and

@@ -7,7 +7,7 @@ the package loads the library and raises if it is missing - there is no CPU or P
 from ._lib import LIB_PATH, StrixError, lib  # noqa: F401
 from . import kernels  # noqa: F401
 from . import layer  # noqa: F401
-from .kernels import Act, MoeMath, QMixStack, QWeight  # noqa: F401
+from .kernels import Act, Fp8Weight, MoeMath, QMixStack, QWeight  # noqa: F401
 from .layer import MoeLayer  # noqa: F401
 
 __version__ = lib.strix_version().decode()

@@ -27,6 +27,12 @@ class QMixView(C.Structure):
                 ("E", C.c_int64), ("N", C.c_int64), ("K", C.c_int64), ("G", C.c_int64)]
 
 
+class Fp8View(C.Structure):
+    """strix_fp8view: an e4m3 matrix with an FP32 scale per 128 x 128 block."""
+
+    _fields_ = [("q", C.c_void_p), ("scale", C.c_void_p), ("N", C.c_int64), ("K", C.c_int64)]
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -39,7 +45,7 @@ def _load():
 lib = _load()
 
 _vp, _i64, _i32, _u32, _int, _sz = C.c_void_p, C.c_int64, C.c_int32, C.c_uint32, C.c_int, C.c_size_t
-_qv, _qm = C.POINTER(QView), C.POINTER(QMixView)
+_qv, _qm, _fv = C.POINTER(QView), C.POINTER(QMixView), C.POINTER(Fp8View)
 
 # name -> argument types; every function returns int unless listed in _RESTYPES.
 SIGNATURES = {
@@ -49,6 +55,12 @@ SIGNATURES = {
     "strix_row_bytes": [_int, _i64],
     "strix_quantize_device": [_int, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp],
     "strix_moe_router": [_vp, _i64, _i64, _i64, _i64, _vp, _i64, _i32, _vp, _vp, _int, _vp, _vp],
+    "strix_moe_router_scored": [_vp, _i64, _i64, _i64, _i64, _int, _vp, _i64, _i64, _i64, _int, C.c_float, _vp, _i64, _i32, _vp, _vp, _int, _vp, _vp],
+    "strix_linear_fp8": [_vp, _vp, _fv, _vp, _i64, _int, _vp],
+    "strix_swiglu_fp8": [_vp, _vp, _vp, _i64, _i64, _int, _vp],
+    "strix_residual_rmsnorm_fp8": [_vp, _vp, _vp, _int, C.c_float, _i64, _i64, _vp, _vp, _vp, _vp, _int, _vp],
+    "strix_linear_fp8_experts_gather_grouped": [_vp, _vp, _fv, _i64, _vp, _sz, _i64, _i64, _vp, _int, _vp],
+    "strix_linear_fp8_experts_combine_grouped": [_vp, _vp, _fv, _i64, _vp, _vp, _vp, _sz, _vp, _i64, _i64, _vp, _int, _vp],
     "strix_check_router_error": [_vp, C.c_char_p],
     "strix_report_router_error": [_vp, C.c_char_p],
     "strix_moe_shared_add": [_vp, _vp, _vp, _i64, _i64, _i64, _u32, _int, _vp, _vp],

@@ -1,0 +1,180 @@
+// The two places of a layer where activations become FP8 rows: the RMS norm in front of the FFN (with the residual's addition)
+// and the SwiGLU between its two products.
+#include "fp8.cuh"
+
+#include "strixite_b200.h"
+
+namespace {
+
+using namespace sb;
+
+constexpr int kNormMaxThreads = 256;
+constexpr int kNormMaxVec = 8;  // 8-element pieces a thread can hold: d <= 256 * 8 * 8
+
+// One block per row; a thread holds VEC pieces of 8 consecutive elements in registers, so a row is read once whatever its
+// length: x' = x + y rounded to the activation type (what the residual stream keeps), r = 1 / sqrt(mean(x'^2) + eps) from the stored
+// values, h = x' r g. 16 neighbouring threads hold one 128-column block: its largest magnitude is a half-warp reduction.
+// Bound by memory: nothing is read twice, and the row's values never leave the registers.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kNormMaxThreads)
+    rmsnorm_fp8_kernel(const T *x, const T *y, const float *w, float w_add, float eps, int d, T *x_out, T *h_out, uint8_t *q, float *scale, int blocks) {
+    __shared__ float part[kNormMaxThreads / 32];
+    const int64_t row = blockIdx.x, base = row * d;
+    float v[VEC][8];
+    float sq = 0.f;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+        const int c = (threadIdx.x + i * blockDim.x) * 8;
+        if (c < d) {
+            load8(x + base + c, v[i]);
+            if (y != nullptr) {
+                float a[8];
+                load8(y + base + c, a);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] = as_stored(v[i][j] + a[j], x_out);
+                store8(x_out + base + c, v[i]);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sq = fmaf(v[i][j], v[i][j], sq);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+        }
+    }
+    sq = warp_sum(sq);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sq;
+    __syncthreads();
+    float total = 0.f;
+    for (int i = 0; i < (int)blockDim.x / 32; ++i) total += part[i];
+    const float r = 1.0f / sqrtf(total / (float)d + eps);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+        const int c = (threadIdx.x + i * blockDim.x) * 8;
+        uint32_t top = 0;
+        if (c < d) {
+            float g[8];
+            load8(w + c, g);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[i][j] = v[i][j] * r * (g[j] + w_add);
+                top = max(top, abs_bits(v[i][j]));
+            }
+            if (h_out != nullptr) store8(h_out + base + c, v[i]);
+        }
+        if (q != nullptr) {  // the same for the whole grid; the reduction runs on full warps
+            const float s = fp8_scale(half_warp_max(top));
+            if (c < d) {
+                *reinterpret_cast<uint2 *>(q + base + c) = fp8_pack8(v[i], s);
+                if ((c & (kFp8Block - 1)) == 0) scale[row * blocks + c / kFp8Block] = s;
+            }
+        }
+    }
+}
+
+template <typename T>
+void launch_norm(const void *x, const void *y, const float *w, float w_add, float eps, int64_t M, int64_t d, void *x_out, void *h, uint8_t *q, float *scale,
+                 cudaStream_t st) {
+    const int pieces = (int)(d / 8);
+    int vec = 1;
+    while (vec < kNormMaxVec && pieces > vec * kNormMaxThreads) vec *= 2;
+    const int threads = ((pieces + vec - 1) / vec + 31) / 32 * 32;
+    const int blocks = (int)fp8_blocks(d);
+#define SB_NORM(V) \
+    rmsnorm_fp8_kernel<T, V><<<(unsigned)M, threads, 0, st>>>((const T *)x, (const T *)y, w, w_add, eps, (int)d, (T *)x_out, (T *)h, q, scale, blocks)
+    if (vec == 1) SB_NORM(1);
+    else if (vec == 2) SB_NORM(2);
+    else if (vec == 4) SB_NORM(4);
+    else SB_NORM(8);
+#undef SB_NORM
+}
+
+// A half warp per (row, 128-column block) of h = silu(gate) * up, 8 elements a thread. Gate and up stay FP32 until the one rounding
+// to e4m3.
+template <typename T>
+__global__ void __launch_bounds__(256) swiglu_fp8_kernel(const T *gu, uint8_t *q, float *scale, int64_t rows, int I, int blocks) {
+    const int64_t units = rows * blocks, stride = (int64_t)gridDim.x * (blockDim.x / 16);
+    const int t = threadIdx.x & 15;
+    for (int64_t u0 = (int64_t)blockIdx.x * (blockDim.x / 16); u0 < units; u0 += stride) {
+        const int64_t u = u0 + threadIdx.x / 16;
+        const int64_t row = u / blocks;
+        const int b = (int)(u - row * blocks), c = b * kFp8Block + t * 8;
+        const bool live = u < units && c < I;
+        float h[8];
+        uint32_t top = 0;
+        if (live) {
+            float g[8], up[8];
+            load8(gu + row * 2 * I + c, g);
+            load8(gu + row * 2 * I + I + c, up);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[j] = silu_f(g[j]) * up[j], top = max(top, abs_bits(h[j]));
+        }
+        const float s = fp8_scale(half_warp_max(top));
+        if (live) {
+            *reinterpret_cast<uint2 *>(q + row * I + c) = fp8_pack8(h, s);
+            if (t == 0) scale[u] = s;
+        }
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+int strix_residual_rmsnorm_fp8(const void *x, const void *y, const float *w, int centered, float eps, int64_t M, int64_t d, void *x_out, void *h,
+                               uint8_t *q, float *scale, int act, void *stream) {
+    const char *fn = "residual_rmsnorm_fp8";
+    SB_CHECK(x != nullptr && w != nullptr, fn, ": null pointer (x=", x, ", w=", (const void *)w, ")");
+    SB_CHECK((y == nullptr) == (x_out == nullptr), fn, ": y and x_out come together (y=", y, ", x_out=", x_out, ")");
+    SB_CHECK((q == nullptr) == (scale == nullptr), fn, ": q and scale come together (q=", (const void *)q, ", scale=", (const void *)scale, ")");
+    SB_CHECK(h != nullptr || q != nullptr, fn, ": neither h nor q is asked for");
+    SB_CHECK(act_ok(act), fn, ": unsupported activation dtype ", act);
+    SB_CHECK(M >= 1 && M <= 0x7fffffff, fn, ": M = ", M, " rows, expected 1..2^31-1");
+    SB_CHECK(d >= 16 && d % 16 == 0 && d <= kNormMaxThreads * kNormMaxVec * 8, fn, ": d = ", d, ", expected a multiple of 16 up to ",
+             kNormMaxThreads * kNormMaxVec * 8);
+    SB_CHECK(eps >= 0.0f, fn, ": eps = ", eps, ", expected >= 0");
+    SB_CHECK(aligned16(x) && aligned16(y) && aligned16(w) && aligned16(x_out) && aligned16(h) && aligned16(q) && reinterpret_cast<uintptr_t>(scale) % 4 == 0,
+             fn, ": x, y, w, x_out, h and q must be 16-byte aligned, scale 4-byte");
+    const int64_t xb = M * d * act_size(act), qb = M * d, sb_ = M * fp8_blocks(d) * 4, wb = d * 4;
+    // a block of threads reads a whole row before it writes h and q, but other rows' blocks run at the same time: only exact aliases
+    // of the same rows are harmless
+    SB_CHECK(x_out == nullptr || ((x_out == x || apart(x_out, xb, x, xb)) && (x_out == y || apart(x_out, xb, y, xb))), fn,
+             ": x_out partly overlaps x or y");
+    const void *ins[3] = {x, y, w}, *outs[4] = {x_out, h, q, scale};
+    const int64_t in_b[3] = {xb, xb, wb}, out_b[4] = {xb, xb, qb, sb_};
+    for (int o = 0; o < 4; ++o) {
+        if (outs[o] == nullptr) continue;
+        for (int i = 0; i < 3; ++i)
+            SB_CHECK(ins[i] == nullptr || (o == 0 && i < 2) || apart(outs[o], out_b[o], ins[i], in_b[i]), fn, ": output ", o, " [", outs[o], ", +", out_b[o],
+                     " B) overlaps input ", i, " [", ins[i], ", +", in_b[i], " B)");
+        for (int p = 0; p < o; ++p)
+            SB_CHECK(outs[p] == nullptr || apart(outs[o], out_b[o], outs[p], out_b[p]), fn, ": outputs ", p, " and ", o, " overlap");
+    }
+    auto st = static_cast<cudaStream_t>(stream);
+    const float w_add = centered ? 1.0f : 0.0f;
+    if (act == kF32) launch_norm<float>(x, y, w, w_add, eps, M, d, x_out, h, q, scale, st);
+    else launch_norm<uint16_t>(x, y, w, w_add, eps, M, d, x_out, h, q, scale, st);
+    SB_LAUNCH_OK(fn, " ", act_name(act), " M=", M, " d=", d);
+    return 0;
+}
+
+int strix_swiglu_fp8(const void *gu, uint8_t *q, float *scale, int64_t rows, int64_t I, int act, void *stream) {
+    const char *fn = "swiglu_fp8";
+    SB_CHECK(gu != nullptr && q != nullptr && scale != nullptr, fn, ": null pointer (gu=", gu, ", q=", (const void *)q, ", scale=", (const void *)scale, ")");
+    SB_CHECK(act_ok(act), fn, ": unsupported activation dtype ", act);
+    SB_CHECK(rows >= 1 && I >= 16 && I % 16 == 0 && I <= (1 << 24), fn, ": rows = ", rows, ", I = ", I, " (I a multiple of 16 up to 2^24)");
+    SB_CHECK(rows <= (1ll << 40) / I / 2, fn, ": rows * 2I = ", rows, " * ", 2 * I, " is too large (rows/I swapped?)");
+    SB_CHECK(aligned16(gu) && aligned16(q) && reinterpret_cast<uintptr_t>(scale) % 4 == 0, fn, ": gu and q must be 16-byte aligned, scale 4-byte");
+    const int64_t gb = rows * 2 * I * act_size(act), qb = rows * I, sb_ = rows * fp8_blocks(I) * 4;
+    SB_CHECK(apart(q, qb, gu, gb) && apart(scale, sb_, gu, gb) && apart(q, qb, scale, sb_), fn, ": q [", (const void *)q, "], scale [", (const void *)scale,
+             "] and gu [", gu, "] overlap");
+    const int blocks = (int)fp8_blocks(I);
+    const int64_t units = rows * blocks, want = (units + 15) / 16, cap = (int64_t)sm_count() * 32;
+    const unsigned grid = (unsigned)(want < cap ? want : cap);
+    auto st = static_cast<cudaStream_t>(stream);
+    if (act == kF32) swiglu_fp8_kernel<float><<<grid, 256, 0, st>>>((const float *)gu, q, scale, rows, (int)I, blocks);
+    else swiglu_fp8_kernel<uint16_t><<<grid, 256, 0, st>>>((const uint16_t *)gu, q, scale, rows, (int)I, blocks);
+    SB_LAUNCH_OK(fn, " ", act_name(act), " rows=", rows, " I=", I);
+    return 0;
+}
+
+}  // extern "C"

@@ -1,0 +1,585 @@
+// Products in 8-bit floating point with a scale per block of 128, dense and for the experts' routed slots, on the tensor cores.
+//
+//   y[r, n] = sum_kb (xs[r, kb] * ws[n / 128, kb]) * (sum over the 128 k of block kb of xq[r, k] * wq[n, k])
+//
+// The inner sum of a block is one tcgen05 accumulation (kind::f8f6f4; the products of two e4m3 values are exact and are summed in
+// FP32), the outer sum an FP32 FMA of that accumulator, taken from tensor memory, into registers: a scale per 128 columns cannot be
+// applied inside the accumulation.
+//
+// Weight rows are the M axis of the MMA (128 lanes: one block row of scales) and the rows of x its N axis, up to TOK at a time: a few
+// rows (decode) cost a narrow instruction, and an expert's ragged slot list is padded to 16. Warp roles of a CTA:
+//   promotion warps   tcgen05.ld of a finished block accumulator, acc = fma(scale, block, acc); at the end the store of y
+//   TMA warp          weight boxes [128 rows x 128 bytes] and rows of x (a box, or gathered by slot for the experts), 128-byte swizzle
+//   MMA warp          four K = 32 instructions per block into one of NBUF accumulators, two commits
+//   scale warp        xs * ws of the block for the TOK columns, through a ring in shared memory
+// CTAs walk the (x tile, weight tile) pairs; where there are fewer pairs than SMs the blocks of K are split over the CTAs of a cluster,
+// whose register sums meet in distributed shared memory and are added in rank order (the same result on every run).
+// Every mbarrier wait is bounded: on expiry the CTA raises the abort counter, waits for its copies, frees its tensor memory, returns.
+#include <cuda.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "fp8.cuh"
+#include "grouped.cuh"
+#include "prefill_umma.cuh"
+#include "strixite_b200.h"
+#include "umma.cuh"
+
+namespace {
+
+using namespace sb;
+using namespace sb::umma;
+
+__device__ unsigned int g_fp8_aborts = 0;
+__device__ unsigned int g_fp8_refusals = 0;
+
+constexpr int kBK = 128;                  // K per stage: one scale block, one 128-byte swizzle row
+constexpr int kATile = kTileM * kBK;      // 16 KB of weights
+constexpr int kScaleSlots = 4;
+constexpr int kMaxSplit = 8;              // portable cluster size
+constexpr int kMaxE = 1023;
+
+template <int TOK>
+struct Cfg {
+    static constexpr int BTile = TOK * kBK;
+    static constexpr int Stages = TOK >= 256 ? 4 : TOK >= 128 ? 6 : TOK >= 64 ? 8 : TOK >= 32 ? 9 : 10;
+    static constexpr int NBuf = TOK >= 256 ? 2 : 4;                // accumulators in tensor memory
+    static constexpr int TmemCols = NBuf * TOK < 32 ? 32 : NBuf * TOK;
+    static constexpr int PromoWarps = TOK >= 128 ? 8 : 4;
+    static constexpr int Cols = TOK / (PromoWarps / 4);            // columns a promotion thread holds
+    static constexpr int Threads = (PromoWarps + 3) * 32;
+    static constexpr int StageBytes = kATile + BTile;
+};
+
+template <int TOK>
+struct Ctl {
+    using C = Cfg<TOK>;
+    uint64_t full[C::Stages], empty[C::Stages], acc_full[C::NBuf], acc_empty[C::NBuf], sc_full[kScaleSlots], sc_empty[kScaleSlots];
+    uint32_t tmem_base;
+    int abort_flag;
+    int warp_tot[32];
+    alignas(16) float scales[kScaleSlots][TOK];  // read as float4
+    int prefix[kMaxE + 1 + 1];  // grouped: first tile of each bucket
+};
+
+template <int TOK>
+constexpr size_t smem_bytes() {
+    return (size_t)Cfg<TOK>::Stages * Cfg<TOK>::StageBytes + sizeof(Ctl<TOK>) + 1024;
+}
+
+struct GemmArgs {
+    const float *xs, *ws;    // scales of x rows [.., KB] and of the weight blocks [(E *) NB, KB]
+    const int32_t *group;    // grouped: the workspace of moe_group_routes
+    void *y;
+    int out_f32;
+    int M, N, KB, NB;        // dense: rows of x; rows of one matrix, blocks of K, block rows of one matrix
+    int E, div;              // grouped: slot s reads row s / div
+    int64_t S;
+    int NT, split;           // weight tiles of one matrix; CTAs that share a pair's K blocks
+};
+
+// kind::f8f6f4: D = F32 (bits 4-5 = 1), A and B e4m3 (0), both K-major, N = n, M = 128.
+__device__ __forceinline__ uint32_t idesc_e4m3(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24); }
+__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+        ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(0u)
+        : "memory");
+}
+// Four rows r0..r3 of a tensor map whose box is one row of 128 bytes, to four consecutive 128-byte rows of shared memory.
+__device__ __forceinline__ void tma_gather4(void *dst, const void *tmap, int x, int r0, int r1, int r2, int r3, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(
+            smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(smem_u32(bar))
+        : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_peer(uint32_t addr, uint32_t rank) {
+    uint32_t p;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(p) : "memory");
+    return v;
+}
+
+// One (x tile, weight tile) pair: its first row of the weight stack, first weight row and block row inside its matrix, and its columns -
+// dense: rows first .. first + n of x; grouped: the slots list[first .. first + n).
+struct Pair {
+    int wrow, n0, ws_row, first, n;
+};
+
+template <int TOK, bool GROUPED>
+__global__ void __launch_bounds__(Cfg<TOK>::Threads, 1)
+    fp8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const GemmArgs a) {
+    using C = Cfg<TOK>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    Ctl<TOK> &ctl = *reinterpret_cast<Ctl<TOK> *>(base + C::Stages * C::StageBytes);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    constexpr int kTmaWarp = C::PromoWarps, kMmaWarp = kTmaWarp + 1, kScaleWarp = kTmaWarp + 2;
+    if (GROUPED && !ws_is_for(a.group, a.S, a.E, &g_fp8_refusals)) return;  // the whole grid leaves
+    if (tid == 0) {
+        for (int i = 0; i < C::Stages; ++i) mbar_init(&ctl.full[i], 1), mbar_init(&ctl.empty[i], 1);
+        for (int i = 0; i < C::NBuf; ++i) mbar_init(&ctl.acc_full[i], 1), mbar_init(&ctl.acc_empty[i], C::PromoWarps);
+        for (int i = 0; i < kScaleSlots; ++i) mbar_init(&ctl.sc_full[i], 1), mbar_init(&ctl.sc_empty[i], C::PromoWarps);
+        ctl.abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem_base)), "r"((uint32_t)C::TmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    RouteTables rt{};
+    int x_tiles;
+    if constexpr (GROUPED) {
+        // tiles of TOK slots per bucket, as a prefix over the buckets: a thread owns kPer neighbouring ones
+        constexpr int kPer = (kMaxE + C::Threads) / C::Threads;
+        rt = route_tables(a.group, a.S, a.E);
+        int nt[kPer], sum = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int e = tid * kPer + i;
+            nt[i] = e < a.E ? (rt.offsets[e + 1] - rt.offsets[e] + TOK - 1) / TOK : 0;
+            sum += nt[i];
+        }
+        int incl = sum;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, incl, off);
+            if (lane >= off) incl += o;
+        }
+        if (lane == 31) ctl.warp_tot[warp] = incl;
+        __syncthreads();
+        int before = incl - sum;
+        x_tiles = 0;
+        for (int i = 0; i < C::Threads / 32; ++i) {
+            const int t = ctl.warp_tot[i];
+            before += i < warp ? t : 0;
+            x_tiles += t;
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int e = tid * kPer + i;
+            if (e <= a.E) ctl.prefix[e] = before;
+            before += nt[i];
+        }
+        if (tid == 0) ctl.prefix[a.E] = x_tiles;
+    } else {
+        x_tiles = (a.M + TOK - 1) / TOK;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = ctl.tmem_base;
+    volatile int *abort_flag = &ctl.abort_flag;
+    const int rank = a.split > 1 ? (int)cluster_rank() : 0;
+    const int n_pairs = x_tiles * a.NT, first_pair = blockIdx.x / a.split, pair_step = gridDim.x / a.split;
+    const int kb0 = (int)((int64_t)a.KB * rank / a.split), kb1 = (int)((int64_t)a.KB * (rank + 1) / a.split);
+
+    auto pair_of = [&](int p) {  // warp-uniform
+        const int xt = p / a.NT, nt = p - xt * a.NT;
+        Pair r;
+        r.n0 = nt * kTileM;
+        if constexpr (GROUPED) {
+            int lo = 0, hi = a.E;  // prefix[lo] <= xt < prefix[hi]
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (ctl.prefix[mid] <= xt) lo = mid;
+                else hi = mid;
+            }
+            const int begin = rt.offsets[lo] + (xt - ctl.prefix[lo]) * TOK;
+            r.wrow = lo * a.N + r.n0, r.ws_row = lo * a.NB + nt;
+            r.first = begin, r.n = min(TOK, rt.offsets[lo + 1] - begin);
+        } else {
+            r.wrow = r.n0, r.ws_row = nt;
+            r.first = xt * TOK, r.n = min(TOK, a.M - r.first);
+        }
+        return r;
+    };
+    auto row_of = [&](const Pair &p, int j) {  // the row of x behind column j < p.n
+        if constexpr (GROUPED) return rt.slots[p.first + j] / a.div;
+        else return p.first + j;
+    };
+
+    if (warp == kTmaWarp) {
+        constexpr int kQuads = TOK / 4, kPerLane = (kQuads + 31) / 32;
+        uint32_t it = 0;
+        bool ok = true;
+        for (int p = first_pair; p < n_pairs && ok; p += pair_step) {
+            const Pair t = pair_of(p);
+            int rows[kPerLane][4];
+            uint32_t bytes = C::StageBytes;
+            if constexpr (GROUPED) {
+                // columns beyond the list's end repeat its last row; whole quads beyond it are not fetched, and what their columns
+                // compute is not stored
+                for (int i = 0; i < kPerLane; ++i)
+                    for (int j = 0; j < 4; ++j) rows[i][j] = row_of(t, min((lane + 32 * i) * 4 + j, t.n - 1));
+                bytes = kATile + (uint32_t)((t.n + 3) / 4) * 4 * kBK;
+            }
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int s = it % C::Stages;
+                if (lane == 0) ok = mbar_wait(&ctl.empty[s], ((it / C::Stages) & 1u) ^ 1u, abort_flag);
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (!ok) break;
+                uint8_t *dst = base + s * C::StageBytes;
+                if (lane == 0) {
+                    mbar_expect_tx(&ctl.full[s], bytes);
+                    tma_load_2d(dst, &w_map, kb * kBK, t.wrow, &ctl.full[s]);
+                    if constexpr (!GROUPED) tma_load_2d(dst + kATile, &x_map, kb * kBK, t.first, &ctl.full[s]);
+                }
+                __syncwarp();
+                if constexpr (GROUPED) {
+#pragma unroll
+                    for (int i = 0; i < kPerLane; ++i) {
+                        const int quad = lane + 32 * i;
+                        if (quad < kQuads && quad * 4 < t.n)
+                            tma_gather4(dst + kATile + quad * 4 * kBK, &x_map, kb * kBK, rows[i][0], rows[i][1], rows[i][2], rows[i][3], &ctl.full[s]);
+                    }
+                }
+            }
+        }
+        if (!ok && lane == 0) {  // abandoned: the copies in flight land before the shared memory goes
+            for (uint32_t i = it > C::Stages ? it - C::Stages : 0; i < it; ++i)
+                for (uint32_t n = 0; n < kSpinLimit && !mbar_try_wait(&ctl.full[i % C::Stages], (i / C::Stages) & 1u); ++n) {
+                }
+        }
+        __syncwarp();
+    } else if (warp == kMmaWarp) {
+        uint32_t it = 0;
+        bool ok = true;
+        for (int p = first_pair; p < n_pairs && ok; p += pair_step) {
+            const Pair t = pair_of(p);
+            const uint32_t idesc = idesc_e4m3((t.n + 15) & ~15);
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int s = it % C::Stages, b = it % C::NBuf;
+                ok = mbar_wait(&ctl.acc_empty[b], ((it / C::NBuf) & 1u) ^ 1u, abort_flag) && mbar_wait(&ctl.full[s], (it / C::Stages) & 1u, abort_flag);
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint32_t at = smem_u32(base + s * C::StageBytes);
+                    const uint64_t da = umma_desc(at), db = umma_desc(at + kATile);
+#pragma unroll
+                    for (int k = 0; k < kBK / 32; ++k) umma_f8(tmem + b * TOK, da + 2 * k, db + 2 * k, idesc, k != 0);
+                    umma_commit(&ctl.empty[s]);
+                    umma_commit(&ctl.acc_full[b]);
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp == kScaleWarp) {
+        constexpr int kPerLane = (TOK + 31) / 32;
+        uint32_t it = 0;
+        bool ok = true;
+        for (int p = first_pair; p < n_pairs && ok; p += pair_step) {
+            const Pair t = pair_of(p);
+            const float *xp[kPerLane];
+            // four blocks at a time: a row's four scales share a 32-byte sector, and a round of loads is under way while the round before
+            // it is handed over
+            float cur[kPerLane][4], nxt[kPerLane][4];
+            const float *wp = a.ws + (int64_t)t.ws_row * a.KB;
+            auto fetch = [&](float(&to)[kPerLane][4], int kb) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const bool in = kb + q < kb1;
+                    const float w = in ? wp[kb + q] : 0.f;
+#pragma unroll
+                    for (int i = 0; i < kPerLane; ++i) to[i][q] = in && xp[i] != nullptr ? xp[i][kb + q] * w : 0.f;
+                }
+            };
+#pragma unroll
+            for (int i = 0; i < kPerLane; ++i) xp[i] = lane + 32 * i < t.n ? a.xs + (int64_t)row_of(t, lane + 32 * i) * a.KB : nullptr;
+            fetch(cur, kb0);
+            for (int kb = kb0; kb < kb1 && ok; kb += 4) {
+                fetch(nxt, kb + 4);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if (kb + q >= kb1 || !ok) continue;
+                    const int s = it % kScaleSlots;
+                    ok = __all_sync(0xffffffffu, mbar_wait(&ctl.sc_empty[s], ((it / kScaleSlots) & 1u) ^ 1u, abort_flag));
+                    if (!ok) continue;
+#pragma unroll
+                    for (int i = 0; i < kPerLane; ++i)
+                        if (lane + 32 * i < TOK) ctl.scales[s][lane + 32 * i] = cur[i][q];
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&ctl.sc_full[s]);
+                    ++it;
+                }
+#pragma unroll
+                for (int i = 0; i < kPerLane; ++i)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) cur[i][q] = nxt[i][q];
+            }
+        }
+    } else {
+        // ---- promotion ----
+        constexpr int kChunk = C::Cols < 32 ? C::Cols : 32;
+        const int col0 = (warp / 4) * C::Cols, r = (warp & 3) * 32 + lane;
+        const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16) + col0;
+        uint32_t it = 0;
+        bool ok = true;
+        for (int p = first_pair; p < n_pairs && ok; p += pair_step) {
+            const Pair t = pair_of(p);
+            float acc[C::Cols];
+#pragma unroll
+            for (int j = 0; j < C::Cols; ++j) acc[j] = 0.f;
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int b = it % C::NBuf, s = it % kScaleSlots;
+                ok = mbar_wait(&ctl.sc_full[s], (it / kScaleSlots) & 1u, abort_flag) && mbar_wait(&ctl.acc_full[b], (it / C::NBuf) & 1u, abort_flag);
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < C::Cols; c += kChunk) {
+                    if (col0 + c >= t.n) continue;  // warp-uniform
+                    uint32_t v[kChunk];
+                    if constexpr (kChunk == 32) tmem_ld32(lane_base + b * TOK + c, v);
+                    else tmem_ld16(lane_base + b * TOK + c, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < kChunk; j += 4) {
+                        const float4 f = *reinterpret_cast<const float4 *>(&ctl.scales[s][col0 + c + j]);
+                        acc[c + j] = fmaf(f.x, __uint_as_float(v[j]), acc[c + j]);
+                        acc[c + j + 1] = fmaf(f.y, __uint_as_float(v[j + 1]), acc[c + j + 1]);
+                        acc[c + j + 2] = fmaf(f.z, __uint_as_float(v[j + 2]), acc[c + j + 2]);
+                        acc[c + j + 3] = fmaf(f.w, __uint_as_float(v[j + 3]), acc[c + j + 3]);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctl.acc_empty[b]), mbar_arrive(&ctl.sc_empty[s]);
+            }
+            if (!ok) break;
+            if (a.split > 1) {
+                // the sums go to this CTA's own shared memory (its stages are spent: every block's MMAs have completed)
+                float *red = reinterpret_cast<float *>(base);
+#pragma unroll
+                for (int j = 0; j < C::Cols; ++j)
+                    if (col0 + j < t.n) red[(col0 + j) * kTileM + r] = acc[j];
+            } else if (t.n0 + r < a.N) {
+#pragma unroll
+                for (int j = 0; j < C::Cols; ++j) {
+                    if (col0 + j < t.n) {
+                        int64_t row = t.first + col0 + j;
+                        if constexpr (GROUPED) row = rt.slots[row];
+                        const int64_t o = row * a.N + t.n0 + r;
+                        if (a.out_f32) static_cast<float *>(a.y)[o] = acc[j];
+                        else static_cast<uint16_t *>(a.y)[o] = f32_to_bf16_bits(acc[j]);
+                    }
+                }
+            }
+        }
+    }
+
+    if (a.split > 1) {  // the grid has at most one pair per cluster
+        __syncwarp();
+        cluster_sync();
+        if (warp < C::PromoWarps && first_pair < n_pairs) {
+            const Pair t = pair_of(first_pair);
+            const int r = (warp & 3) * 32 + lane;
+            const uint32_t red = smem_u32(base);
+            for (int j = rank + (warp / 4) * a.split; j < t.n; j += a.split * (C::PromoWarps / 4)) {
+                float v = 0.f;
+                for (int q = 0; q < a.split; ++q) v += ld_peer(red + (uint32_t)(j * kTileM + r) * 4, q);
+                if (t.n0 + r < a.N) {
+                    int64_t row = t.first + j;
+                    if constexpr (GROUPED) row = rt.slots[row];
+                    const int64_t o = row * a.N + t.n0 + r;
+                    if (a.out_f32) static_cast<float *>(a.y)[o] = v;
+                    else static_cast<uint16_t *>(a.y)[o] = f32_to_bf16_bits(v);
+                }
+            }
+        }
+        __syncwarp();
+        cluster_sync();  // nobody's shared memory goes while a peer reads it
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (tid == 0 && ctl.abort_flag) atomicAdd(&g_fp8_aborts, 1u);
+    if (warp == kMmaWarp)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)C::TmemCols) : "memory");
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                              const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+int encoder(const char *fn, EncodeFn *out) {
+    static std::mutex mu;
+    static EncodeFn cached = nullptr;
+    std::lock_guard<std::mutex> lock(mu);
+    if (cached == nullptr) {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        SB_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q), fn, ": looking up the tensor-map encoder");
+        SB_CHECK(q == cudaDriverEntryPointSuccess && p != nullptr, fn, ": the driver has no tensor-map encoder");
+        cached = reinterpret_cast<EncodeFn>(p);
+    }
+    *out = cached;
+    return 0;
+}
+
+// rows x K bytes, boxes of box_rows x 128 bytes (128-byte swizzle); bytes beyond K and rows beyond the end read as zero.
+int make_map(const char *fn, CUtensorMap *m, const uint8_t *ptr, int64_t rows, int64_t K, int box_rows) {
+    EncodeFn enc;
+    SB_TRY(encoder(fn, &enc));
+    const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)K};
+    const cuuint32_t box[2] = {(cuuint32_t)kBK, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    const CUresult rc = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    SB_CHECK(rc == CUDA_SUCCESS, fn, ": cuTensorMapEncodeTiled failed with ", (int)rc, " for a [", rows, ", ", K, "] byte matrix");
+    return 0;
+}
+
+template <int TOK, bool GROUPED>
+int launch(const char *fn, const uint8_t *w, int64_t w_rows, const uint8_t *x, int64_t x_rows, int64_t K, GemmArgs a, int64_t most_tiles, cudaStream_t st) {
+    static thread_local int prepared = -1;
+    constexpr size_t smem = smem_bytes<TOK>();
+    int dev = 0;
+    SB_CUDA(cudaGetDevice(&dev), fn);
+    if (prepared != dev) {
+        SB_CUDA(cudaFuncSetAttribute(fp8_gemm_kernel<TOK, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), fn);
+        prepared = dev;
+    }
+    CUtensorMap wm, xm;
+    SB_TRY(make_map(fn, &wm, w, w_rows, K, kTileM));
+    SB_TRY(make_map(fn, &xm, x, x_rows, K, GROUPED ? 1 : TOK));
+    const int64_t pairs = most_tiles * a.NT, sms = sm_count();
+    a.split = 1;
+    while (a.split < kMaxSplit && a.split * 2 <= a.KB && pairs * a.split * 2 <= sms) a.split *= 2;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(a.split > 1 ? pairs * a.split : std::min(pairs, sms)));
+    cfg.blockDim = dim3(Cfg<TOK>::Threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)a.split, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr, cfg.numAttrs = 1;
+    SB_CUDA((cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<TOK, GROUPED>, wm, xm, a)), fn, " (", TOK, " columns, split ", a.split, ") N=", a.N, " K=", K);
+    return 0;
+}
+
+int check_view(const char *fn, const strix_fp8view *w) {
+    SB_CHECK(w != nullptr && w->q != nullptr && w->scale != nullptr, fn, ": null weight view, codes or scales");
+    SB_CHECK(w->N >= 1 && w->N <= 0x7fffff80 && w->K >= 16 && w->K <= (1 << 24) && w->K % 16 == 0, fn, ": weight [", w->N, ", ", w->K,
+             "], expected N 1..2^31-128 and K a multiple of 16 up to 2^24");
+    SB_CHECK(aligned16(w->q) && reinterpret_cast<uintptr_t>(w->scale) % 4 == 0, fn, ": weight codes ", (const void *)w->q,
+             " must be 16-byte aligned, scales 4-byte");
+    return 0;
+}
+
+int check_rows(const char *fn, const uint8_t *xq, const float *xs, int64_t rows, int64_t K, const void *y, int64_t y_bytes, int out_act) {
+    SB_CHECK(xq != nullptr && xs != nullptr && y != nullptr, fn, ": null pointer (xq=", (const void *)xq, ", xs=", (const void *)xs, ", y=", y, ")");
+    SB_CHECK(aligned16(xq) && reinterpret_cast<uintptr_t>(xs) % 4 == 0 && reinterpret_cast<uintptr_t>(y) % 4 == 0, fn, ": xq ", (const void *)xq,
+             " must be 16-byte aligned, xs and y 4-byte");
+    SB_CHECK(act_ok(out_act), fn, ": unsupported output dtype ", out_act);
+    SB_CHECK(apart(y, y_bytes, xq, rows * K) && apart(y, y_bytes, xs, rows * fp8_blocks(K) * 4), fn, ": output [", y, ", +", y_bytes,
+             " B) overlaps the rows [", (const void *)xq, "] or their scales [", (const void *)xs, "]");
+    return 0;
+}
+
+int grouped(const char *fn, const uint8_t *xq, const float *xs, const strix_fp8view *w, int64_t E, const void *ws, size_t ws_bytes, int64_t M, int64_t A,
+            int64_t rows, void *y, int out_act, cudaStream_t st) {
+    SB_TRY(check_view(fn, w));
+    SB_CHECK(M >= 1 && A >= 1 && A <= 64 && M <= (1 << 20) && M * A <= (1 << 20), fn, ": M = ", M, ", A = ", A, " (A <= 64, M * A <= 2^20)");
+    SB_CHECK(E >= 1 && E <= kMaxE && w->N % E == 0, fn, ": weight has ", w->N, " rows for E = ", E, " experts (E must be 1..1023 and divide the rows)");
+    SB_CHECK(ws != nullptr && reinterpret_cast<uintptr_t>(ws) % 4 == 0, fn, ": null or unaligned workspace");
+    const size_t need = strix_moe_route_workspace_bytes(M, A, E);
+    SB_CHECK(need != 0 && ws_bytes >= need, fn, ": workspace of ", ws_bytes, " bytes, needs ", need, " for M = ", M, ", A = ", A, ", E = ", E);
+    const int64_t N = w->N / E, S = M * A;
+    SB_TRY(check_rows(fn, xq, xs, rows, w->K, y, S * N * act_size(out_act), out_act));
+    SB_CHECK(apart(y, S * N * act_size(out_act), ws, (int64_t)need), fn, ": output overlaps the workspace");
+    GemmArgs a{};
+    a.xs = xs, a.ws = w->scale, a.group = static_cast<const int32_t *>(ws), a.y = y, a.out_f32 = out_act == kF32;
+    a.M = (int)M, a.N = (int)N, a.KB = (int)fp8_blocks(w->K), a.NB = (int)fp8_blocks(N), a.E = (int)E, a.div = (int)(rows == S ? 1 : A), a.S = S;
+    a.NT = (int)((N + kTileM - 1) / kTileM);
+    const int64_t mean = (S + E - 1) / E;
+    auto tiles = [&](int64_t tok) { return std::min(S, E + S / tok); };  // at most: every bucket may end in a partial tile
+    SB_CHECK(tiles(16) <= 0x7fffffff / a.NT, fn, ": ", S, " slots of N = ", N, " outputs are too many tiles");
+    if (mean <= 8) return launch<16, true>(fn, w->q, w->N, xq, rows, w->K, a, tiles(16), st);
+    if (mean <= 16) return launch<32, true>(fn, w->q, w->N, xq, rows, w->K, a, tiles(32), st);
+    if (mean <= 40) return launch<64, true>(fn, w->q, w->N, xq, rows, w->K, a, tiles(64), st);
+    return launch<128, true>(fn, w->q, w->N, xq, rows, w->K, a, tiles(128), st);
+}
+
+}  // namespace
+
+namespace sb {
+
+unsigned int fp8_aborts() {
+    unsigned int v = 0;
+    cudaMemcpyFromSymbol(&v, g_fp8_aborts, sizeof(v));
+    return v;
+}
+unsigned int fp8_ws_refusals() {
+    unsigned int v = 0;
+    cudaMemcpyFromSymbol(&v, g_fp8_refusals, sizeof(v));
+    return v;
+}
+
+}  // namespace sb
+
+extern "C" {
+
+int strix_linear_fp8(const uint8_t *xq, const float *xs, const strix_fp8view *w, void *y, int64_t M, int out_act, void *stream) {
+    const char *fn = "linear_fp8";
+    SB_TRY(check_view(fn, w));
+    SB_CHECK(M >= 1 && M <= 0x7fffff00, fn, ": M = ", M, " rows, expected 1..2^31-256");
+    SB_TRY(check_rows(fn, xq, xs, M, w->K, y, M * w->N * act_size(out_act), out_act));
+    GemmArgs a{};
+    a.xs = xs, a.ws = w->scale, a.y = y, a.out_f32 = out_act == kF32;
+    a.M = (int)M, a.N = (int)w->N, a.KB = (int)fp8_blocks(w->K), a.NB = (int)fp8_blocks(w->N), a.E = 1, a.div = 1, a.S = M;
+    a.NT = (int)((w->N + kTileM - 1) / kTileM);
+    auto st = static_cast<cudaStream_t>(stream);
+    auto tiles = [&](int64_t tok) { return (M + tok - 1) / tok; };
+    SB_CHECK(tiles(16) <= 0x7fffffff / a.NT, fn, ": M = ", M, " rows of N = ", w->N, " outputs are too many tiles");
+    if (M <= 16) return launch<16, false>(fn, w->q, w->N, xq, M, w->K, a, tiles(16), st);
+    if (M <= 32) return launch<32, false>(fn, w->q, w->N, xq, M, w->K, a, tiles(32), st);
+    if (M <= 64) return launch<64, false>(fn, w->q, w->N, xq, M, w->K, a, tiles(64), st);
+    if (M <= 128) return launch<128, false>(fn, w->q, w->N, xq, M, w->K, a, tiles(128), st);
+    return launch<256, false>(fn, w->q, w->N, xq, M, w->K, a, tiles(256), st);
+}
+
+int strix_linear_fp8_experts_gather_grouped(const uint8_t *xq, const float *xs, const strix_fp8view *w, int64_t E, const void *ws, size_t ws_bytes,
+                                            int64_t M, int64_t A, void *y, int out_act, void *stream) {
+    return grouped("linear_fp8_experts_gather_grouped", xq, xs, w, E, ws, ws_bytes, M, A, M, y, out_act, static_cast<cudaStream_t>(stream));
+}
+
+int strix_linear_fp8_experts_combine_grouped(const uint8_t *hq, const float *hs, const strix_fp8view *w, int64_t E, const int32_t *ids, const float *coef,
+                                             const void *ws, size_t ws_bytes, float *partial, int64_t M, int64_t A, void *y, int act, void *stream) {
+    const char *fn = "linear_fp8_experts_combine_grouped";
+    SB_CHECK(ids != nullptr && coef != nullptr && y != nullptr, fn, ": null pointer (ids=", (const void *)ids, ", coef=", (const void *)coef, ", y=", y, ")");
+    SB_CHECK(act_ok(act), fn, ": unsupported activation dtype ", act);
+    SB_CHECK(M >= 1 && A >= 1 && A <= 64 && M <= (1 << 20) && M * A <= (1 << 20), fn, ": M = ", M, ", A = ", A, " (A <= 64, M * A <= 2^20)");
+    SB_CHECK(w != nullptr && E >= 1 && E <= kMaxE && w->N >= 1 && w->N % E == 0, fn, ": null weight view, or its rows are not those of E = ", E, " experts (1..1023)");
+    const int64_t N = w->N / E, yb = M * N * act_size(act), pb = M * A * N * 4;
+    SB_CHECK(partial != nullptr && apart(y, yb, partial, pb), fn, ": null partial, or it overlaps y");
+    SB_CHECK(apart(y, yb, ids, M * A * 4) && apart(y, yb, coef, M * A * 4) && apart(partial, pb, ids, M * A * 4) && apart(partial, pb, coef, M * A * 4), fn,
+             ": y or partial overlaps ids or coef");
+    SB_CHECK(ws == nullptr || apart(y, yb, ws, (int64_t)ws_bytes), fn, ": y overlaps the workspace");
+    SB_CHECK(hq == nullptr || hs == nullptr || (apart(y, yb, hq, M * A * w->K) && apart(y, yb, hs, M * A * fp8_blocks(w->K) * 4)), fn,
+             ": y overlaps the rows or their scales");
+    auto st = static_cast<cudaStream_t>(stream);
+    SB_TRY(grouped(fn, hq, hs, w, E, ws, ws_bytes, M, A, M * A, partial, kF32, st));
+    return sb::combine_reduce(fn, partial, ids, coef, M, A, E, N, y, act, st);
+}
+
+}  // extern "C"

@@ -554,9 +554,9 @@ extern "C" {
 unsigned int strix_workspace_refusal_count(void) {
     unsigned int v = 0;
     cudaMemcpyFromSymbol(&v, g_ws_refusals, sizeof(v));
-    return v + sb::grouped_umma_ws_refusals() + sb::prefill_ws_refusals();
+    return v + sb::grouped_umma_ws_refusals() + sb::prefill_ws_refusals() + sb::fp8_ws_refusals();
 }
-unsigned int strix_umma_abort_count(void) { return sb::grouped_umma_aborts() + sb::prefill_aborts(); }
+unsigned int strix_umma_abort_count(void) { return sb::grouped_umma_aborts() + sb::prefill_aborts() + sb::fp8_aborts(); }
 void strix_umma_wait_cycles(unsigned long long *out32, int reset) { sb::prefill_cycles(out32, reset != 0); }
 
 size_t strix_moe_route_workspace_bytes(int64_t M, int64_t A, int64_t E) {

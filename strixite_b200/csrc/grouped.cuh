@@ -49,6 +49,10 @@ int dense_umma(const char *fn, const void *x, const StackView &w, int64_t M, voi
 // Launches refused because the workspace was grouped for other sizes than the call states (0 in a healthy run).
 unsigned int grouped_umma_ws_refusals();
 
+// The same two counts of the FP8 products (fp8_gemm.cu).
+unsigned int fp8_ws_refusals();
+unsigned int fp8_aborts();
+
 // CTAs of the tensor-core grouped GEMM that gave up on a bounded wait since the library was loaded (0 in a healthy run).
 unsigned int grouped_umma_aborts();
 

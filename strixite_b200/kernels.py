@@ -12,7 +12,7 @@ import enum
 import numpy as np
 import torch
 
-from ._lib import QMixView, QView, StrixError, call, lib  # noqa: F401
+from ._lib import Fp8View, QMixView, QView, StrixError, call, lib  # noqa: F401
 
 
 class Act(enum.IntEnum):  # strixite kernels/norm.hpp:20
@@ -501,3 +501,143 @@ def linear_qw_experts_combine_grouped(h, w, E, ids, coef, ws, ws_bytes, partial,
     """strixite runtime/qweight.hpp:113-125."""
     _combine_grouped(_expert_bits("linear_qw_experts_combine_grouped", w), h, w.w, E, ids, coef, ws, ws_bytes, partial, M, A, y, act, math,
                      stream)
+
+
+# ---- 8-bit floating point (e4m3, a scale per block of 128) ------------------------------------------------------------
+# No counterpart in the reference. These wrappers look at dtype, size and device of every tensor, because a byte matrix of the wrong
+# shape has no other sign of it; a tensor of another device than the current one is refused (the launch goes to the current one).
+
+
+class Score(enum.IntEnum):
+    Softmax = 0
+    Sigmoid = 1
+
+
+_SCORES = {"softmax": 0, "sigmoid": 1, 0: 0, 1: 1}
+FP8_BLOCK = 128
+
+
+def fp8_blocks(n):
+    """Scale blocks along a dimension of n."""
+    return -(-n // FP8_BLOCK)
+
+
+def _t(fn, name, t, dtypes, n, optional=False):
+    """The address of a contiguous tensor of one of `dtypes` with at least n elements on the current device."""
+    if t is None:
+        if optional:
+            return None
+        raise StrixError("%s: %s is None" % (fn, name))
+    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+        raise StrixError("%s: %s is on %s, expected the current device cuda:%d" % (fn, name, t.device, torch.cuda.current_device()))
+    if t.dtype not in dtypes:
+        raise StrixError("%s: %s is %s, expected %s" % (fn, name, t.dtype, " or ".join(str(d) for d in dtypes)))
+    if t.numel() < n or not t.is_contiguous():
+        raise StrixError("%s: %s has %s elements%s, expected %d contiguous" % (fn, name, t.numel(), "" if t.is_contiguous() else " (not contiguous)", n))
+    return t.data_ptr()
+
+
+_F8, _F32, _I32 = (torch.float8_e4m3fn, torch.uint8), (torch.float32,), (torch.int32,)
+_ACTS = {0: (torch.float32,), 1: (torch.bfloat16,)}
+
+
+def _act_dtypes(fn, act):
+    if int(act) not in _ACTS:
+        raise StrixError("%s: unsupported activation dtype %r" % (fn, act))
+    return _ACTS[int(act)]
+
+
+class Fp8Weight:
+    """An e4m3 matrix [N, K] with an FP32 scale per 128 x 128 block (strix_fp8view), or a stack of `experts` such matrices of N / experts
+    rows each: q float8_e4m3fn (or its bytes) [N, K], scale [experts * blocks(N / experts), blocks(K)] - the arrays of an FP8 checkpoint as
+    they are."""
+
+    def __init__(self, q, scale, experts=1):
+        if q.dim() != 2 or q.dtype not in _F8 or not q.is_contiguous():
+            raise StrixError("Fp8Weight: q must be a contiguous [N, K] tensor of float8_e4m3fn or uint8, got %s %s" % (tuple(q.shape), q.dtype))
+        self.N, self.K, self.experts = int(q.shape[0]), int(q.shape[1]), int(experts)
+        if self.experts < 1 or self.N % self.experts:
+            raise StrixError("Fp8Weight: %d rows for %d experts" % (self.N, self.experts))
+        want = (self.experts * fp8_blocks(self.N // self.experts), fp8_blocks(self.K))
+        if tuple(scale.shape) != want or scale.dtype != torch.float32 or not scale.is_contiguous():
+            raise StrixError("Fp8Weight: scale must be a contiguous float32 %s tensor, got %s %s" % (want, tuple(scale.shape), scale.dtype))
+        if q.device != scale.device:
+            raise StrixError("Fp8Weight: q is on %s, scale on %s" % (q.device, scale.device))
+        self.q, self.scale = q, scale
+        self._view = Fp8View(q.data_ptr(), scale.data_ptr(), self.N, self.K)
+
+    def view(self):
+        return self._view
+
+    def nbytes(self):
+        return self.q.numel() + 4 * self.scale.numel()
+
+
+def _fp8w(fn, w, experts):
+    if not isinstance(w, Fp8Weight):
+        raise StrixError("%s: expected an Fp8Weight, got %s" % (fn, type(w).__name__))
+    if w.experts != experts:
+        raise StrixError("%s: the weight holds %d experts, the call states %d" % (fn, w.experts, experts))
+    _t(fn, "the weight", w.q, _F8, w.N * w.K)
+    return C.byref(w._view)
+
+
+def moe_router_scored(logits, ld, M, E, k, score, bias, n_group, topk_group, group_top, renorm, route_scale, shared_logit, shared_ld, shared_id, ids, coef, act,
+                      err, stream=None):
+    """Score-based routing: `score` 'softmax' or 'sigmoid' (or Score), an optional balance bias [E] for the choice, n_group groups of which
+    topk_group stay open (a group's value: its group_top = 1 or 2 largest), k picks, weights renormalised when `renorm`, times route_scale.
+    logits: a tensor whose first element is token 0's first logit, rows ld apart; shared_logit as in moe_router."""
+    fn = "moe_router_scored"
+    if score not in _SCORES:
+        raise StrixError("%s: score %r, expected 'softmax' or 'sigmoid'" % (fn, score))
+    dt = _act_dtypes(fn, act)
+    A = k + (0 if shared_logit is None else 1)
+    for name, t in (("logits", logits), ("shared_logit", shared_logit)):  # views into rows of stride ld
+        if t is not None and (not t.is_cuda or t.device.index != torch.cuda.current_device() or t.dtype not in dt):
+            raise StrixError("%s: %s must be %s on the current device, got %s on %s" % (fn, name, dt[0], t.dtype, t.device))
+    call("strix_moe_router_scored", logits.data_ptr(), ld, M, E, k, _SCORES[score], _t(fn, "bias", bias, _F32, E, True), n_group, topk_group, group_top, int(bool(renorm)),
+         float(route_scale), None if shared_logit is None else shared_logit.data_ptr(), shared_ld, shared_id, _t(fn, "ids", ids, _I32, M * A),
+         _t(fn, "coef", coef, _F32, M * A), int(act), _t(fn, "err", err, _I32, 3), _s(stream))
+
+
+def residual_rmsnorm_fp8(x, y, w, M, d, eps, x_out, h, q, scale, act, centered=False, stream=None):
+    """x_out = x + y (both None: x alone; x_out may be x or y), h = RMSnorm(x_out) * (w, or 1 + w when centered), q / scale: h as FP8 rows.
+    h, or q and scale, may be None."""
+    fn = "residual_rmsnorm_fp8"
+    dt, n = _act_dtypes(fn, act), M * d
+    call("strix_residual_rmsnorm_fp8", _t(fn, "x", x, dt, n), _t(fn, "y", y, dt, n, True), _t(fn, "w", w, _F32, d), int(bool(centered)), float(eps), M, d,
+         _t(fn, "x_out", x_out, dt, n, True), _t(fn, "h", h, dt, n, True), _t(fn, "q", q, _F8, n, True),
+         _t(fn, "scale", scale, _F32, M * fp8_blocks(d), True), int(act), _s(stream))
+
+
+def swiglu_fp8(gu, q, scale, rows, I, act, stream=None):
+    """swiglu of merged [gate | up] rows [rows, 2I] with the result as FP8 rows q [rows, I], scale [rows, blocks(I)]."""
+    fn = "swiglu_fp8"
+    call("strix_swiglu_fp8", _t(fn, "gu", gu, _act_dtypes(fn, act), rows * 2 * I), _t(fn, "q", q, _F8, rows * I), _t(fn, "scale", scale, _F32, rows * fp8_blocks(I)), rows, I,
+         int(act), _s(stream))
+
+
+def linear_fp8(xq, xs, w, y, M, out_act, stream=None):
+    """y[M, N] = the FP8 rows (xq [M, K], xs [M, blocks(K)]) times an Fp8Weight [N, K] transposed, FP32 or BF16."""
+    fn = "linear_fp8"
+    v = _fp8w(fn, w, 1)
+    call("strix_linear_fp8", _t(fn, "xq", xq, _F8, M * w.K), _t(fn, "xs", xs, _F32, M * fp8_blocks(w.K)), v, _t(fn, "y", y, _act_dtypes(fn, out_act), M * w.N), M,
+         int(out_act), _s(stream))
+
+
+def linear_fp8_experts_gather_grouped(xq, xs, w, E, ws, ws_bytes, M, A, y, out_act, stream=None):
+    """y[slot, :] = expert ids[slot] of the stack times FP8 row slot / A, over the workspace of moe_group_routes(ids, M, A, E, ...)."""
+    fn = "linear_fp8_experts_gather_grouped"
+    v = _fp8w(fn, w, E)
+    call("strix_linear_fp8_experts_gather_grouped", _t(fn, "xq", xq, _F8, M * w.K), _t(fn, "xs", xs, _F32, M * fp8_blocks(w.K)), v, E,
+         _t(fn, "ws", ws, (ws.dtype,), -(-ws_bytes // ws.element_size())), ws_bytes, M, A, _t(fn, "y", y, _act_dtypes(fn, out_act), M * A * (w.N // E)), int(out_act), _s(stream))
+
+
+def linear_fp8_experts_combine_grouped(hq, hs, w, E, ids, coef, ws, ws_bytes, partial, M, A, y, act, stream=None):
+    """y[m, :] = sum over a of coef[m, a] * (expert ids[m, a] of the stack times FP8 row m * A + a); partial: M * A * N floats."""
+    fn = "linear_fp8_experts_combine_grouped"
+    v = _fp8w(fn, w, E)
+    S, N = M * A, w.N // E
+    call("strix_linear_fp8_experts_combine_grouped", _t(fn, "hq", hq, _F8, S * w.K), _t(fn, "hs", hs, _F32, S * fp8_blocks(w.K)), v, E, _t(fn, "ids", ids, _I32, S),
+         _t(fn, "coef", coef, _F32, S), _t(fn, "ws", ws, (ws.dtype,), -(-ws_bytes // ws.element_size())), ws_bytes, _t(fn, "partial", partial, _F32, S * N), M, A,
+         _t(fn, "y", y, _act_dtypes(fn, act), M * N), int(act), _s(stream))
