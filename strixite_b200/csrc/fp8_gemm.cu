@@ -20,25 +20,22 @@
 #include <algorithm>
 #include <mutex>
 
-#include "fp8.cuh"
-#include "grouped.cuh"
+#include "fp8_gemm.cuh"
 #include "prefill_umma.cuh"
 #include "strixite_b200.h"
-#include "umma.cuh"
 
 namespace {
 
 using namespace sb;
 using namespace sb::umma;
+using namespace sb::fp8;
 
 __device__ unsigned int g_fp8_aborts = 0;
 __device__ unsigned int g_fp8_refusals = 0;
 
-constexpr int kBK = 128;                  // K per stage: one scale block, one 128-byte swizzle row
 constexpr int kATile = kTileM * kBK;      // 16 KB of weights
 constexpr int kScaleSlots = 4;
 constexpr int kMaxSplit = 8;              // portable cluster size
-constexpr int kMaxE = 1023;
 
 template <int TOK>
 struct Cfg {
@@ -68,19 +65,6 @@ constexpr size_t smem_bytes() {
     return (size_t)Cfg<TOK>::Stages * Cfg<TOK>::StageBytes + sizeof(Ctl<TOK>) + 1024;
 }
 
-struct GemmArgs {
-    const float *xs, *ws;    // scales of x rows [.., KB] and of the weight blocks [(E *) NB, KB]
-    const int32_t *group;    // grouped: the workspace of moe_group_routes
-    void *y;
-    int out_f32;
-    int M, N, KB, NB;        // dense: rows of x; rows of one matrix, blocks of K, block rows of one matrix
-    int E, div;              // grouped: slot s reads row s / div
-    int64_t S;
-    int NT, split;           // weight tiles of one matrix; CTAs that share a pair's K blocks
-};
-
-// kind::f8f6f4: D = F32 (bits 4-5 = 1), A and B e4m3 (0), both K-major, N = n, M = 128.
-__device__ __forceinline__ uint32_t idesc_e4m3(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24); }
 __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -88,22 +72,6 @@ __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t da, uint64_t d
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
         ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(0u)
         : "memory");
-}
-// Four rows r0..r3 of a tensor map whose box is one row of 128 bytes, to four consecutive 128-byte rows of shared memory.
-__device__ __forceinline__ void tma_gather4(void *dst, const void *tmap, int x, int r0, int r1, int r2, int r3, uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(
-            smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(smem_u32(bar))
-        : "memory");
-}
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ float ld_peer(uint32_t addr, uint32_t rank) {
     uint32_t p;
@@ -126,7 +94,7 @@ __global__ void __launch_bounds__(Cfg<TOK>::Threads, 1)
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     Ctl<TOK> &ctl = *reinterpret_cast<Ctl<TOK> *>(base + C::Stages * C::StageBytes);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     constexpr int kTmaWarp = C::PromoWarps, kMmaWarp = kTmaWarp + 1, kScaleWarp = kTmaWarp + 2;
     if (GROUPED && !ws_is_for(a.group, a.S, a.E, &g_fp8_refusals)) return;  // the whole grid leaves
     if (tid == 0) {
@@ -143,38 +111,8 @@ __global__ void __launch_bounds__(Cfg<TOK>::Threads, 1)
     RouteTables rt{};
     int x_tiles;
     if constexpr (GROUPED) {
-        // tiles of TOK slots per bucket, as a prefix over the buckets: a thread owns kPer neighbouring ones
-        constexpr int kPer = (kMaxE + C::Threads) / C::Threads;
         rt = route_tables(a.group, a.S, a.E);
-        int nt[kPer], sum = 0;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int e = tid * kPer + i;
-            nt[i] = e < a.E ? (rt.offsets[e + 1] - rt.offsets[e] + TOK - 1) / TOK : 0;
-            sum += nt[i];
-        }
-        int incl = sum;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const int o = __shfl_up_sync(0xffffffffu, incl, off);
-            if (lane >= off) incl += o;
-        }
-        if (lane == 31) ctl.warp_tot[warp] = incl;
-        __syncthreads();
-        int before = incl - sum;
-        x_tiles = 0;
-        for (int i = 0; i < C::Threads / 32; ++i) {
-            const int t = ctl.warp_tot[i];
-            before += i < warp ? t : 0;
-            x_tiles += t;
-        }
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int e = tid * kPer + i;
-            if (e <= a.E) ctl.prefix[e] = before;
-            before += nt[i];
-        }
-        if (tid == 0) ctl.prefix[a.E] = x_tiles;
+        x_tiles = tile_prefix<TOK, C::Threads>(rt, a.E, ctl.prefix, ctl.warp_tot);
     } else {
         x_tiles = (a.M + TOK - 1) / TOK;
     }
@@ -192,12 +130,7 @@ __global__ void __launch_bounds__(Cfg<TOK>::Threads, 1)
         Pair r;
         r.n0 = nt * kTileM;
         if constexpr (GROUPED) {
-            int lo = 0, hi = a.E;  // prefix[lo] <= xt < prefix[hi]
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (ctl.prefix[mid] <= xt) lo = mid;
-                else hi = mid;
-            }
+            const int lo = bucket_of(ctl.prefix, a.E, xt);
             const int begin = rt.offsets[lo] + (xt - ctl.prefix[lo]) * TOK;
             r.wrow = lo * a.N + r.n0, r.ws_row = lo * a.NB + nt;
             r.first = begin, r.n = min(TOK, rt.offsets[lo + 1] - begin);
@@ -229,11 +162,10 @@ __global__ void __launch_bounds__(Cfg<TOK>::Threads, 1)
             }
             for (int kb = kb0; kb < kb1; ++kb, ++it) {
                 const int s = it % C::Stages;
-                if (lane == 0) ok = mbar_wait(&ctl.empty[s], ((it / C::Stages) & 1u) ^ 1u, abort_flag);
-                ok = __shfl_sync(0xffffffffu, ok, 0);
+                ok = __all_sync(0xffffffffu, mbar_wait(&ctl.empty[s], ((it / C::Stages) & 1u) ^ 1u, abort_flag));
                 if (!ok) break;
                 uint8_t *dst = base + s * C::StageBytes;
-                if (lane == 0) {
+                if (elect_one()) {
                     mbar_expect_tx(&ctl.full[s], bytes);
                     tma_load_2d(dst, &w_map, kb * kBK, t.wrow, &ctl.full[s]);
                     if constexpr (!GROUPED) tma_load_2d(dst + kATile, &x_map, kb * kBK, t.first, &ctl.full[s]);
@@ -249,7 +181,9 @@ __global__ void __launch_bounds__(Cfg<TOK>::Threads, 1)
                 }
             }
         }
-        if (!ok && lane == 0) {  // abandoned: the copies in flight land before the shared memory goes
+        // The last blocks' MMAs have read their stages and signalled it; after an abandoned wait, the copies in flight have landed.
+        for (uint32_t i = it > C::Stages ? it - C::Stages : 0; i < it && ok; ++i) ok = __all_sync(0xffffffffu, mbar_wait(&ctl.empty[i % C::Stages], (i / C::Stages) & 1u, abort_flag));
+        if (!ok && lane == 0) {
             for (uint32_t i = it > C::Stages ? it - C::Stages : 0; i < it; ++i)
                 for (uint32_t n = 0; n < kSpinLimit && !mbar_try_wait(&ctl.full[i % C::Stages], (i / C::Stages) & 1u); ++n) {
                 }
@@ -260,7 +194,7 @@ __global__ void __launch_bounds__(Cfg<TOK>::Threads, 1)
         bool ok = true;
         for (int p = first_pair; p < n_pairs && ok; p += pair_step) {
             const Pair t = pair_of(p);
-            const uint32_t idesc = idesc_e4m3((t.n + 15) & ~15);
+            const uint32_t idesc = idesc_e4m3(kTileM, (t.n + 15) & ~15);
             for (int kb = kb0; kb < kb1; ++kb, ++it) {
                 const int s = it % C::Stages, b = it % C::NBuf;
                 ok = mbar_wait(&ctl.acc_empty[b], ((it / C::NBuf) & 1u) ^ 1u, abort_flag) && mbar_wait(&ctl.full[s], (it / C::Stages) & 1u, abort_flag);
@@ -269,7 +203,7 @@ __global__ void __launch_bounds__(Cfg<TOK>::Threads, 1)
                     break;
                 }
                 tc_fence_after();
-                if (lane == 0) {
+                if (elect_one()) {
                     const uint32_t at = smem_u32(base + s * C::StageBytes);
                     const uint64_t da = umma_desc(at), db = umma_desc(at + kATile);
 #pragma unroll
@@ -416,12 +350,15 @@ __global__ void __launch_bounds__(Cfg<TOK>::Threads, 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)C::TmemCols) : "memory");
 }
 
-// ---- host ------------------------------------------------------------------------------------------------------------
+}  // namespace
+
+namespace sb {
+namespace fp8 {
 
 using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                               const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-int encoder(const char *fn, EncodeFn *out) {
+static int encoder(const char *fn, EncodeFn *out) {
     static std::mutex mu;
     static EncodeFn cached = nullptr;
     std::lock_guard<std::mutex> lock(mu);
@@ -447,6 +384,13 @@ int make_map(const char *fn, CUtensorMap *m, const uint8_t *ptr, int64_t rows, i
     SB_CHECK(rc == CUDA_SUCCESS, fn, ": cuTensorMapEncodeTiled failed with ", (int)rc, " for a [", rows, ", ", K, "] byte matrix");
     return 0;
 }
+
+}  // namespace fp8
+}  // namespace sb
+
+namespace {
+
+// ---- host ------------------------------------------------------------------------------------------------------------
 
 template <int TOK, bool GROUPED>
 int launch(const char *fn, const uint8_t *w, int64_t w_rows, const uint8_t *x, int64_t x_rows, int64_t K, GemmArgs a, int64_t most_tiles, cudaStream_t st) {
@@ -517,7 +461,7 @@ int grouped(const char *fn, const uint8_t *xq, const float *xs, const strix_fp8v
     if (mean <= 8) return launch<16, true>(fn, w->q, w->N, xq, rows, w->K, a, tiles(16), st);
     if (mean <= 16) return launch<32, true>(fn, w->q, w->N, xq, rows, w->K, a, tiles(32), st);
     if (mean <= 40) return launch<64, true>(fn, w->q, w->N, xq, rows, w->K, a, tiles(64), st);
-    return launch<128, true>(fn, w->q, w->N, xq, rows, w->K, a, tiles(128), st);
+    return wide_grouped(fn, w->q, w->N, xq, rows, w->K, a, st);
 }
 
 }  // namespace
@@ -527,12 +471,12 @@ namespace sb {
 unsigned int fp8_aborts() {
     unsigned int v = 0;
     cudaMemcpyFromSymbol(&v, g_fp8_aborts, sizeof(v));
-    return v;
+    return v + fp8::wide_aborts();
 }
 unsigned int fp8_ws_refusals() {
     unsigned int v = 0;
     cudaMemcpyFromSymbol(&v, g_fp8_refusals, sizeof(v));
-    return v;
+    return v + fp8::wide_ws_refusals();
 }
 
 }  // namespace sb
@@ -554,8 +498,7 @@ int strix_linear_fp8(const uint8_t *xq, const float *xs, const strix_fp8view *w,
     if (M <= 16) return launch<16, false>(fn, w->q, w->N, xq, M, w->K, a, tiles(16), st);
     if (M <= 32) return launch<32, false>(fn, w->q, w->N, xq, M, w->K, a, tiles(32), st);
     if (M <= 64) return launch<64, false>(fn, w->q, w->N, xq, M, w->K, a, tiles(64), st);
-    if (M <= 128) return launch<128, false>(fn, w->q, w->N, xq, M, w->K, a, tiles(128), st);
-    return launch<256, false>(fn, w->q, w->N, xq, M, w->K, a, tiles(256), st);
+    return wide_dense(fn, w->q, w->N, xq, M, w->K, a, st);
 }
 
 int strix_linear_fp8_experts_gather_grouped(const uint8_t *xq, const float *xs, const strix_fp8view *w, int64_t E, const void *ws, size_t ws_bytes,

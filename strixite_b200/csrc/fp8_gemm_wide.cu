@@ -1,0 +1,424 @@
+// The FP8 products for many rows: y[r, n] = sum_kb (xs[r, kb] * ws[n / 128, kb]) * (block sum of xq * wq), as in fp8_gemm.cu, with the rows
+// of x on the accumulator's lanes and 256 weight rows as its columns.
+//
+// A thread that takes block sums out of tensor memory holds ONE row of x and 128 columns that share a weight block, so the scale of a
+// whole block is one number per thread: the promotion is one packed FMA for two columns and nothing else. (With weight rows on the lanes
+// each column has its own scale: a shared-memory load for four columns, and a warp that prepares them; at 4096^3 that took 162 us.)
+//
+// GROUP = 2 (dense): a cluster of two CTAs works on 256 rows x 256 columns with cta_group::2 instructions. Each CTA loads its 128 rows of
+// x and half of the weight rows, 32 KB a block of K instead of 48: the feed from L2 (about 58 bytes a clock and SM, measured) is what
+// bounds the one-CTA form. GROUP = 1 (the experts' slots, gathered by row): an expert has seldom more than 128 rows.
+//
+// Roles: warps 0-3 / 4-7 promote column half 0 / 1 (each half has two accumulators, so the tensor cores run up to three half blocks
+// ahead), warp 8 issues TMA, warp 9 issues the MMAs (of CTA 0 for both CTAs). The sums leave through a 64-byte-wide staging strip per warp so that a
+// store covers whole sectors of a row.
+// Every mbarrier wait is bounded: on expiry the CTA raises the abort counter, waits for its copies, frees its tensor memory, returns.
+#include <algorithm>
+
+#include "fp8_gemm.cuh"
+
+namespace {
+
+using namespace sb;
+using namespace sb::fp8;
+
+__device__ unsigned int g_wide_aborts = 0;
+__device__ unsigned int g_wide_refusals = 0;
+
+constexpr int kRows = 128;               // rows of x per CTA = accumulator lanes
+constexpr int kColTile = 256;            // weight rows per tile
+constexpr int kHalf = 128;               // columns of a promotion warpgroup: one block row of weight scales
+constexpr int kPromoWarps = 8;
+constexpr int kTmaWarp = 8, kMmaWarp = 9;
+constexpr int kThreads = 12 * 32;        // three warpgroups; two warps of the last one are idle
+constexpr int kStripPitch = 80;          // 64 bytes of a row + 16: rows start in different banks
+constexpr int kStrip = 32 * kStripPitch;
+
+template <int GROUP>
+struct Cfg {
+    static constexpr int ATile = kRows * kBK, BTile = kColTile / GROUP * kBK;  // per CTA and block of K
+    static constexpr int StageBytes = ATile + BTile;
+    static constexpr int Stages = GROUP == 2 ? 6 : 4;
+};
+
+template <int GROUP>
+struct Ctl {
+    uint64_t full[Cfg<GROUP>::Stages], empty[Cfg<GROUP>::Stages], acc_full[2][2], acc_empty[2][2];  // [half][buffer]
+    uint32_t tmem_base;
+    int abort_flag;
+    int warp_tot[32];
+    int prefix[kMaxE + 1 + 1];  // grouped: first tile of each bucket
+};
+
+template <int GROUP>
+constexpr size_t smem_bytes() {
+    return (size_t)Cfg<GROUP>::Stages * Cfg<GROUP>::StageBytes + kPromoWarps * kStrip + sizeof(Ctl<GROUP>) + 1024;
+}
+
+template <int GROUP>
+__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (GROUP == 1) {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+            : "memory");
+    }
+}
+// Arrival on `bar` of this CTA (GROUP 1) or of both CTAs (GROUP 2) when the MMAs issued so far have completed.
+template <int GROUP>
+__device__ __forceinline__ void commit(uint64_t *bar) {
+    if constexpr (GROUP == 1) umma_commit(bar);
+    else
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3)
+                     : "memory");
+}
+// A box into this CTA's shared memory, counted on the barrier at cluster address `bar` (the leader's).
+__device__ __forceinline__ void tma_load_pair(void *dst, const void *tmap, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+                 "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(bar)
+                 : "memory");
+}
+// An arrival on a barrier of the pair. What it hands over is tensor memory, ordered by the tcgen05 fence in front of it; a release at
+// cluster scope would wait for the scale loads in flight as well (1700 clocks a block of K, measured).
+__device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+// (a.x, a.y) += (s, s) * (v0, v1): one instruction, each lane of it an FP32 FMA.
+__device__ __forceinline__ void fma2(float2 &a, float s, uint32_t v0, uint32_t v1) {
+    asm("{\n\t.reg .b64 x, y, z;\n\t"
+        "mov.b64 x, {%2, %2};\n\t"
+        "mov.b64 y, {%3, %4};\n\t"
+        "mov.b64 z, {%0, %1};\n\t"
+        "fma.rn.f32x2 z, x, y, z;\n\t"
+        "mov.b64 {%0, %1}, z;\n\t}"
+        : "+f"(a.x), "+f"(a.y)
+        : "f"(s), "r"(v0), "r"(v1));
+}
+__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// A tile: its first row of the weight stack, first weight row and block row inside its matrix, halves with weight rows in them, and this
+// CTA's rows - dense: rows first .. of x; grouped: the slots list[first .. first + n).
+struct Tile {
+    int wrow, n0, ws_row, halves, first, n;
+};
+
+template <int GROUP, bool GROUPED>
+__global__ void __launch_bounds__(kThreads, 1)
+    fp8_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const GemmArgs a) {
+    using C = Cfg<GROUP>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t *strips = base + C::Stages * C::StageBytes;
+    Ctl<GROUP> &ctl = *reinterpret_cast<Ctl<GROUP> *>(strips + kPromoWarps * kStrip);
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    if (GROUPED && !ws_is_for(a.group, a.S, a.E, &g_wide_refusals)) return;  // the whole grid leaves
+    const uint32_t rank = GROUP == 2 ? cluster_rank() : 0;
+    if (tid == 0) {
+        for (int i = 0; i < C::Stages; ++i) mbar_init(&ctl.full[i], 1), mbar_init(&ctl.empty[i], 1);
+        for (int i = 0; i < 4; ++i) mbar_init(&ctl.acc_full[i / 2][i % 2], 1), mbar_init(&ctl.acc_empty[i / 2][i % 2], 4 * GROUP);
+        ctl.abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMmaWarp) {
+        if constexpr (GROUP == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem_base)), "r"(512u) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem_base)), "r"(512u) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        }
+    }
+    RouteTables rt{};
+    int x_tiles;
+    if constexpr (GROUPED) {
+        rt = route_tables(a.group, a.S, a.E);
+        x_tiles = tile_prefix<kRows, kThreads>(rt, a.E, ctl.prefix, ctl.warp_tot);
+    } else {
+        x_tiles = (a.M + kRows * GROUP - 1) / (kRows * GROUP);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (GROUP == 2) cluster_sync();  // both CTAs' barriers exist before either is signalled
+    tc_fence_after();
+    const uint32_t tmem = ctl.tmem_base;
+    volatile int *abort_flag = &ctl.abort_flag;
+    const int n_tiles = x_tiles * a.NT, step = gridDim.x / GROUP;
+
+    auto tile_of = [&](int p) {  // warp-uniform
+        const int xt = p / a.NT, nt = p - xt * a.NT;
+        Tile t;
+        t.n0 = nt * kColTile;
+        t.halves = a.N - t.n0 > kHalf ? 2 : 1;
+        if constexpr (GROUPED) {
+            const int e = bucket_of(ctl.prefix, a.E, xt);
+            t.first = rt.offsets[e] + (xt - ctl.prefix[e]) * kRows;
+            t.n = min(kRows, rt.offsets[e + 1] - t.first);
+            t.wrow = e * a.N + t.n0, t.ws_row = e * a.NB + nt * 2;
+        } else {
+            t.first = (xt * GROUP + (int)rank) * kRows;
+            t.n = min(kRows, a.M - t.first);  // may be negative: the pair's second CTA beyond the end
+            t.wrow = t.n0, t.ws_row = nt * 2;
+        }
+        return t;
+    };
+
+    if (warp == kTmaWarp) {
+        uint32_t it = 0;
+        bool ok = true;
+        for (int p = blockIdx.x / GROUP; p < n_tiles && ok; p += step) {
+            const Tile t = tile_of(p);
+            int rows[4] = {0, 0, 0, 0};
+            uint32_t bytes = (uint32_t)C::StageBytes * GROUP;
+            if constexpr (GROUPED) {
+                // rows beyond the list's end repeat its last one; whole quads beyond it are not fetched, and what their lanes compute is
+                // not stored
+                for (int j = 0; j < 4; ++j) rows[j] = rt.slots[t.first + min(lane * 4 + j, t.n - 1)] / a.div;
+                bytes = C::BTile + (uint32_t)((t.n + 3) / 4) * 4 * kBK;
+            }
+            for (int kb = 0; kb < a.KB; ++kb, ++it) {
+                const int s = it % C::Stages;
+                ok = __all_sync(0xffffffffu, mbar_wait(&ctl.empty[s], ((it / C::Stages) & 1u) ^ 1u, abort_flag));
+                if (!ok) break;
+                uint8_t *dst = base + s * C::StageBytes;
+                if (elect_one()) {
+                    if constexpr (GROUP == 2) {
+                        // the leader's barrier counts both CTAs' bytes; this CTA's weight rows are the rank-th 64 of each half, so that a
+                        // half's instruction (64 rows from each CTA) covers 128 neighbouring rows
+                        if (rank == 0) mbar_expect_tx(&ctl.full[s], bytes);
+                        const uint32_t bar = peer_addr(&ctl.full[s], 0);
+                        tma_load_pair(dst, &x_map, kb * kBK, t.first, bar);
+                        tma_load_pair(dst + C::ATile, &w_map, kb * kBK, t.wrow + (int)rank * 64, bar);
+                        tma_load_pair(dst + C::ATile + 64 * kBK, &w_map, kb * kBK, t.wrow + kHalf + (int)rank * 64, bar);
+                    } else {
+                        mbar_expect_tx(&ctl.full[s], bytes);
+                        for (int i = 0; i < 4; ++i) tma_load_2d(dst + C::ATile + i * 64 * kBK, &w_map, kb * kBK, t.wrow + i * 64, &ctl.full[s]);
+                        if constexpr (!GROUPED) tma_load_2d(dst, &x_map, kb * kBK, t.first, &ctl.full[s]);
+                    }
+                }
+                __syncwarp();
+                if constexpr (GROUPED) {
+                    if (lane * 4 < t.n) tma_gather4(dst + lane * 4 * kBK, &x_map, kb * kBK, rows[0], rows[1], rows[2], rows[3], &ctl.full[s]);
+                }
+            }
+        }
+        // The last blocks' MMAs have read their stages and signalled it; after an abandoned wait, the copies in flight have landed.
+        for (uint32_t i = it > C::Stages ? it - C::Stages : 0; i < it && ok; ++i) ok = __all_sync(0xffffffffu, mbar_wait(&ctl.empty[i % C::Stages], (i / C::Stages) & 1u, abort_flag));
+        if (!ok && lane == 0 && rank == 0) {
+            for (uint32_t i = it > C::Stages ? it - C::Stages : 0; i < it; ++i)
+                for (uint32_t n = 0; n < kSpinLimit && !mbar_try_wait(&ctl.full[i % C::Stages], (i / C::Stages) & 1u); ++n) {
+                }
+        }
+        __syncwarp();
+    } else if (warp == kMmaWarp && rank == 0) {
+        constexpr uint32_t idesc_m = kRows * GROUP;
+        const uint32_t idesc = idesc_e4m3(idesc_m, kHalf);
+        uint32_t it = 0, done[2] = {0, 0};
+        bool ok = true;
+        for (int p = blockIdx.x / GROUP; p < n_tiles && ok; p += step) {
+            const Tile t = tile_of(p);
+            for (int kb = 0; kb < a.KB && ok; ++kb, ++it) {
+                const int s = it % C::Stages;
+                ok = __all_sync(0xffffffffu, mbar_wait(&ctl.full[s], (it / C::Stages) & 1u, abort_flag));
+                if (!ok) break;
+                const uint32_t at = smem_u32(base + s * C::StageBytes);
+                const uint64_t da = umma_desc(at);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (h >= t.halves || !ok) continue;
+                    const uint32_t b = done[h] & 1u;
+                    ok = __all_sync(0xffffffffu, mbar_wait(&ctl.acc_empty[h][b], ((done[h] >> 1) & 1u) ^ 1u, abort_flag));
+                    if (!ok) continue;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint64_t db = umma_desc(at + C::ATile + h * (C::BTile / 2));
+#pragma unroll
+                        for (int k = 0; k < kBK / 32; ++k) umma_f8<GROUP>(tmem + (b * 2 + h) * kHalf, da + 2 * k, db + 2 * k, idesc, k != 0);
+                        if (h == t.halves - 1) commit<GROUP>(&ctl.empty[s]);
+                        commit<GROUP>(&ctl.acc_full[h][b]);
+                    }
+                    __syncwarp();
+                    ++done[h];
+                }
+            }
+        }
+    } else if (warp < kPromoWarps) {
+        const int h = warp >> 2, r = (warp & 3) * 32 + lane;
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + h * kHalf;
+        uint8_t *strip = strips + warp * kStrip;
+        uint32_t done = 0;
+        bool ok = true;
+        for (int p = blockIdx.x / GROUP; p < n_tiles && ok; p += step) {
+            const Tile t = tile_of(p);
+            if (h >= t.halves) continue;
+            int64_t row = t.first + r;  // of y
+            const float *xp = nullptr;  // this thread's scales: null beyond the rows
+            if (r < t.n) {
+                int64_t from = row;
+                if constexpr (GROUPED) {
+                    row = rt.slots[row];
+                    from = (int)row / a.div;
+                }
+                xp = a.xs + from * a.KB;
+            }
+            const float *wp = a.ws + (int64_t)(t.ws_row + h) * a.KB;
+            float2 acc[kHalf / 2];
+#pragma unroll
+            for (int j = 0; j < kHalf / 2; ++j) acc[j] = make_float2(0.f, 0.f);
+            float sx = xp != nullptr ? xp[0] : 0.f, sw = wp[0];
+            for (int kb = 0; kb < a.KB; ++kb, ++done) {
+                const float s = sx * sw;
+                if (kb + 1 < a.KB) sx = xp != nullptr ? xp[kb + 1] : 0.f, sw = wp[kb + 1];  // under the next wait
+                const uint32_t b = done & 1u;
+                ok = __all_sync(0xffffffffu, mbar_wait(&ctl.acc_full[h][b], (done >> 1) & 1u, abort_flag));
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t v0[16], v1[16];
+                tmem_ld16(lanes + b * 2 * kHalf, v0);
+#pragma unroll
+                for (int c = 0; c < kHalf; c += 32) {
+                    tmem_ld_wait();
+                    tmem_ld16(lanes + b * 2 * kHalf + c + 16, v1);
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) fma2(acc[(c + j) / 2], s, v0[j], v0[j + 1]);
+                    tmem_ld_wait();
+                    if (c + 32 < kHalf) tmem_ld16(lanes + b * 2 * kHalf + c + 32, v0);
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) fma2(acc[(c + 16 + j) / 2], s, v1[j], v1[j + 1]);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (GROUP == 2) arrive_at(peer_addr(&ctl.acc_empty[h][b], 0));
+                    else mbar_arrive(&ctl.acc_empty[h][b]);
+                }
+            }
+            if (!ok) break;
+            // y: 64 bytes of every row at a time through the strip; then 4 lanes write a row's 64 bytes, 8 rows an instruction
+            const int es = a.out_f32 ? 4 : 2, per = 64 / es;  // columns of a strip
+            const bool wide = ((int64_t)a.N * es) % 16 == 0 && reinterpret_cast<uintptr_t>(a.y) % 16 == 0;
+            const int n_base = t.n0 + h * kHalf;
+            auto flush = [&](int col) {  // columns col .. col + per of the half
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int rr = i * 8 + (lane >> 2), n = n_base + col + (lane & 3) * (16 / es);
+                    const int64_t orow = __shfl_sync(0xffffffffu, row, rr);
+                    const bool live = (warp & 3) * 32 + rr < t.n;
+                    const uint4 q = *reinterpret_cast<const uint4 *>(strip + rr * kStripPitch + (lane & 3) * 16);
+                    uint8_t *dst = static_cast<uint8_t *>(a.y) + (orow * a.N + n) * es;
+                    if (!live) continue;
+                    if (wide) {
+                        if (n < a.N) *reinterpret_cast<uint4 *>(dst) = q;
+                    } else {
+                        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+                        for (int e = 0; e < 16 / es; ++e) {
+                            if (n + e >= a.N) break;
+                            if (es == 4) reinterpret_cast<uint32_t *>(dst)[e] = w[e];
+                            else reinterpret_cast<uint16_t *>(dst)[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+                        }
+                    }
+                }
+                __syncwarp();
+            };
+            uint4 *mine = reinterpret_cast<uint4 *>(strip + lane * kStripPitch);
+            if (a.out_f32) {
+#pragma unroll
+                for (int c = 0; c < kHalf; c += 16) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 u = acc[c / 2 + 2 * j], v = acc[c / 2 + 2 * j + 1];
+                        mine[j] = make_uint4(__float_as_uint(u.x), __float_as_uint(u.y), __float_as_uint(v.x), __float_as_uint(v.y));
+                    }
+                    flush(c);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < kHalf; c += 32) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 *v = &acc[c / 2 + 4 * j];
+                        mine[j] = make_uint4(bf16x2(v[0].x, v[0].y), bf16x2(v[1].x, v[1].y), bf16x2(v[2].x, v[2].y), bf16x2(v[3].x, v[3].y));
+                    }
+                    flush(c);
+                }
+            }
+        }
+    }
+
+    __syncwarp();
+    tc_fence_before();
+    if constexpr (GROUP == 2) cluster_sync();  // nobody's barriers or shared memory go while the peer signals or reads them
+    __syncthreads();
+    tc_fence_after();
+    if (tid == 0 && ctl.abort_flag) atomicAdd(&g_wide_aborts, 1u);
+    if (warp == kMmaWarp) {
+        if constexpr (GROUP == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+template <int GROUP, bool GROUPED>
+int launch(const char *fn, const uint8_t *w, int64_t w_rows, const uint8_t *x, int64_t x_rows, int64_t K, GemmArgs a, int64_t tiles, cudaStream_t st) {
+    static thread_local int prepared = -1;
+    constexpr size_t smem = smem_bytes<GROUP>();
+    int dev = 0;
+    SB_CUDA(cudaGetDevice(&dev), fn);
+    if (prepared != dev) {
+        SB_CUDA(cudaFuncSetAttribute(fp8_wide_kernel<GROUP, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), fn);
+        prepared = dev;
+    }
+    CUtensorMap wm, xm;
+    SB_TRY(make_map(fn, &wm, w, w_rows, K, 64));
+    SB_TRY(make_map(fn, &xm, x, x_rows, K, GROUPED ? 1 : kRows));
+    a.NT = (a.N + kColTile - 1) / kColTile;
+    const int64_t all = tiles * a.NT, room = sm_count() / GROUP;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(std::min(all, room) * GROUP));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = GROUP, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr, cfg.numAttrs = 1;
+    SB_CUDA((cudaLaunchKernelEx(&cfg, fp8_wide_kernel<GROUP, GROUPED>, wm, xm, a)), fn, " (wide) N=", a.N, " K=", K);
+    return 0;
+}
+
+}  // namespace
+
+namespace sb {
+namespace fp8 {
+
+int wide_dense(const char *fn, const uint8_t *w, int64_t w_rows, const uint8_t *x, int64_t x_rows, int64_t K, const GemmArgs &a, cudaStream_t st) {
+    return launch<2, false>(fn, w, w_rows, x, x_rows, K, a, (a.M + 2 * kRows - 1) / (2 * kRows), st);
+}
+
+int wide_grouped(const char *fn, const uint8_t *w, int64_t w_rows, const uint8_t *x, int64_t x_rows, int64_t K, const GemmArgs &a, cudaStream_t st) {
+    return launch<1, true>(fn, w, w_rows, x, x_rows, K, a, std::min(a.S, a.E + a.S / kRows), st);
+}
+
+unsigned int wide_aborts() {
+    unsigned int v = 0;
+    cudaMemcpyFromSymbol(&v, g_wide_aborts, sizeof(v));
+    return v;
+}
+unsigned int wide_ws_refusals() {
+    unsigned int v = 0;
+    cudaMemcpyFromSymbol(&v, g_wide_refusals, sizeof(v));
+    return v;
+}
+
+}  // namespace fp8
+}  // namespace sb
