@@ -118,7 +118,7 @@ int strix_moe_shared_add_inject(void *y, const void *s, const float *gate_logit,
  * (score 1) of the logits [M, E] (row stride ld); c = s + bias (FP32 [E] or NULL: a balance bias takes part in the choice only). The
  * experts form n_group groups of E / n_group neighbours; a group's value is its largest c (group_top 1) or the sum of its two
  * largest (2); the topk_group largest groups stay open and the k largest c among their experts are the picks. Ties go to the lower
- * index; the order is that of the 64-bit values of c. coef = s of the picks, divided by their sum when renorm (picks whose scores
+ * index; the order is that of the 64-bit values of c (without a bias, of the logits). coef = s of the picks, divided by their sum when renorm (picks whose scores
  * all underflow to zero keep 0), times route_scale. ids, coef [M, A] in descending c, A = k (+ 1 with the shared slot, which is
  * filled as moe_router does). n_group <= 32 divides E <= 1024; k <= min(32, topk_group * E / n_group). A non-finite logit or bias
  * fails the token: ids -1, coef NaN, err = {1, token, expert}. */

@@ -6,8 +6,9 @@
 //   the topk_group largest groups are open (ties: lower group); the k largest c of open groups are the picks (ties: lower expert)
 //   coef = s_pick (/ the picks' sum) * route_scale
 //
-// The order is decided by the 64-bit values of c: two experts whose sums agree to 32 bits still have an order, and a token's experts do
-// not depend on the last bit of an exponential.
+// The order is decided by the 64-bit values of c (without a bias: by the logits, which order the scores): two experts whose sums agree to
+// 32 bits still have an order, and a token's experts do not depend on the last bit of an exponential. The kernel works in FP32 with a bound
+// on its own error; a token in which two values that the choice tells apart lie closer than that bound is done again in 64 bits.
 #include "common.cuh"
 
 #include "strixite_b200.h"
@@ -18,7 +19,8 @@ namespace {
 
 using namespace sb;
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 4;        // tokens per block
+constexpr int kMaxCand = 256;    // candidates a token may have in the FP32 path
 constexpr int64_t kMaxExperts = 1024, kMaxTopK = 32, kMaxGroups = 32;
 enum Score : int { kSoftmax = 0, kSigmoid = 1 };
 
@@ -32,13 +34,20 @@ struct RouteArgs {
     int32_t *ids;
     float *coef;
     int A;
+    int per, L;  // experts of a group; lanes of a group: 32 / (G rounded up to a power of two)
     uint32_t *err;
 };
 
-// Order-preserving map of a double (no NaN) to 64 bits.
+// Order-preserving maps to unsigned integers (no NaN; -0 and +0 are equal).
+__device__ __forceinline__ uint32_t order_key(float f) {
+    uint32_t u = __float_as_uint(f);
+    if (u == 0x80000000u) u = 0u;
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
 __device__ __forceinline__ uint64_t order_key(double v) {
     uint64_t u = (uint64_t)__double_as_longlong(v);
-    if (u == 0x8000000000000000ull) u = 0;  // -0 and +0 are equal
+    if (u == 0x8000000000000000ull) u = 0;
     return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
 }
 __device__ __forceinline__ double warp_sum_d(double v) {
@@ -46,136 +55,313 @@ __device__ __forceinline__ double warp_sum_d(double v) {
     for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
     return v;
 }
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+    return v;
+}
 
-// One warp per token. The lanes are dealt to the groups: with GP = G rounded up to a power of two, group g belongs to the L = 32 / GP
-// lanes from g * L on, and lane `sub` of them holds the group's experts sub, sub + L, .. in registers (NV of them).
-template <typename T, int NV>
-__global__ void __launch_bounds__(kWarps * 32) router_scored_kernel(const T *logits, const T *shared, const RouteArgs a) {
+// A token in 64 bits, one warp, finite logits and bias. Lane `sub` of group g holds the group's experts sub, sub + L, .. Seldom run, so its
+// loops are not unrolled and its values live in local memory: it must not cost the FP32 path registers.
+template <typename T>
+__device__ __noinline__ void route_64(const T *row, const RouteArgs &a, int64_t m) {
     const unsigned full = 0xffffffffu;
-    const int lane = threadIdx.x & 31;
-    const int64_t m = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-    if (m >= a.M) return;  // whole warps leave together; no block-level barrier below
-    int gp = 1;
-    while (gp < a.G) gp *= 2;
-    const int L = 32 / gp, g = lane / L, sub = lane % L, per = a.E / a.G;
-    const T *row = logits + m * a.ld;
-    auto expert = [&](int j) { return g * per + sub + L * j; };
-    auto holds = [&](int j) { return g < a.G && sub + L * j < per; };
-
-    float l[NV];
-    float top = -INFINITY;
-    unsigned bad = UINT_MAX;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        l[j] = -INFINITY;
-        if (holds(j)) {
-            l[j] = ld_act(row, expert(j));
-            if (!isfinite(l[j]) || (a.bias != nullptr && !isfinite(a.bias[expert(j)]))) bad = min(bad, (unsigned)expert(j));
-            top = fmaxf(top, l[j]);
-        }
-    }
-    float sl = 0.f;
-    if (shared != nullptr) {
-        sl = ld_act(shared, m * a.shared_ld);
-        if (!isfinite(sl)) bad = min(bad, (unsigned)a.E);
-    }
-    bad = __reduce_min_sync(full, bad);
-    int32_t *id_row = a.ids + m * a.A;
-    float *coef_row = a.coef + m * a.A;
-    if (bad != UINT_MAX) {  // a non-finite logit or bias fails the token: ids -1, coefficients NaN
-        if (lane == 0) raise_err(a.err, (uint32_t)m, bad);
-        for (int i = lane; i < a.A; i += 32) id_row[i] = -1, coef_row[i] = qnan();
-        return;
-    }
-
-    double p[NV], c[NV];
-    if (a.score == kSigmoid) {
-#pragma unroll
-        for (int j = 0; j < NV; ++j) p[j] = holds(j) ? 1.0 / (1.0 + exp(-(double)l[j])) : 0.0;
-    } else {
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(full, top, off));
-        double sum = 0.0;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            p[j] = holds(j) ? exp((double)l[j] - (double)top) : 0.0;
-            sum += p[j];
-        }
+    const int lane = threadIdx.x & 31, g = lane / a.L, sub = lane % a.L;
+    const int n = g < a.G && sub < a.per ? (a.per - sub + a.L - 1) / a.L : 0;
+    double c[64];  // of the lane's experts: what they are chosen by
+    auto expert = [&](int j) { return g * a.per + sub + a.L * j; };
+    double top = -INFINITY, sum = 1.0;
+    if (a.score == kSoftmax) {
+#pragma unroll 1
+        for (int j = 0; j < n; ++j) top = fmax(top, (double)ld_act(row, expert(j)));
+#pragma unroll 1
+        for (int off = 16; off > 0; off >>= 1) top = fmax(top, __shfl_xor_sync(full, top, off));
+        sum = 0.0;
+#pragma unroll 1
+        for (int j = 0; j < n; ++j) sum += exp((double)ld_act(row, expert(j)) - top);
         sum = warp_sum_d(sum);
-#pragma unroll
-        for (int j = 0; j < NV; ++j) p[j] /= sum;
     }
-#pragma unroll
-    for (int j = 0; j < NV; ++j) c[j] = holds(j) ? p[j] + (a.bias != nullptr ? (double)a.bias[expert(j)] : 0.0) : -INFINITY;
-
+    auto score = [&](float l) { return a.score == kSigmoid ? 1.0 / (1.0 + exp(-(double)l)) : exp((double)l - top) / sum; };
+    const bool biased = a.bias != nullptr;
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+        const float l = ld_act(row, expert(j));
+        c[j] = biased ? score(l) + (double)a.bias[expert(j)] : (double)l;
+    }
     if (a.topk_group < a.G) {
         double b1 = -INFINITY, b2 = -INFINITY;  // the two largest of the lane, then of the group
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
+#pragma unroll 1
+        for (int j = 0; j < n; ++j) {
             if (c[j] > b1) b2 = b1, b1 = c[j];
             else if (c[j] > b2) b2 = c[j];
         }
-        for (int off = L / 2; off > 0; off >>= 1) {
+#pragma unroll 1
+        for (int off = a.L / 2; off > 0; off >>= 1) {
             const double o1 = __shfl_xor_sync(full, b1, off), o2 = __shfl_xor_sync(full, b2, off);
             b2 = o1 > b1 ? fmax(b1, o2) : fmax(b2, o1);
             b1 = fmax(b1, o1);
         }
-        const double value = a.group_top == 2 && per > 1 ? b1 + b2 : b1;
+        double value = b1;
+        if (a.group_top == 2 && a.per > 1) value = biased ? b1 + b2 : score((float)b1) + score((float)b2);
         int rank = 0;  // groups in front of this lane's
+#pragma unroll 1
         for (int h = 0; h < a.G; ++h) {
-            const double o = __shfl_sync(full, value, h * L);
+            const double o = __shfl_sync(full, value, h * a.L);
             rank += o > value || (o == value && h < g);
         }
         if (g >= a.G || rank >= a.topk_group) {
+#pragma unroll 1
+            for (int j = 0; j < n; ++j) c[j] = -INFINITY;
+        }
+    }
+    int my_i = -1;
+#pragma unroll 1
+    for (int r = 0; r < a.k; ++r) {
+        double lv = -INFINITY;
+        int li = INT_MAX, lj = 0;
+#pragma unroll 1
+        for (int j = 0; j < n; ++j)
+            if (c[j] > lv) lv = c[j], li = expert(j), lj = j;  // ascending with strict >: the lower index survives a tie
+        const uint64_t key = order_key(lv);
+        const uint32_t hi = (uint32_t)(key >> 32), hmax = __reduce_max_sync(full, hi);
+        const uint32_t lmax = __reduce_max_sync(full, hi == hmax ? (uint32_t)key : 0u);
+        const unsigned pick = __reduce_min_sync(full, hi == hmax && (uint32_t)key == lmax ? (unsigned)li : UINT_MAX);
+        if (lane == r) my_i = (int)pick;
+        if ((unsigned)li == pick) c[lj] = -INFINITY;
+    }
+    const double p = lane < a.k ? score(ld_act(row, my_i)) : 0.0, of_picks = warp_sum_d(p);
+    if (lane < a.k) {
+        a.ids[m * a.A + lane] = my_i;
+        // scores that all underflow to zero stay zero
+        a.coef[m * a.A + lane] = (float)((a.renorm ? (of_picks > 0.0 ? p / of_picks : 0.0) : p) * (double)a.route_scale);
+    }
+}
+
+// 4 neighbouring logits.
+__device__ __forceinline__ float4 load4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
+__device__ __forceinline__ float4 load4(const uint16_t *p) {
+    const uint2 u = *reinterpret_cast<const uint2 *>(p);
+    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
+}
+
+// One warp per token. The lanes are dealt to the groups (a group's L neighbouring lanes hold its experts, NV a lane, in runs of four where
+// VEC), so a group's value is a reduction over L lanes and a closed group is a lane that drops out.
+// The choice: the k-th largest lane maximum bounds the k-th largest value from below, what reaches it are the candidates (about 1.3 k of
+// them), they meet in shared memory and each counts those in front of it: no k rounds of warp-wide maxima.
+//
+// The FP32 errors that the choice allows for (documented bounds: expf 2 ulp, __expf 2 + 1.17 |x| ulp, __fdividef 2 ulp):
+//   sigmoid  e = __expf(-l): p moves by p (1 - p) (2 + 1.17 |l|) 2^-23 <= 0.77 * 2^-23, 1 + e by 2^-24, the quotient by 2^-22: 3.3 * 2^-23, for
+//            two values 6.6 * 2^-23 < 2^-20
+//   softmax  e = expf(l - top): (2 + |x| / 2) 2^-23 of e; the sum of up to 64 a lane and 5 steps: 35 * 2^-23 and the terms' mean, at most
+//            2 + ln(1024) / 2; p by at most 45 * 2^-23 of the largest p, for two values 90 * 2^-23 < 2^-16
+//   c = p + bias one rounding each, 2^-24 |c|: 2^-22 (|c| + |c'|) is above both
+template <typename T, int NV, bool VEC>
+__global__ void __launch_bounds__(kWarps * 32) router_scored_kernel(const T *logits, const T *shared, const RouteArgs a) {
+    __shared__ uint64_t cand[kWarps][kMaxCand];
+    __shared__ uint64_t sorted[kWarps][40];
+    const unsigned full = 0xffffffffu;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t m = (int64_t)blockIdx.x * kWarps + warp;
+    if (m >= a.M) return;  // whole warps leave together; no block-level barrier below
+    const int L = a.L, g = lane / L, sub = lane % L;
+    const T *row = logits + m * a.ld;
+    auto expert = [&](int j) { return VEC ? g * a.per + (j >> 2) * 4 * L + sub * 4 + (j & 3) : g * a.per + sub + L * j; };
+    auto holds = [&](int j) { return g < a.G && (VEC ? (j >> 2) * 4 * L + sub * 4 : sub + L * j) < a.per; };
+
+    float c[NV];  // the logits, then what the experts are chosen by
+    float chk = 0.f;  // stays 0 while everything is finite: 0 * inf and 0 * NaN are NaN
+    if constexpr (VEC) {
+#pragma unroll
+        for (int j = 0; j < NV; j += 4) {
+            float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            if (holds(j)) {
+                v = load4(row + expert(j));
+                chk = fmaf(v.x, 0.f, fmaf(v.y, 0.f, fmaf(v.z, 0.f, fmaf(v.w, 0.f, chk))));
+            }
+            c[j] = v.x, c[j + 1] = v.y, c[j + 2] = v.z, c[j + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            c[j] = -INFINITY;
+            if (holds(j)) c[j] = ld_act(row, expert(j)), chk = fmaf(c[j], 0.f, chk);
+        }
+    }
+    float sl = 0.f;
+    if (shared != nullptr) sl = ld_act(shared, m * a.shared_ld), chk = fmaf(sl, 0.f, chk);
+
+    const bool biased = a.bias != nullptr;
+    float top = 0.f, sum = 1.f, base = 0.f;
+    if (a.score == kSoftmax) {
+        top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) top = fmaxf(top, c[j]);
+        top = warp_max(top);
+        if (biased || !a.renorm) {
+            sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) sum += expf(c[j] - top);  // absent experts: exp(-inf) = 0
+            sum = warp_sum(sum);
+        }
+    }
+    if (biased) {
+        const float inv = 1.0f / sum;
+        base = a.score == kSigmoid ? 0x1p-20f : 0x1p-16f * inv;
+#pragma unroll
+        for (int j = 0; j < NV; j += VEC ? 4 : 1) {
+            if (!holds(j)) continue;
+            float b[4];
+            if constexpr (VEC) {
+                const float4 v = load4(a.bias + expert(j));
+                b[0] = v.x, b[1] = v.y, b[2] = v.z, b[3] = v.w;
+            } else {
+                b[0] = a.bias[expert(j)];
+            }
+#pragma unroll
+            for (int i = 0; i < (VEC ? 4 : 1); ++i) {
+                chk = fmaf(b[i], 0.f, chk);
+                const float l = c[j + i];
+                c[j + i] = (a.score == kSigmoid ? __fdividef(1.0f, 1.0f + __expf(-l)) : expf(l - top) * inv) + b[i];
+            }
+        }
+    }
+    if (__any_sync(full, !(chk == 0.f))) {  // a non-finite logit or bias fails the token: ids -1, coefficients NaN
+        unsigned bad = UINT_MAX;
+        for (int e = lane; e < a.E; e += 32)
+            if (!isfinite(ld_act(row, e)) || (biased && !isfinite(a.bias[e]))) bad = min(bad, (unsigned)e);
+        if (!isfinite(sl)) bad = min(bad, (unsigned)a.E);
+        bad = __reduce_min_sync(full, bad);
+        if (lane == 0) raise_err(a.err, (uint32_t)m, bad);
+        for (int i = lane; i < a.A; i += 32) a.ids[m * a.A + i] = -1, a.coef[m * a.A + i] = qnan();
+        return;
+    }
+
+    bool close = false;  // two values that the choice tells apart lie within the error
+    if (a.topk_group < a.G) {
+        float b1 = -INFINITY, b2 = -INFINITY;  // the two largest of the lane, then of the group
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            b2 = fmaxf(b2, fminf(b1, c[j]));
+            b1 = fmaxf(b1, c[j]);
+        }
+        for (int off = L / 2; off > 0; off >>= 1) {
+            const float o1 = __shfl_xor_sync(full, b1, off), o2 = __shfl_xor_sync(full, b2, off);
+            b2 = fmaxf(fmaxf(b2, o2), fminf(b1, o1));
+            b1 = fmaxf(b1, o1);
+        }
+        float value = b1, tol = 0.f;
+        if (a.group_top == 2 && a.per > 1) {
+            if (biased) value = b1 + b2, tol = 2.f * base + 0x1p-21f * (fabsf(b1) + fabsf(b2));
+            else if (a.score == kSigmoid) value = __fdividef(1.0f, 1.0f + __expf(-b1)) + __fdividef(1.0f, 1.0f + __expf(-b2)), tol = 0x1p-18f;
+            else value = expf(b1 - top) + expf(b2 - top), tol = 0x1p-18f;
+        } else if (biased) {
+            tol = base + 0x1p-21f * fabsf(b1);
+        }
+        int rank = 0;  // groups in front of this lane's
+        for (int h = 0; h < a.G; ++h) {
+            const float o = __shfl_sync(full, value, h * L);
+            rank += o > value || (o == value && h < g);
+        }
+        const bool open = g < a.G && rank < a.topk_group;
+        if (!open) {
 #pragma unroll
             for (int j = 0; j < NV; ++j) c[j] = -INFINITY;
         }
-    }
-
-    double lv, lp;  // the lane's best candidate: value, score, expert
-    int li;
-    auto rescan = [&]() {
-        lv = -INFINITY, lp = 0.0, li = INT_MAX;
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-            if (c[j] > lv) lv = c[j], lp = p[j], li = expert(j);  // ascending with strict >: the lower index survives a tie
-    };
-    rescan();
-    double my_p = 0.0;
-    int my_i = -1;
-    for (int r = 0; r < a.k; ++r) {
-        const uint64_t key = order_key(lv);
-        const uint32_t hi = (uint32_t)(key >> 32), hmax = __reduce_max_sync(full, hi);
-        const uint32_t lo = hi == hmax ? (uint32_t)key : 0u, lmax = __reduce_max_sync(full, lo);
-        const bool best = hi == hmax && (uint32_t)key == lmax;
-        const unsigned pick = __reduce_min_sync(full, best ? (unsigned)li : UINT_MAX);
-        const bool mine = (unsigned)li == pick;
-        const int owner = __ffs(__ballot_sync(full, mine)) - 1;
-        const double score = __shfl_sync(full, lp, owner);
-        if (lane == r) my_p = score, my_i = (int)pick;
-        if (mine) {
-#pragma unroll
-            for (int j = 0; j < NV; ++j)
-                if (holds(j) && expert(j) == (int)pick) c[j] = -INFINITY;
-            rescan();
+        if (biased || (a.group_top == 2 && a.per > 1)) {  // else the values are exact
+            const float worst = __uint_as_float(__reduce_max_sync(full, g < a.G ? __float_as_uint(tol) : 0u));
+            const float least_open = key_value(__reduce_min_sync(full, open ? order_key(value) : UINT_MAX));
+            const float most_shut = key_value(__reduce_max_sync(full, g < a.G && !open ? order_key(value) : order_key(-INFINITY)));
+            close = !(least_open - most_shut > worst);
         }
     }
-    const double sum = warp_sum_d(my_p);  // lanes >= k hold 0
-    if (lane < a.k) {
-        id_row[lane] = my_i;
-        // scores that all underflow to zero stay zero
-        coef_row[lane] = (float)((a.renorm ? (sum > 0.0 ? my_p / sum : 0.0) : my_p) * (double)a.route_scale);
+
+    int n = 0;  // candidates
+    if (!close) {
+        float lm = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) lm = fmaxf(lm, c[j]);
+        // the lane maxima in descending order (a bitonic network over the lanes), of which the k-th
+#pragma unroll
+        for (int size = 2; size <= 32; size *= 2) {
+#pragma unroll
+            for (int off = size / 2; off > 0; off /= 2) {
+                const float o = __shfl_xor_sync(full, lm, off);
+                const bool larger = ((lane & off) == 0) == ((lane & size) == 0);  // this lane keeps the larger of the two
+                lm = larger ? fmaxf(lm, o) : fminf(lm, o);
+            }
+        }
+        const float kth = __shfl_sync(full, lm, a.k - 1);
+        // what lies below the k-th by no more than the error is a candidate too: nothing that is left out can belong to the picks
+        const float bound = biased ? kth - (base + 0x1p-21f * fabsf(kth)) : kth;
+        int mine = 0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) mine += c[j] >= bound && c[j] > -INFINITY;
+        int at = mine;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int o = __shfl_up_sync(full, at, off);
+            if (lane >= off) at += o;
+        }
+        n = __shfl_sync(full, at, 31);
+        at -= mine;
+        if (n <= kMaxCand) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                if (c[j] >= bound && c[j] > -INFINITY) cand[warp][at++] = ((uint64_t)order_key(c[j]) << 32) | (uint32_t)~expert(j);
+            __syncwarp();
+            // a larger key is in front: larger value, then lower expert; the keys differ, so the ranks are 0 .. n - 1
+            for (int i = lane; i < n; i += 32) {
+                const uint64_t key = cand[warp][i];
+                int rank = 0;
+                for (int q = 0; q < n; ++q) rank += cand[warp][q] > key;
+                if (rank <= a.k) sorted[warp][rank] = key;
+            }
+            __syncwarp();
+        }
     }
-    if (shared != nullptr && lane == 0) id_row[a.k] = a.shared_id, coef_row[a.k] = sigmoid_f(sl);
+    int pick = -1;
+    float l = 0.f, value = 0.f;
+    if (!close && n <= kMaxCand) {
+        if (lane < a.k) {
+            const uint64_t key = sorted[warp][lane];
+            pick = (int)~(uint32_t)key, value = key_value((uint32_t)(key >> 32));
+            if (biased && lane + 1 < n) {
+                const float next = key_value((uint32_t)(sorted[warp][lane + 1] >> 32));
+                close = !(value - next > base + 0x1p-22f * (fabsf(value) + fabsf(next)));
+            }
+            l = ld_act(row, pick);
+            close |= (a.score == kSigmoid ? l : l - top) < -80.f;  // the score leaves FP32's normal range
+        }
+    } else {
+        close = true;
+    }
+    if (__any_sync(full, close)) {
+        route_64(row, a, m);
+    } else {
+        float p = 0.f;
+        if (lane < a.k) {
+            if (a.score == kSigmoid) {
+                p = sigmoid_f(l);
+            } else {
+                const float x = l - top, lost = (l - (x - (x - l))) + (-top - (x - l));  // l - top = x + lost exactly
+                p = expf(x);
+                p = fmaf(p, lost, p);
+            }
+        }
+        const float of_picks = a.renorm ? warp_sum(p) : sum;  // sigmoid without renorm: 1
+        if (lane < a.k) {
+            a.ids[m * a.A + lane] = pick;
+            a.coef[m * a.A + lane] = p / of_picks * a.route_scale;
+        }
+    }
+    if (shared != nullptr && lane == 0) a.ids[m * a.A + a.k] = a.shared_id, a.coef[m * a.A + a.k] = sigmoid_f(sl);
 }
 
-template <typename T>
+template <typename T, bool VEC>
 void launch(const void *logits, const void *shared, const RouteArgs &a, cudaStream_t st) {
-    int gp = 1;
-    while (gp < a.G) gp *= 2;
-    const int L = 32 / gp, nv = (a.E / a.G + L - 1) / L;
+    const int nv = (a.per + a.L - 1) / a.L;
     const unsigned blocks = (unsigned)((a.M + kWarps - 1) / kWarps);
-#define SB_ROUTE(NV) router_scored_kernel<T, NV><<<blocks, kWarps * 32, 0, st>>>((const T *)logits, (const T *)shared, a)
+#define SB_ROUTE(NV) router_scored_kernel<T, NV, VEC><<<blocks, kWarps * 32, 0, st>>>((const T *)logits, (const T *)shared, a)
     if (nv <= 4) SB_ROUTE(4);
     else if (nv <= 8) SB_ROUTE(8);
     else if (nv <= 16) SB_ROUTE(16);
@@ -218,9 +404,16 @@ int strix_moe_router_scored(const void *logits, int64_t ld, int64_t M, int64_t E
     a.ld = ld, a.M = M, a.E = (int)E, a.k = (int)k, a.score = score, a.G = (int)n_group, a.topk_group = (int)topk_group, a.group_top = (int)group_top;
     a.renorm = renorm != 0, a.route_scale = route_scale, a.bias = bias, a.shared_ld = shared_ld, a.shared_id = shared_id, a.ids = ids, a.coef = coef;
     a.A = (int)A, a.err = err;
+    int gp = 1;
+    while (gp < a.G) gp *= 2;
+    a.per = a.E / a.G, a.L = 32 / gp;
+    // runs of four where they fill the lanes of a group evenly and every row starts aligned
+    const bool vec = a.per % (4 * a.L) == 0 && ld % 4 == 0 && reinterpret_cast<uintptr_t>(logits) % (4 * act_size(act)) == 0 && aligned16(bias);
     auto st = static_cast<cudaStream_t>(stream);
-    if (act == kF32) launch<float>(logits, shared_logit, a, st);
-    else launch<uint16_t>(logits, shared_logit, a, st);
+    if (act == kF32 && vec) launch<float, true>(logits, shared_logit, a, st);
+    else if (act == kF32) launch<float, false>(logits, shared_logit, a, st);
+    else if (vec) launch<uint16_t, true>(logits, shared_logit, a, st);
+    else launch<uint16_t, false>(logits, shared_logit, a, st);
     SB_LAUNCH_OK(fn, " ", act_name(act), " M=", M, " E=", E, " k=", k, " groups=", n_group);
     return 0;
 }

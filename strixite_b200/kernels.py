@@ -52,8 +52,15 @@ def _p(t):
 
 
 def _s(stream):
-    st = torch.cuda.current_stream() if stream is None else stream
-    return C.c_void_p(st.cuda_stream)
+    return C.c_void_p(_raw(stream, torch.cuda.current_device()))
+
+
+_current_raw = torch._C._cuda_getCurrentRawStream  # the stream's handle without a Stream object: 0.1 instead of 1 us a call
+
+
+def _raw(stream, device):
+    """The handle of `stream`, or of the device's current stream."""
+    return _current_raw(device) if stream is None else stream.cuda_stream
 
 
 def new_err(device="cuda"):
@@ -513,7 +520,7 @@ class Score(enum.IntEnum):
     Sigmoid = 1
 
 
-_SCORES = {"softmax": 0, "sigmoid": 1, 0: 0, 1: 1}
+_SCORES = {"softmax": 0, "sigmoid": 1, 0: 0, 1: 1}  # a Score is an int
 FP8_BLOCK = 128
 
 
@@ -522,29 +529,31 @@ def fp8_blocks(n):
     return -(-n // FP8_BLOCK)
 
 
-def _t(fn, name, t, dtypes, n, optional=False):
-    """The address of a contiguous tensor of one of `dtypes` with at least n elements on the current device."""
+def _t(fn, name, t, dtypes, n, device, optional=False):
+    """The address of a contiguous tensor of one of `dtypes` with at least n elements on `device`. On the path of every call: a good tensor
+    costs a handful of attribute reads."""
+    if t is None and optional:
+        return None
+    if t is not None and t.get_device() == device and t.dtype in dtypes and t.numel() >= n and t.is_contiguous():
+        return t.data_ptr()
     if t is None:
-        if optional:
-            return None
         raise StrixError("%s: %s is None" % (fn, name))
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
-        raise StrixError("%s: %s is on %s, expected the current device cuda:%d" % (fn, name, t.device, torch.cuda.current_device()))
+    if t.get_device() != device:
+        raise StrixError("%s: %s is on %s, expected the current device cuda:%d" % (fn, name, t.device, device))
     if t.dtype not in dtypes:
         raise StrixError("%s: %s is %s, expected %s" % (fn, name, t.dtype, " or ".join(str(d) for d in dtypes)))
-    if t.numel() < n or not t.is_contiguous():
-        raise StrixError("%s: %s has %s elements%s, expected %d contiguous" % (fn, name, t.numel(), "" if t.is_contiguous() else " (not contiguous)", n))
-    return t.data_ptr()
+    raise StrixError("%s: %s has %s elements%s, expected %d contiguous" % (fn, name, t.numel(), "" if t.is_contiguous() else " (not contiguous)", n))
 
 
 _F8, _F32, _I32 = (torch.float8_e4m3fn, torch.uint8), (torch.float32,), (torch.int32,)
-_ACTS = {0: (torch.float32,), 1: (torch.bfloat16,)}
+_ACTS = {0: (torch.float32,), 1: (torch.bfloat16,)}  # an Act is an int
 
 
 def _act_dtypes(fn, act):
-    if int(act) not in _ACTS:
+    dt = _ACTS.get(act)
+    if dt is None:
         raise StrixError("%s: unsupported activation dtype %r" % (fn, act))
-    return _ACTS[int(act)]
+    return dt
 
 
 class Fp8Weight:
@@ -563,8 +572,9 @@ class Fp8Weight:
             raise StrixError("Fp8Weight: scale must be a contiguous float32 %s tensor, got %s %s" % (want, tuple(scale.shape), scale.dtype))
         if q.device != scale.device:
             raise StrixError("Fp8Weight: q is on %s, scale on %s" % (q.device, scale.device))
-        self.q, self.scale = q, scale
+        self.q, self.scale, self.KB, self.device = q, scale, want[1], q.get_device()
         self._view = Fp8View(q.data_ptr(), scale.data_ptr(), self.N, self.K)
+        self._ref = C.byref(self._view)
 
     def view(self):
         return self._view
@@ -573,13 +583,21 @@ class Fp8Weight:
         return self.q.numel() + 4 * self.scale.numel()
 
 
-def _fp8w(fn, w, experts):
+def _fp8w(fn, w, experts, device):
     if not isinstance(w, Fp8Weight):
         raise StrixError("%s: expected an Fp8Weight, got %s" % (fn, type(w).__name__))
     if w.experts != experts:
         raise StrixError("%s: the weight holds %d experts, the call states %d" % (fn, w.experts, experts))
-    _t(fn, "the weight", w.q, _F8, w.N * w.K)
-    return C.byref(w._view)
+    if w.device != device:
+        raise StrixError("%s: the weight is on %s, expected the current device cuda:%d" % (fn, w.q.device, device))
+    return w._ref
+
+
+def _any_bytes(fn, name, t, n, device):
+    """The address of a contiguous tensor of any dtype with at least n bytes."""
+    if t is None or t.get_device() != device or not t.is_contiguous() or t.numel() * t.element_size() < n:
+        raise StrixError("%s: %s must be a contiguous tensor of at least %d bytes on the current device cuda:%d" % (fn, name, n, device))
+    return t.data_ptr()
 
 
 def moe_router_scored(logits, ld, M, E, k, score, bias, n_group, topk_group, group_top, renorm, route_scale, shared_logit, shared_ld, shared_id, ids, coef, act,
@@ -587,57 +605,63 @@ def moe_router_scored(logits, ld, M, E, k, score, bias, n_group, topk_group, gro
     """Score-based routing: `score` 'softmax' or 'sigmoid' (or Score), an optional balance bias [E] for the choice, n_group groups of which
     topk_group stay open (a group's value: its group_top = 1 or 2 largest), k picks, weights renormalised when `renorm`, times route_scale.
     logits: a tensor whose first element is token 0's first logit, rows ld apart; shared_logit as in moe_router."""
-    fn = "moe_router_scored"
-    if score not in _SCORES:
+    fn, dev = "moe_router_scored", torch.cuda.current_device()
+    how = _SCORES.get(score)
+    if how is None:
         raise StrixError("%s: score %r, expected 'softmax' or 'sigmoid'" % (fn, score))
     dt = _act_dtypes(fn, act)
-    A = k + (0 if shared_logit is None else 1)
-    for name, t in (("logits", logits), ("shared_logit", shared_logit)):  # views into rows of stride ld
-        if t is not None and (not t.is_cuda or t.device.index != torch.cuda.current_device() or t.dtype not in dt):
-            raise StrixError("%s: %s must be %s on the current device, got %s on %s" % (fn, name, dt[0], t.dtype, t.device))
-    call("strix_moe_router_scored", logits.data_ptr(), ld, M, E, k, _SCORES[score], _t(fn, "bias", bias, _F32, E, True), n_group, topk_group, group_top, int(bool(renorm)),
-         float(route_scale), None if shared_logit is None else shared_logit.data_ptr(), shared_ld, shared_id, _t(fn, "ids", ids, _I32, M * A),
-         _t(fn, "coef", coef, _F32, M * A), int(act), _t(fn, "err", err, _I32, 3), _s(stream))
+    A = k if shared_logit is None else k + 1
+    # views into rows of stride ld: what lies behind their first element in the storage has to hold the last row
+    for name, t, stride, last in (("logits", logits, ld, E), ("shared_logit", shared_logit, shared_ld, 1)):
+        if t is None and name == "shared_logit":
+            continue
+        if t is None or t.get_device() != dev or t.dtype not in dt:
+            raise StrixError("%s: %s must be a %s tensor on the current device cuda:%d" % (fn, name, dt[0], dev))
+        if t.untyped_storage().nbytes() // t.element_size() - t.storage_offset() < (M - 1) * stride + last:
+            raise StrixError("%s: %s ends before the last of %d rows, %d apart" % (fn, name, M, stride))
+    call("strix_moe_router_scored", logits.data_ptr(), ld, M, E, k, how, _t(fn, "bias", bias, _F32, E, dev, True), n_group, topk_group, group_top, 1 if renorm else 0,
+         route_scale, None if shared_logit is None else shared_logit.data_ptr(), shared_ld, shared_id, _t(fn, "ids", ids, _I32, M * A, dev),
+         _t(fn, "coef", coef, _F32, M * A, dev), act, _t(fn, "err", err, _I32, 3, dev), _raw(stream, dev))
 
 
 def residual_rmsnorm_fp8(x, y, w, M, d, eps, x_out, h, q, scale, act, centered=False, stream=None):
     """x_out = x + y (both None: x alone; x_out may be x or y), h = RMSnorm(x_out) * (w, or 1 + w when centered), q / scale: h as FP8 rows.
     h, or q and scale, may be None."""
-    fn = "residual_rmsnorm_fp8"
+    fn, dev = "residual_rmsnorm_fp8", torch.cuda.current_device()
     dt, n = _act_dtypes(fn, act), M * d
-    call("strix_residual_rmsnorm_fp8", _t(fn, "x", x, dt, n), _t(fn, "y", y, dt, n, True), _t(fn, "w", w, _F32, d), int(bool(centered)), float(eps), M, d,
-         _t(fn, "x_out", x_out, dt, n, True), _t(fn, "h", h, dt, n, True), _t(fn, "q", q, _F8, n, True),
-         _t(fn, "scale", scale, _F32, M * fp8_blocks(d), True), int(act), _s(stream))
+    call("strix_residual_rmsnorm_fp8", _t(fn, "x", x, dt, n, dev), _t(fn, "y", y, dt, n, dev, True), _t(fn, "w", w, _F32, d, dev), 1 if centered else 0, eps, M, d,
+         _t(fn, "x_out", x_out, dt, n, dev, True), _t(fn, "h", h, dt, n, dev, True), _t(fn, "q", q, _F8, n, dev, True),
+         _t(fn, "scale", scale, _F32, M * fp8_blocks(d), dev, True), act, _raw(stream, dev))
 
 
 def swiglu_fp8(gu, q, scale, rows, I, act, stream=None):
     """swiglu of merged [gate | up] rows [rows, 2I] with the result as FP8 rows q [rows, I], scale [rows, blocks(I)]."""
-    fn = "swiglu_fp8"
-    call("strix_swiglu_fp8", _t(fn, "gu", gu, _act_dtypes(fn, act), rows * 2 * I), _t(fn, "q", q, _F8, rows * I), _t(fn, "scale", scale, _F32, rows * fp8_blocks(I)), rows, I,
-         int(act), _s(stream))
+    fn, dev = "swiglu_fp8", torch.cuda.current_device()
+    call("strix_swiglu_fp8", _t(fn, "gu", gu, _act_dtypes(fn, act), rows * 2 * I, dev), _t(fn, "q", q, _F8, rows * I, dev),
+         _t(fn, "scale", scale, _F32, rows * fp8_blocks(I), dev), rows, I, act, _raw(stream, dev))
 
 
 def linear_fp8(xq, xs, w, y, M, out_act, stream=None):
     """y[M, N] = the FP8 rows (xq [M, K], xs [M, blocks(K)]) times an Fp8Weight [N, K] transposed, FP32 or BF16."""
-    fn = "linear_fp8"
-    v = _fp8w(fn, w, 1)
-    call("strix_linear_fp8", _t(fn, "xq", xq, _F8, M * w.K), _t(fn, "xs", xs, _F32, M * fp8_blocks(w.K)), v, _t(fn, "y", y, _act_dtypes(fn, out_act), M * w.N), M,
-         int(out_act), _s(stream))
+    fn, dev = "linear_fp8", torch.cuda.current_device()
+    v = _fp8w(fn, w, 1, dev)
+    call("strix_linear_fp8", _t(fn, "xq", xq, _F8, M * w.K, dev), _t(fn, "xs", xs, _F32, M * w.KB, dev), v, _t(fn, "y", y, _act_dtypes(fn, out_act), M * w.N, dev), M,
+         out_act, _raw(stream, dev))
 
 
 def linear_fp8_experts_gather_grouped(xq, xs, w, E, ws, ws_bytes, M, A, y, out_act, stream=None):
     """y[slot, :] = expert ids[slot] of the stack times FP8 row slot / A, over the workspace of moe_group_routes(ids, M, A, E, ...)."""
-    fn = "linear_fp8_experts_gather_grouped"
-    v = _fp8w(fn, w, E)
-    call("strix_linear_fp8_experts_gather_grouped", _t(fn, "xq", xq, _F8, M * w.K), _t(fn, "xs", xs, _F32, M * fp8_blocks(w.K)), v, E,
-         _t(fn, "ws", ws, (ws.dtype,), -(-ws_bytes // ws.element_size())), ws_bytes, M, A, _t(fn, "y", y, _act_dtypes(fn, out_act), M * A * (w.N // E)), int(out_act), _s(stream))
+    fn, dev = "linear_fp8_experts_gather_grouped", torch.cuda.current_device()
+    v = _fp8w(fn, w, E, dev)
+    call("strix_linear_fp8_experts_gather_grouped", _t(fn, "xq", xq, _F8, M * w.K, dev), _t(fn, "xs", xs, _F32, M * w.KB, dev), v, E, _any_bytes(fn, "ws", ws, ws_bytes, dev),
+         ws_bytes, M, A, _t(fn, "y", y, _act_dtypes(fn, out_act), M * A * (w.N // E), dev), out_act, _raw(stream, dev))
 
 
 def linear_fp8_experts_combine_grouped(hq, hs, w, E, ids, coef, ws, ws_bytes, partial, M, A, y, act, stream=None):
     """y[m, :] = sum over a of coef[m, a] * (expert ids[m, a] of the stack times FP8 row m * A + a); partial: M * A * N floats."""
-    fn = "linear_fp8_experts_combine_grouped"
-    v = _fp8w(fn, w, E)
+    fn, dev = "linear_fp8_experts_combine_grouped", torch.cuda.current_device()
+    v = _fp8w(fn, w, E, dev)
     S, N = M * A, w.N // E
-    call("strix_linear_fp8_experts_combine_grouped", _t(fn, "hq", hq, _F8, S * w.K), _t(fn, "hs", hs, _F32, S * fp8_blocks(w.K)), v, E, _t(fn, "ids", ids, _I32, S),
-         _t(fn, "coef", coef, _F32, S), _t(fn, "ws", ws, (ws.dtype,), -(-ws_bytes // ws.element_size())), ws_bytes, _t(fn, "partial", partial, _F32, S * N), M, A,
-         _t(fn, "y", y, _act_dtypes(fn, act), M * N), int(act), _s(stream))
+    call("strix_linear_fp8_experts_combine_grouped", _t(fn, "hq", hq, _F8, S * w.K, dev), _t(fn, "hs", hs, _F32, S * w.KB, dev), v, E, _t(fn, "ids", ids, _I32, S, dev),
+         _t(fn, "coef", coef, _F32, S, dev), _any_bytes(fn, "ws", ws, ws_bytes, dev), ws_bytes, _t(fn, "partial", partial, _F32, S * N, dev), M, A,
+         _t(fn, "y", y, _act_dtypes(fn, act), M * N, dev), act, _raw(stream, dev))
