@@ -11,15 +11,16 @@ constexpr int kFp8Block = 128;
 inline int64_t fp8_blocks(int64_t n) { return (n + kFp8Block - 1) / kFp8Block; }
 
 #ifdef __CUDACC__
-// |v| as an integer that orders like |v|, with every NaN above infinity: an integer maximum keeps a NaN that fmaxf would drop.
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// The larger of a and |v|; a NaN in either stays one (fmaxf would drop it).
+__device__ __forceinline__ float max_abs(float a, float v) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(v)));
+    return r;
+}
 
 // The scale of a block from its largest magnitude: 448 (the largest e4m3 value) stands for it. The floor 2^-100 gives a block of
 // zeros a scale that divides and keeps the quotient away from the subnormals; a NaN stays one.
-__device__ __forceinline__ float fp8_scale(uint32_t amax_bits) {
-    const uint32_t floor_bits = 0x0D800000u;  // 2^-100
-    return __uint_as_float(amax_bits < floor_bits ? floor_bits : amax_bits) / 448.0f;
-}
+__device__ __forceinline__ float fp8_scale(float amax) { return max_abs(0x1p-100f, amax) / 448.0f; }
 
 // Two values in e4m3, round to nearest even, saturating at +-448 (NaN -> the NaN code); `lo` in the low byte.
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
@@ -28,22 +29,62 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     return r;
 }
 
-// 8 values of one block -> 8 e4m3 bytes of v / scale. An IEEE division, as the definition says: a reciprocal moves values that lie
-// next to a rounding border.
+// v / d to the last bit or the one next to it: the hardware's approximate reciprocal r of d (1 ulp), the quotient v * r (2 ulp) and one
+// correction by its remainder, which the FMA gives exactly (Markstein's step). d and v / d well inside FP32's range.
+__device__ __forceinline__ float fast_rcp(float d) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+    return r;
+}
+__device__ __forceinline__ float quotient(float v, float d, float r) {
+    const float q = v * r;
+    return fmaf(fmaf(-q, d, v), r, q);
+}
+
+// 8 values of one block -> 8 e4m3 bytes of v / scale. A product with the reciprocal alone would move values that lie next to a
+// rounding border; 8 IEEE divisions cost as many instructions as the rest of the kernels that use this.
 __device__ __forceinline__ uint2 fp8_pack8(const float (&v)[8], float scale) {
     uint32_t h[4];
+    if (scale < 0x1p100f) {
+        const float r = fast_rcp(scale);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = e4m3x2(__fdiv_rn(v[2 * i], scale), __fdiv_rn(v[2 * i + 1], scale));
+        for (int i = 0; i < 4; ++i) h[i] = e4m3x2(quotient(v[2 * i], scale, r), quotient(v[2 * i + 1], scale, r));
+    } else {  // near FP32's end, infinite or NaN
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = e4m3x2(__fdiv_rn(v[2 * i], scale), __fdiv_rn(v[2 * i + 1], scale));
+    }
     return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
 }
 
-// The largest abs_bits among the 16 lanes of a half warp (the 16 x 8 values of a block).
-__device__ __forceinline__ uint32_t half_warp_max(uint32_t v) {
+// silu(g) * u of 8 pairs with the same division; where a gate is near the ends of the exponential's range (or infinite), as the
+// definition says.
+__device__ __forceinline__ void swiglu8(const float (&g)[8], const float (&u)[8], float (&h)[8]) {
+    float most = 0.f;
 #pragma unroll
-    for (int off = 8; off > 0; off >>= 1) {
-        const uint32_t o = __shfl_xor_sync(0xffffffffu, v, off);
-        v = o > v ? o : v;
+    for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(g[j]));
+    if (most < 80.0f) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float d = 1.0f + expf(-g[j]);
+            h[j] = quotient(g[j], d, fast_rcp(d)) * u[j];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[j] = silu_f(g[j]) * u[j];
     }
+}
+
+// Two values in BF16, round to nearest even; `lo` in the low half.
+__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// The largest of the 16 lanes of a half warp (the 16 x 8 values of a block); NaN if one is.
+__device__ __forceinline__ float half_warp_max(float v) {
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) v = max_abs(v, __shfl_xor_sync(0xffffffffu, v, off));
     return v;
 }
 
@@ -63,9 +104,17 @@ __device__ __forceinline__ void store8(float *p, const float (&v)[8]) {
     *reinterpret_cast<float4 *>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
 }
 __device__ __forceinline__ void store8(uint16_t *p, const float (&v)[8]) {
+    *reinterpret_cast<uint4 *>(p) = make_uint4(bf16x2(v[0], v[1]), bf16x2(v[2], v[3]), bf16x2(v[4], v[5]), bf16x2(v[6], v[7]));
+}
+// The values that a store8 followed by a load8 gives back, and the store.
+__device__ __forceinline__ void store8_and_keep(float *p, float (&v)[8]) { store8(p, v); }
+__device__ __forceinline__ void store8_and_keep(uint16_t *p, float (&v)[8]) {
     uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)f32_to_bf16_bits(v[2 * i]) | ((uint32_t)f32_to_bf16_bits(v[2 * i + 1]) << 16);
+    for (int i = 0; i < 4; ++i) {
+        w[i] = bf16x2(v[2 * i], v[2 * i + 1]);
+        v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
     *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 #endif  // __CUDACC__

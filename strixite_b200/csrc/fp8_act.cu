@@ -31,8 +31,8 @@ __global__ void __launch_bounds__(kNormMaxThreads)
                 float a[8];
                 load8(y + base + c, a);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[i][j] = as_stored(v[i][j] + a[j], x_out);
-                store8(x_out + base + c, v[i]);
+                for (int j = 0; j < 8; ++j) v[i][j] += a[j];
+                store8_and_keep(x_out + base + c, v[i]);
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) sq = fmaf(v[i][j], v[i][j], sq);
@@ -50,14 +50,14 @@ __global__ void __launch_bounds__(kNormMaxThreads)
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
         const int c = (threadIdx.x + i * blockDim.x) * 8;
-        uint32_t top = 0;
+        float top = 0.f;
         if (c < d) {
             float g[8];
             load8(w + c, g);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 v[i][j] = v[i][j] * r * (g[j] + w_add);
-                top = max(top, abs_bits(v[i][j]));
+                top = max_abs(top, v[i][j]);
             }
             if (h_out != nullptr) store8(h_out + base + c, v[i]);
         }
@@ -90,23 +90,24 @@ void launch_norm(const void *x, const void *y, const float *w, float w_add, floa
 
 // A half warp per (row, 128-column block) of h = silu(gate) * up, 8 elements a thread. Gate and up stay FP32 until the one rounding
 // to e4m3.
-template <typename T>
+template <typename T, typename Index>
 __global__ void __launch_bounds__(256) swiglu_fp8_kernel(const T *gu, uint8_t *q, float *scale, int64_t rows, int I, int blocks) {
     const int64_t units = rows * blocks, stride = (int64_t)gridDim.x * (blockDim.x / 16);
     const int t = threadIdx.x & 15;
     for (int64_t u0 = (int64_t)blockIdx.x * (blockDim.x / 16); u0 < units; u0 += stride) {
         const int64_t u = u0 + threadIdx.x / 16;
-        const int64_t row = u / blocks;
+        const int64_t row = (Index)u / (Index)blocks;  // 32 bits where they hold it: a 64-bit division is 80 instructions
         const int b = (int)(u - row * blocks), c = b * kFp8Block + t * 8;
         const bool live = u < units && c < I;
         float h[8];
-        uint32_t top = 0;
+        float top = 0.f;
         if (live) {
             float g[8], up[8];
             load8(gu + row * 2 * I + c, g);
             load8(gu + row * 2 * I + I + c, up);
+            swiglu8(g, up, h);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) h[j] = silu_f(g[j]) * up[j], top = max(top, abs_bits(h[j]));
+            for (int j = 0; j < 8; ++j) top = max_abs(top, h[j]);
         }
         const float s = fp8_scale(half_warp_max(top));
         if (live) {
@@ -171,8 +172,13 @@ int strix_swiglu_fp8(const void *gu, uint8_t *q, float *scale, int64_t rows, int
     const int64_t units = rows * blocks, want = (units + 15) / 16, cap = (int64_t)sm_count() * 32;
     const unsigned grid = (unsigned)(want < cap ? want : cap);
     auto st = static_cast<cudaStream_t>(stream);
-    if (act == kF32) swiglu_fp8_kernel<float><<<grid, 256, 0, st>>>((const float *)gu, q, scale, rows, (int)I, blocks);
-    else swiglu_fp8_kernel<uint16_t><<<grid, 256, 0, st>>>((const uint16_t *)gu, q, scale, rows, (int)I, blocks);
+    const bool small = units + cap * 16 < (1ll << 31);
+#define SB_SWIGLU(T, INDEX) swiglu_fp8_kernel<T, INDEX><<<grid, 256, 0, st>>>((const T *)gu, q, scale, rows, (int)I, blocks)
+    if (act == kF32 && small) SB_SWIGLU(float, uint32_t);
+    else if (act == kF32) SB_SWIGLU(float, int64_t);
+    else if (small) SB_SWIGLU(uint16_t, uint32_t);
+    else SB_SWIGLU(uint16_t, int64_t);
+#undef SB_SWIGLU
     SB_LAUNCH_OK(fn, " ", act_name(act), " rows=", rows, " I=", I);
     return 0;
 }

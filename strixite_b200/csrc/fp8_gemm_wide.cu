@@ -101,12 +101,6 @@ __device__ __forceinline__ void fma2(float2 &a, float s, uint32_t v0, uint32_t v
         : "+f"(a.x), "+f"(a.y)
         : "f"(s), "r"(v0), "r"(v1));
 }
-__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
 // A tile: its first row of the weight stack, first weight row and block row inside its matrix, halves with weight rows in them, and this
 // CTA's rows - dense: rows first .. of x; grouped: the slots list[first .. first + n).
 struct Tile {
