@@ -21,7 +21,9 @@ namespace {
 
 using namespace sb;
 
-constexpr int kRouteThreads = 1024, kRouteWarps = 32;
+constexpr int kRouteThreads = 1024, kRouteWarps = 32, kMaxBuckets = 1024;
+constexpr int kRouteBlocks = 8;            // the portable cluster size
+constexpr int64_t kRouteClusterSlots = 2048;  // from here on a cluster groups the slots
 
 // Exclusive scan of one int per thread over the 1024-thread block: warp shuffles, then the 32 warp totals.
 __device__ int block_exclusive_scan(int v, int *warp_tot, int *total) {
@@ -61,10 +63,48 @@ __device__ int bucket_of_tile(const int *prefix, int B, int i) {
     return lo;
 }
 
-// One block. Warp w owns the contiguous slot segment [w * seg, (w + 1) * seg): it counts its slots per bucket in its own
-// row of `cnt`, the per-bucket prefix over the warps turns the counts into the warp's first position in each bucket,
-// and the warp then places its slots in slot order (ranks inside a 32-slot step by __match_any_sync). So a bucket
-// lists its slots ascending, whatever the scheduling: the permutation is a pure function of ids.
+// Exclusive scan of three sums at once: a block's slots, 16-slot tiles and 64-slot tiles, packed into 21 + 21 + 21 bits (S <= 2^20).
+__device__ uint64_t block_exclusive_scan3(int count, uint64_t *warp_tot, uint64_t *total) {
+    const uint64_t v = (uint64_t)count | (uint64_t)((count + 15) / 16) << 21 | (uint64_t)((count + 63) / 64) << 42;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint64_t incl = v;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const uint64_t o = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += o;
+    }
+    if (lane == 31) warp_tot[warp] = incl;
+    __syncthreads();
+    if (warp == 0) {
+        const uint64_t t = warp_tot[lane];
+        uint64_t ti = t;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const uint64_t o = __shfl_up_sync(0xffffffffu, ti, off);
+            if (lane >= off) ti += o;
+        }
+        warp_tot[lane] = ti - t;
+        if (lane == 31) *total = ti;
+    }
+    __syncthreads();
+    return warp_tot[warp] + incl - v;
+}
+
+__device__ __forceinline__ uint32_t peer_u32(const void *p, uint32_t rank) {  // a word of another block of the cluster
+    uint32_t at = (uint32_t)__cvta_generic_to_shared(p), v;
+    asm volatile("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(at) : "r"(rank));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_meet() { asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory"); }
+
+// One block, or (CLUSTER) the blocks of one cluster. Warp w of the whole owns the contiguous slot segment [w * seg, (w + 1) * seg): it counts
+// its slots per bucket in its own row of `cnt`, the per-bucket prefix over the warps (and over the blocks in front, read from their
+// shared memory) turns the counts into the warp's first position in each bucket, and the warp then places its slots in slot order (ranks inside a
+// 32-slot step by __match_any_sync). So a bucket lists its slots ascending, whatever the scheduling: the permutation is a pure
+// function of ids. Bound by the latency of the steps of a segment: 40960 slots over 513 buckets took 53 us in one block, 8 blocks
+// cut the steps to an eighth.
+template <bool CLUSTER>
 __global__ void __launch_bounds__(kRouteThreads)
     route_kernel(const int32_t *ids, int S, int E, int Tmax, int WTmax, int32_t *ws, uint32_t *err) {
     extern __shared__ int smem[];
@@ -73,67 +113,97 @@ __global__ void __launch_bounds__(kRouteThreads)
     int *start = cnt + kRouteWarps * B;   // [B + 1] first slot position of each bucket
     int *tile0 = start + B + 1;           // [B + 1] first 16-slot tile of each bucket
     int *wtile0 = tile0 + B + 1;          // [B + 1] first 64-slot tile
-    int *warp_tot = wtile0 + B + 1;       // [32]
-    __shared__ int first_bad, total_a, total_b, total_c;
+    __shared__ int first_bad;
+    __shared__ uint64_t warp_tot[kRouteWarps], total;
+    __shared__ int block_count[kMaxBuckets];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    for (int i = t; i < kRouteWarps * B; i += kRouteThreads) cnt[i] = 0;
+    const int rank = CLUSTER ? (int)blockIdx.x : 0, blocks = CLUSTER ? (int)gridDim.x : 1;  // the grid is one cluster
+    const int seg = ((S + kRouteWarps * blocks - 1) / (kRouteWarps * blocks) + 31) & ~31;
+    const int s_begin = min(S, (rank * kRouteWarps + warp) * seg), s_end = min(S, s_begin + seg);
+    const int left = S - rank * kRouteWarps * seg, live_warps = left <= 0 ? 0 : min(kRouteWarps, (left + seg - 1) / seg);  // with slots of their own
+    for (int i = t; i < live_warps * B; i += kRouteThreads) cnt[i] = 0;
     if (t == 0) first_bad = 0x7fffffff;
     __syncthreads();
-    const int seg = ((S + kRouteWarps - 1) / kRouteWarps + 31) & ~31;
-    const int s_begin = min(S, warp * seg), s_end = min(S, s_begin + seg);
-    for (int s = s_begin + lane; s < s_end; s += 32) {
-        const int32_t id = ids[s];
-        const bool bad = id < 0 || id >= E;
-        atomicAdd(&cnt[warp * B + (bad ? E : id)], 1);
-        if (bad) atomicMin(&first_bad, s);
+    for (int s0 = s_begin + lane; s0 < s_end; s0 += 128) {  // four ids in flight
+        int32_t id[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) id[j] = s0 + 32 * j < s_end ? ids[s0 + 32 * j] : 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (s0 + 32 * j >= s_end) continue;
+            const bool bad = id[j] < 0 || id[j] >= E;
+            atomicAdd(&cnt[warp * B + (bad ? E : id[j])], 1);
+            if (bad) atomicMin(&first_bad, s0 + 32 * j);
+        }
     }
     __syncthreads();
-    if (t == 0 && first_bad != 0x7fffffff) raise_err(err, (uint32_t)ids[first_bad], (uint32_t)first_bad);
     int count = 0;
     if (t < B) {
-        for (int w = 0; w < kRouteWarps; ++w) {
+        for (int w = 0; w < live_warps; ++w) {
             const int c = cnt[w * B + t];
-            cnt[w * B + t] = count;  // this warp's first rank inside the bucket
+            cnt[w * B + t] = count;  // this warp's first rank inside the block's share of the bucket
             count += c;
         }
     }
-    const int st = block_exclusive_scan(count, warp_tot, &total_a);
-    const int tl = block_exclusive_scan((count + 15) / 16, warp_tot, &total_b);
-    const int wt = block_exclusive_scan((count + 63) / 64, warp_tot, &total_c);
+    int before = 0;  // slots of bucket t in the blocks in front
+    if constexpr (CLUSTER) {
+        if (t < B) block_count[t] = count;
+        cluster_meet();
+        if (t < B) {
+            count = 0;
+            for (int r = 0; r < blocks; ++r) {
+                const int c = (int)peer_u32(&block_count[t], r);
+                before += r < rank ? c : 0;
+                count += c;
+            }
+        }
+        if (rank == 0 && t == 0)
+            for (int r = 1; r < blocks; ++r) first_bad = min(first_bad, (int)peer_u32(&first_bad, r));
+    }
+    if (rank == 0 && t == 0 && first_bad != 0x7fffffff) raise_err(err, (uint32_t)ids[first_bad], (uint32_t)first_bad);
+    const uint64_t sums = block_exclusive_scan3(count, warp_tot, &total);
+    constexpr uint64_t kField = (1u << 21) - 1;
+    const int st = (int)(sums & kField), tl = (int)(sums >> 21 & kField), wt = (int)(sums >> 42);
+    const int total_a = (int)(total & kField), total_b = (int)(total >> 21 & kField), total_c = (int)(total >> 42);
     int32_t *offsets = ws + 4, *slots = offsets + E + 2, *tile_bucket = slots + S, *tile_start = tile_bucket + Tmax;
     int32_t *wtile_bucket = tile_start + Tmax, *wtile_start = wtile_bucket + WTmax;
-    if (t < B) start[t] = st, tile0[t] = tl, wtile0[t] = wt, offsets[t] = st;
+    if (t < B) {
+        start[t] = st, tile0[t] = tl, wtile0[t] = wt;
+        for (int w = 0; w < live_warps; ++w) cnt[w * B + t] += st + before;  // from here on: the warp's next position in the bucket
+        if (rank == 0) offsets[t] = st;
+    }
     if (t == 0) {
         start[B] = total_a, tile0[B] = total_b, wtile0[B] = total_c;
-        ws[0] = total_b, ws[1] = S, ws[2] = E, ws[3] = total_c;
-        offsets[E + 1] = total_a;
+        if (rank == 0) {
+            ws[0] = total_b, ws[1] = S, ws[2] = E, ws[3] = total_c;
+            offsets[E + 1] = total_a;
+        }
     }
     __syncthreads();
-    for (int i = t; i < total_b; i += kRouteThreads) {
+    for (int i = rank * kRouteThreads + t; i < total_b; i += kRouteThreads * blocks) {
         const int b = bucket_of_tile(tile0, B, i);
         tile_bucket[i] = b, tile_start[i] = start[b] + (i - tile0[b]) * 16;
     }
-    for (int i = t; i < total_c; i += kRouteThreads) {
+    for (int i = rank * kRouteThreads + t; i < total_c; i += kRouteThreads * blocks) {
         const int b = bucket_of_tile(wtile0, B, i);
         wtile_bucket[i] = b, wtile_start[i] = start[b] + (i - wtile0[b]) * 64;
     }
+    int32_t ahead = s_begin + lane < s_end ? ids[s_begin + lane] : 0;
     for (int s0 = s_begin; s0 < s_end; s0 += 32) {
         const int s = s0 + lane;
         const bool live = s < s_end;
+        const int32_t id = ahead;
+        if (s + 32 < s_end) ahead = ids[s + 32];
         int b = 0x40000000 | lane;  // idle lanes: a bucket of their own
-        if (live) {
-            const int32_t id = ids[s];
-            b = (id < 0 || id >= E) ? E : id;
-        }
+        if (live) b = (id < 0 || id >= E) ? E : id;
         const unsigned same = __match_any_sync(0xffffffffu, b);
-        const int rank = __popc(same & ((1u << lane) - 1u));
-        if (live) {
-            slots[start[b] + cnt[warp * B + b] + rank] = s;
-        }
+        const int place = __popc(same & ((1u << lane) - 1u));
+        if (live) slots[cnt[warp * B + b] + place] = s;
         __syncwarp();
-        if (live && rank == 0) cnt[warp * B + b] += __popc(same);
+        if (live && place == 0) cnt[warp * B + b] += __popc(same);
         __syncwarp();
     }
+    if constexpr (CLUSTER) cluster_meet();  // nobody's counts go while another block reads them
 }
 
 // ---- the same grouping over many blocks (the layer object's path; it owns the scratch) -------------------------------
@@ -574,17 +644,31 @@ int strix_moe_group_routes(const int32_t *ids, int64_t M, int64_t A, int64_t E, 
     SB_TRY(sb::route_ints(M, A, E, &ints));
     SB_CHECK(ws_bytes >= (size_t)ints * 4, fn, ": workspace of ", ws_bytes, " bytes, needs ", ints * 4);
     const int64_t S = M * A;
-    const size_t smem = (size_t)(kRouteWarps * (E + 1) + 3 * (E + 2) + 32) * sizeof(int);
+    const size_t smem = (size_t)(kRouteWarps * (E + 1) + 3 * (E + 2)) * sizeof(int);
     static thread_local int attr_dev = -1;
     int dev = 0;
     SB_CUDA(cudaGetDevice(&dev), fn);
     if (attr_dev != dev) {
-        SB_CUDA(cudaFuncSetAttribute(route_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024), fn,
+        SB_CUDA(cudaFuncSetAttribute(route_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024), fn,
+                ": raising the shared-memory limit");
+        SB_CUDA(cudaFuncSetAttribute(route_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024), fn,
                 ": raising the shared-memory limit");
         attr_dev = dev;
     }
-    route_kernel<<<1, kRouteThreads, smem, static_cast<cudaStream_t>(stream)>>>(ids, (int)S, (int)E, (int)(S / 16 + E + 2),
-                                                                               (int)(S / 64 + E + 2), static_cast<int32_t *>(ws), err);
+    auto st = static_cast<cudaStream_t>(stream);
+    auto *wi = static_cast<int32_t *>(ws);
+    const int Tmax = (int)(S / 16 + E + 2), WTmax = (int)(S / 64 + E + 2);
+    if (S < kRouteClusterSlots) {
+        route_kernel<false><<<1, kRouteThreads, smem, st>>>(ids, (int)S, (int)E, Tmax, WTmax, wi, err);
+    } else {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(kRouteBlocks), cfg.blockDim = dim3(kRouteThreads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = kRouteBlocks, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr, cfg.numAttrs = 1;
+        SB_CUDA(cudaLaunchKernelEx(&cfg, route_kernel<true>, ids, (int)S, (int)E, Tmax, WTmax, wi, err), fn, " M=", M, " A=", A, " E=", E);
+    }
     SB_LAUNCH_OK(fn, " M=", M, " A=", A, " E=", E);
     return 0;
 }

@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 import torch
 
+import oracle
 from fp8_ref import FP8, blocks, check_fp8_rows, product_bound, route, rows_fp8, stack_fp8, wide_matrix, wide_rows, matrix_fp8
 from strixite_b200 import StrixError
 from strixite_b200 import kernels as K
@@ -308,6 +309,30 @@ def test_experts_refuse_a_workspace_of_other_sizes():
     before = K.workspace_refusal_count()
     K.linear_fp8_experts_gather_grouped(xq, xs, K.Fp8Weight(wq, wsc, experts=E), E, ws, n, 11, 1, y, K.Act.F32)
     assert K.workspace_refusal_count() == before + 1 and (y == 7.0).all()
+
+
+@pytest.mark.parametrize("M,A,E", [(2047, 1, 5), (2048, 1, 1023), (1, 64, 1), (700, 3, 512), (4097, 11, 513), (16384, 64, 1023), (65536, 10, 8)])
+def test_grouping_by_one_block_and_by_a_cluster(M, A, E):
+    """The workspace is a pure function of the ids, whichever form groups them (one block below 2048 slots, a cluster from there on)."""
+    rng = np.random.default_rng(M + A)
+    ids = rng.integers(0, E, (M, A)).astype(np.int32)
+    ids[rng.random((M, A)) < 0.3] = E - 1
+    if M > 1000:
+        ids[M // 2, 0], ids[M - 1, A - 1] = -5, E
+    ref, err_ref = oracle.group_routes(ids, E)
+    t = torch.from_numpy(ids).cuda()
+    n = K.moe_route_workspace_bytes(M, A, E)
+    for _ in range(2):
+        ws, err = torch.full((n // 4,), -99, dtype=torch.int32, device="cuda"), K.new_err()
+        K.moe_group_routes(t, M, A, E, ws, n, err)
+        got = ws.cpu().numpy()
+        head = 4 + E + 2 + M * A
+        assert np.array_equal(got[:head], ref[:head])
+        Tmax, WTmax = M * A // 16 + E + 2, M * A // 64 + E + 2
+        for at, size, count in ((head, Tmax, ref[0]), (head + 2 * Tmax, WTmax, ref[3])):
+            for col in (at, at + size):
+                assert np.array_equal(got[col : col + count], ref[col : col + count])
+        assert host_err(err) == [int(v) for v in err_ref[:3]]
 
 
 # ---- the run ---------------------------------------------------------------------------------------------------------
