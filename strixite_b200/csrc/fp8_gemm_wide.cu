@@ -10,7 +10,7 @@
 // bounds the one-CTA form. GROUP = 1 (the experts' slots, gathered by row): an expert has seldom more than 128 rows.
 //
 // Roles: warps 0-3 / 4-7 promote column half 0 / 1 (each half has two accumulators, so the tensor cores run up to three half blocks
-// ahead), warp 8 issues TMA, warp 9 issues the MMAs (of CTA 0 for both CTAs). The sums leave through a 64-byte-wide staging strip per warp so that a
+// ahead), warp 8 issues TMA, warp 9 issues the MMAs (of CTA 0 for both CTAs), warp 10 gathers rows of x. The sums leave through a 64-byte-wide staging strip per warp so that a
 // store covers whole sectors of a row.
 // Every mbarrier wait is bounded: on expiry the CTA raises the abort counter, waits for its copies, frees its tensor memory, returns.
 #include <algorithm>
@@ -29,10 +29,13 @@ constexpr int kRows = 128;               // rows of x per CTA = accumulator lane
 constexpr int kColTile = 256;            // weight rows per tile
 constexpr int kHalf = 128;               // columns of a promotion warpgroup: one block row of weight scales
 constexpr int kPromoWarps = 8;
-constexpr int kTmaWarp = 8, kMmaWarp = 9;
-constexpr int kThreads = 12 * 32;        // three warpgroups; two warps of the last one are idle
+constexpr int kTmaWarp = 8, kMmaWarp = 9, kGatherWarp = 10;
 constexpr int kStripPitch = 80;          // 64 bytes of a row + 16: rows start in different banks
 constexpr int kStrip = 32 * kStripPitch;
+
+// Three warpgroups. Registers move from the last one to the two that promote (a thread of theirs holds 128 sums):
+// 2 * 128 * 208 + 128 * 64 <= 3 * 128 * 168, what the block is launched with.
+constexpr int kThreads = 12 * 32;
 
 template <int GROUP>
 struct Cfg {
@@ -167,7 +170,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         return t;
     };
 
-    if (warp == kTmaWarp) {
+    if (warp >= kPromoWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == kTmaWarp || (GROUPED && warp == kGatherWarp)) {
+        // One warp for the boxes; grouped, another for the rows of x: a gather of four rows is an instruction of its own, 32 of them a
+        // block of K would hold up the weights.
         uint32_t it = 0;
         bool ok = true;
         for (int p = blockIdx.x / GROUP; p < n_tiles && ok; p += step) {
@@ -177,15 +184,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             if constexpr (GROUPED) {
                 // rows beyond the list's end repeat its last one; whole quads beyond it are not fetched, and what their lanes compute is
                 // not stored
-                for (int j = 0; j < 4; ++j) rows[j] = rt.slots[t.first + min(lane * 4 + j, t.n - 1)] / a.div;
                 bytes = C::BTile + (uint32_t)((t.n + 3) / 4) * 4 * kBK;
+                if (warp == kGatherWarp)
+                    for (int j = 0; j < 4; ++j) rows[j] = rt.slots[t.first + min(lane * 4 + j, t.n - 1)] / a.div;
             }
             for (int kb = 0; kb < a.KB; ++kb, ++it) {
                 const int s = it % C::Stages;
                 ok = __all_sync(0xffffffffu, mbar_wait(&ctl.empty[s], ((it / C::Stages) & 1u) ^ 1u, abort_flag));
                 if (!ok) break;
                 uint8_t *dst = base + s * C::StageBytes;
-                if (elect_one()) {
+                if (GROUPED && warp == kGatherWarp) {
+                    if (lane * 4 < t.n) tma_gather4(dst + lane * 4 * kBK, &x_map, kb * kBK, rows[0], rows[1], rows[2], rows[3], &ctl.full[s]);
+                } else if (elect_one()) {
                     if constexpr (GROUP == 2) {
                         // the leader's barrier counts both CTAs' bytes; this CTA's weight rows are the rank-th 64 of each half, so that a
                         // half's instruction (64 rows from each CTA) covers 128 neighbouring rows
@@ -196,14 +206,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tma_load_pair(dst + C::ATile + 64 * kBK, &w_map, kb * kBK, t.wrow + kHalf + (int)rank * 64, bar);
                     } else {
                         mbar_expect_tx(&ctl.full[s], bytes);
-                        for (int i = 0; i < 4; ++i) tma_load_2d(dst + C::ATile + i * 64 * kBK, &w_map, kb * kBK, t.wrow + i * 64, &ctl.full[s]);
+                        tma_load_2d(dst + C::ATile, &w_map, kb * kBK, t.wrow, &ctl.full[s]);
                         if constexpr (!GROUPED) tma_load_2d(dst, &x_map, kb * kBK, t.first, &ctl.full[s]);
                     }
                 }
                 __syncwarp();
-                if constexpr (GROUPED) {
-                    if (lane * 4 < t.n) tma_gather4(dst + lane * 4 * kBK, &x_map, kb * kBK, rows[0], rows[1], rows[2], rows[3], &ctl.full[s]);
-                }
             }
         }
         // The last blocks' MMAs have read their stages and signalled it; after an abandoned wait, the copies in flight have landed.
@@ -246,17 +253,26 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         }
-    } else if (warp < kPromoWarps) {
+    }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int h = warp >> 2, r = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + h * kHalf;
         uint8_t *strip = strips + warp * kStrip;
         uint32_t done = 0;
         bool ok = true;
-        for (int p = blockIdx.x / GROUP; p < n_tiles && ok; p += step) {
-            const Tile t = tile_of(p);
-            if (h >= t.halves) continue;
-            int64_t row = t.first + r;  // of y
-            const float *xp = nullptr;  // this thread's scales: null beyond the rows
+        // What a tile starts with - its rows and first scales, up to three dependent loads - is fetched before the store of the tile in
+        // front of it.
+        Tile t{};
+        int64_t row = 0;            // of y
+        const float *xp = nullptr;  // this thread's scales: null beyond the rows
+        const float *wp = nullptr;
+        float sx[2] = {0.f, 0.f}, sw[2] = {0.f, 0.f};  // of the next two blocks
+        auto fetch = [&](int p) {
+            if (p >= n_tiles) return;
+            t = tile_of(p);
+            if (h >= t.halves) return;
+            row = t.first + r, xp = nullptr;
             if (r < t.n) {
                 int64_t from = row;
                 if constexpr (GROUPED) {
@@ -265,14 +281,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 xp = a.xs + from * a.KB;
             }
-            const float *wp = a.ws + (int64_t)(t.ws_row + h) * a.KB;
+            wp = a.ws + (int64_t)(t.ws_row + h) * a.KB;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (i < a.KB) sx[i] = xp != nullptr ? xp[i] : 0.f, sw[i] = wp[i];
+        };
+        fetch(blockIdx.x / GROUP);
+        for (int p = blockIdx.x / GROUP; p < n_tiles; p += step) {
+            if (h >= t.halves) {
+                fetch(p + step);
+                continue;
+            }
             float2 acc[kHalf / 2];
 #pragma unroll
             for (int j = 0; j < kHalf / 2; ++j) acc[j] = make_float2(0.f, 0.f);
-            float sx = xp != nullptr ? xp[0] : 0.f, sw = wp[0];
             for (int kb = 0; kb < a.KB; ++kb, ++done) {
-                const float s = sx * sw;
-                if (kb + 1 < a.KB) sx = xp != nullptr ? xp[kb + 1] : 0.f, sw = wp[kb + 1];  // under the next wait
+                const float s = sx[0] * sw[0];
+                sx[0] = sx[1], sw[0] = sw[1];
+                if (kb + 2 < a.KB) sx[1] = xp != nullptr ? xp[kb + 2] : 0.f, sw[1] = wp[kb + 2];
                 const uint32_t b = done & 1u;
                 ok = __all_sync(0xffffffffu, mbar_wait(&ctl.acc_full[h][b], (done >> 1) & 1u, abort_flag));
                 if (!ok) break;
@@ -286,29 +312,34 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int j = 0; j < 16; j += 2) fma2(acc[(c + j) / 2], s, v0[j], v0[j + 1]);
                     tmem_ld_wait();
-                    if (c + 32 < kHalf) tmem_ld16(lanes + b * 2 * kHalf + c + 32, v0);
+                    if (c + 32 < kHalf) {
+                        tmem_ld16(lanes + b * 2 * kHalf + c + 32, v0);
+                    } else {  // everything is in registers: the accumulator is free
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if constexpr (GROUP == 2) arrive_at(peer_addr(&ctl.acc_empty[h][b], 0));
+                            else mbar_arrive(&ctl.acc_empty[h][b]);
+                        }
+                    }
 #pragma unroll
                     for (int j = 0; j < 16; j += 2) fma2(acc[(c + 16 + j) / 2], s, v1[j], v1[j + 1]);
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    if constexpr (GROUP == 2) arrive_at(peer_addr(&ctl.acc_empty[h][b], 0));
-                    else mbar_arrive(&ctl.acc_empty[h][b]);
-                }
             }
             if (!ok) break;
+            const int n_rows = t.n, n_base = t.n0 + h * kHalf;
+            const int64_t out_row = row;
+            fetch(p + step);
             // y: 64 bytes of every row at a time through the strip; then 4 lanes write a row's 64 bytes, 8 rows an instruction
             const int es = a.out_f32 ? 4 : 2, per = 64 / es;  // columns of a strip
             const bool wide = ((int64_t)a.N * es) % 16 == 0 && reinterpret_cast<uintptr_t>(a.y) % 16 == 0;
-            const int n_base = t.n0 + h * kHalf;
             auto flush = [&](int col) {  // columns col .. col + per of the half
                 __syncwarp();
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int rr = i * 8 + (lane >> 2), n = n_base + col + (lane & 3) * (16 / es);
-                    const int64_t orow = __shfl_sync(0xffffffffu, row, rr);
-                    const bool live = (warp & 3) * 32 + rr < t.n;
+                    const int64_t orow = __shfl_sync(0xffffffffu, out_row, rr);
+                    const bool live = (warp & 3) * 32 + rr < n_rows;
                     const uint4 q = *reinterpret_cast<const uint4 *>(strip + rr * kStripPitch + (lane & 3) * 16);
                     uint8_t *dst = static_cast<uint8_t *>(a.y) + (orow * a.N + n) * es;
                     if (!live) continue;
@@ -373,7 +404,7 @@ int launch(const char *fn, const uint8_t *w, int64_t w_rows, const uint8_t *x, i
         prepared = dev;
     }
     CUtensorMap wm, xm;
-    SB_TRY(make_map(fn, &wm, w, w_rows, K, 64));
+    SB_TRY(make_map(fn, &wm, w, w_rows, K, GROUP == 2 ? 64 : kColTile));
     SB_TRY(make_map(fn, &xm, x, x_rows, K, GROUPED ? 1 : kRows));
     a.NT = (a.N + kColTile - 1) / kColTile;
     const int64_t all = tiles * a.NT, room = sm_count() / GROUP;
