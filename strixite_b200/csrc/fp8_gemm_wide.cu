@@ -10,7 +10,7 @@
 // bounds the one-CTA form. GROUP = 1 (the experts' slots, gathered by row): an expert has seldom more than 128 rows.
 //
 // Roles: warps 0-3 / 4-7 promote column half 0 / 1 (each half has two accumulators, so the tensor cores run up to three half blocks
-// ahead), warp 8 issues TMA, warp 9 issues the MMAs (of CTA 0 for both CTAs), warp 10 gathers rows of x. The sums leave through a 64-byte-wide staging strip per warp so that a
+// ahead), warp 8 issues TMA, warps 9 and 10 the MMAs of half 0 and 1 (those of CTA 0 for both CTAs), warp 11 gathers rows of x. The sums leave through a 64-byte-wide staging strip per warp so that a
 // store covers whole sectors of a row.
 // Every mbarrier wait is bounded: on expiry the CTA raises the abort counter, waits for its copies, frees its tensor memory, returns.
 #include <algorithm>
@@ -29,12 +29,12 @@ constexpr int kRows = 128;               // rows of x per CTA = accumulator lane
 constexpr int kColTile = 256;            // weight rows per tile
 constexpr int kHalf = 128;               // columns of a promotion warpgroup: one block row of weight scales
 constexpr int kPromoWarps = 8;
-constexpr int kTmaWarp = 8, kMmaWarp = 9, kGatherWarp = 10;
+constexpr int kTmaWarp = 8, kMmaWarp = 9, kGatherWarp = 11;  // two MMA warps
 constexpr int kStripPitch = 80;          // 64 bytes of a row + 16: rows start in different banks
 constexpr int kStrip = 32 * kStripPitch;
 
 // Three warpgroups. Registers move from the last one to the two that promote (a thread of theirs holds 128 sums):
-// 2 * 128 * 208 + 128 * 64 <= 3 * 128 * 168, what the block is launched with.
+// 2 * 128 * 216 + 128 * 64 <= 3 * 128 * 168, what the block is launched with.
 constexpr int kThreads = 12 * 32;
 
 template <int GROUP>
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (GROUPED && !ws_is_for(a.group, a.S, a.E, &g_wide_refusals)) return;  // the whole grid leaves
     const uint32_t rank = GROUP == 2 ? cluster_rank() : 0;
     if (tid == 0) {
-        for (int i = 0; i < C::Stages; ++i) mbar_init(&ctl.full[i], 1), mbar_init(&ctl.empty[i], 1);
+        for (int i = 0; i < C::Stages; ++i) mbar_init(&ctl.full[i], 1), mbar_init(&ctl.empty[i], 2);  // empty: both halves' MMAs
         for (int i = 0; i < 4; ++i) mbar_init(&ctl.acc_full[i / 2][i % 2], 1), mbar_init(&ctl.acc_empty[i / 2][i % 2], 4 * GROUP);
         ctl.abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -221,44 +221,51 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
         }
         __syncwarp();
-    } else if (warp == kMmaWarp && rank == 0) {
-        constexpr uint32_t idesc_m = kRows * GROUP;
-        const uint32_t idesc = idesc_e4m3(idesc_m, kHalf);
-        uint32_t it = 0, done[2] = {0, 0};
-        bool ok = true;
-        for (int p = blockIdx.x / GROUP; p < n_tiles && ok; p += step) {
-            const Tile t = tile_of(p);
-            for (int kb = 0; kb < a.KB && ok; ++kb, ++it) {
-                const int s = it % C::Stages;
-                ok = __all_sync(0xffffffffu, mbar_wait(&ctl.full[s], (it / C::Stages) & 1u, abort_flag));
-                if (!ok) break;
-                const uint32_t at = smem_u32(base + s * C::StageBytes);
-                const uint64_t da = umma_desc(at);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (h >= t.halves || !ok) continue;
-                    const uint32_t b = done[h] & 1u;
-                    ok = __all_sync(0xffffffffu, mbar_wait(&ctl.acc_empty[h][b], ((done[h] >> 1) & 1u) ^ 1u, abort_flag));
-                    if (!ok) continue;
-                    tc_fence_after();
-                    if (elect_one()) {
-                        const uint64_t db = umma_desc(at + C::ATile + h * (C::BTile / 2));
+    } else if ((warp == kMmaWarp || warp == kMmaWarp + 1) && rank == 0) {
+        // One thread per half: a half whose accumulators are still being read does not hold up the other. A probe of a barrier takes ~100
+        // clocks to answer even when the phase is over (measured), so the two that a block of K needs are asked under the MMAs of the
+        // block in front of it; only one that was not over then is waited for.
+        if (elect_one()) {
+            const int h = warp - kMmaWarp;
+            const uint32_t idesc = idesc_e4m3(kRows * GROUP, kHalf);
+            uint32_t it = 0, done = 0;
+            bool ok = true, full = false, free = true;  // fresh accumulators are free
+            for (int p = blockIdx.x / GROUP; p < n_tiles && ok; p += step) {
+                const Tile t = tile_of(p);
+                for (int kb = 0; kb < a.KB; ++kb) {
+                    const int s = it % C::Stages;
+                    if (!full) ok = mbar_wait(&ctl.full[s], (it / C::Stages) & 1u, abort_flag);
+                    if (!ok) break;
+                    ++it;
+                    if (h < t.halves) {
+                        const uint32_t b = done & 1u;
+                        if (!free) ok = mbar_wait(&ctl.acc_empty[h][b], ((done >> 1) & 1u) ^ 1u, abort_flag);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t at = smem_u32(base + s * C::StageBytes);
+                        const uint64_t da = umma_desc(at), db = umma_desc(at + C::ATile + h * (C::BTile / 2));
 #pragma unroll
                         for (int k = 0; k < kBK / 32; ++k) umma_f8<GROUP>(tmem + (b * 2 + h) * kHalf, da + 2 * k, db + 2 * k, idesc, k != 0);
-                        if (h == t.halves - 1) commit<GROUP>(&ctl.empty[s]);
+                        ++done;
+                        free = mbar_test(&ctl.acc_empty[h][done & 1u], ((done >> 1) & 1u) ^ 1u);
+                        full = mbar_test(&ctl.full[it % C::Stages], (it / C::Stages) & 1u);
                         commit<GROUP>(&ctl.acc_full[h][b]);
+                        commit<GROUP>(&ctl.empty[s]);
+                    } else {
+                        full = false;
+                        commit<GROUP>(&ctl.empty[s]);  // nothing of this half reads the stage
                     }
-                    __syncwarp();
-                    ++done[h];
                 }
             }
         }
+        __syncwarp();
     }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int h = warp >> 2, r = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + h * kHalf;
         uint8_t *strip = strips + warp * kStrip;
+        const uint32_t empty_at = peer_addr(&ctl.acc_empty[0][0], 0);  // the leader's
         uint32_t done = 0;
         bool ok = true;
         // What a tile starts with - its rows and first scales, up to three dependent loads - is fetched before the store of the tile in
@@ -295,36 +302,47 @@ __global__ void __launch_bounds__(kThreads, 1)
             float2 acc[kHalf / 2];
 #pragma unroll
             for (int j = 0; j < kHalf / 2; ++j) acc[j] = make_float2(0.f, 0.f);
-            for (int kb = 0; kb < a.KB; ++kb, ++done) {
+            // A quarter of the columns is loaded while the one in front of it is added; the last quarter of a block is added under the
+            // first load of the next block, whose barrier was asked about a quarter earlier.
+            uint32_t v0[32], v1[32];
+            auto add = [&](const uint32_t(&v)[32], int quarter, float s) {
+#pragma unroll
+                for (int j = 0; j < 32; j += 2) fma2(acc[quarter * 16 + j / 2], s, v[j], v[j + 1]);
+            };
+            ok = __all_sync(0xffffffffu, mbar_wait(&ctl.acc_full[h][done & 1u], (done >> 1) & 1u, abort_flag));
+            if (!ok) break;
+            tc_fence_after();
+            tmem_ld32(lanes + (done & 1u) * 2 * kHalf, v0);
+            for (int kb = 0; kb < a.KB; ++kb) {
                 const float s = sx[0] * sw[0];
                 sx[0] = sx[1], sw[0] = sw[1];
                 if (kb + 2 < a.KB) sx[1] = xp != nullptr ? xp[kb + 2] : 0.f, sw[1] = wp[kb + 2];
-                const uint32_t b = done & 1u;
-                ok = __all_sync(0xffffffffu, mbar_wait(&ctl.acc_full[h][b], (done >> 1) & 1u, abort_flag));
-                if (!ok) break;
-                tc_fence_after();
-                uint32_t v0[16], v1[16];
-                tmem_ld16(lanes + b * 2 * kHalf, v0);
-#pragma unroll
-                for (int c = 0; c < kHalf; c += 32) {
-                    tmem_ld_wait();
-                    tmem_ld16(lanes + b * 2 * kHalf + c + 16, v1);
-#pragma unroll
-                    for (int j = 0; j < 16; j += 2) fma2(acc[(c + j) / 2], s, v0[j], v0[j + 1]);
-                    tmem_ld_wait();
-                    if (c + 32 < kHalf) {
-                        tmem_ld16(lanes + b * 2 * kHalf + c + 32, v0);
-                    } else {  // everything is in registers: the accumulator is free
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) {
-                            if constexpr (GROUP == 2) arrive_at(peer_addr(&ctl.acc_empty[h][b], 0));
-                            else mbar_arrive(&ctl.acc_empty[h][b]);
-                        }
-                    }
-#pragma unroll
-                    for (int j = 0; j < 16; j += 2) fma2(acc[(c + 16 + j) / 2], s, v1[j], v1[j + 1]);
+                const uint32_t b = done & 1u, from = lanes + b * 2 * kHalf;
+                ++done;
+                tmem_ld_wait();
+                tmem_ld32(from + 32, v1);
+                add(v0, 0, s);
+                tmem_ld_wait();
+                tmem_ld32(from + 64, v0);
+                add(v1, 1, s);
+                tmem_ld_wait();
+                tmem_ld32(from + 96, v1);
+                const bool more = kb + 1 < a.KB, ready = more && mbar_test(&ctl.acc_full[h][done & 1u], (done >> 1) & 1u);
+                add(v0, 2, s);
+                tmem_ld_wait();  // everything is in registers: the accumulator is free
+                tc_fence_before();
+                __syncwarp();
+                if (elect_one()) {
+                    if constexpr (GROUP == 2) arrive_at(empty_at + (h * 2 + b) * 8);
+                    else mbar_arrive(&ctl.acc_empty[h][b]);
                 }
+                if (more) {
+                    if (!__all_sync(0xffffffffu, ready)) ok = __all_sync(0xffffffffu, mbar_wait(&ctl.acc_full[h][done & 1u], (done >> 1) & 1u, abort_flag));
+                    if (!ok) break;
+                    tc_fence_after();
+                    tmem_ld32(lanes + (done & 1u) * 2 * kHalf, v0);
+                }
+                add(v1, 3, s);
             }
             if (!ok) break;
             const int n_rows = t.n, n_base = t.n0 + h * kHalf;
