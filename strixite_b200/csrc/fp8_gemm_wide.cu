@@ -10,7 +10,7 @@
 // bounds the one-CTA form. GROUP = 1 (the experts' slots, gathered by row): an expert has seldom more than 128 rows.
 //
 // Roles: warps 0-3 / 4-7 promote column half 0 / 1 (each half has two accumulators, so the tensor cores run up to three half blocks
-// ahead), warp 8 issues TMA, warps 9 and 10 the MMAs of half 0 and 1 (those of CTA 0 for both CTAs), warp 11 gathers rows of x. The sums leave through a 64-byte-wide staging strip per warp so that a
+// ahead), warp 8 issues TMA, warps 9 and 10 the MMAs of half 0 and 1 (those of CTA 0 for both CTAs), warps 11-15 gather rows of x. The sums leave through a 64-byte-wide staging strip per warp so that a
 // store covers whole sectors of a row.
 // Every mbarrier wait is bounded: on expiry the CTA raises the abort counter, waits for its copies, frees its tensor memory, returns.
 #include <algorithm>
@@ -33,9 +33,11 @@ constexpr int kTmaWarp = 8, kMmaWarp = 9, kGatherWarp = 11;  // two MMA warps
 constexpr int kStripPitch = 80;          // 64 bytes of a row + 16: rows start in different banks
 constexpr int kStrip = 32 * kStripPitch;
 
-// Three warpgroups. Registers move from the last one to the two that promote (a thread of theirs holds 128 sums):
-// 2 * 128 * 216 + 128 * 64 <= 3 * 128 * 168, what the block is launched with.
-constexpr int kThreads = 12 * 32;
+// Two warpgroups promote, one (grouped: two, for the gathers) does the rest. Registers move to the former, a thread of which holds 128
+// sums: 2 * 128 * 208 + 128 * 64 <= 3 * 128 * 168 and 2 * 128 * 208 + 2 * 128 * 48 = 4 * 128 * 128, what the block is launched with.
+template <bool GROUPED>
+constexpr int kThreads = (GROUPED ? 16 : 12) * 32;
+constexpr int kGatherWarps = 5;
 
 template <int GROUP>
 struct Cfg {
@@ -111,7 +113,7 @@ struct Tile {
 };
 
 template <int GROUP, bool GROUPED>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads<GROUPED>, 1)
     fp8_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const GemmArgs a) {
     using C = Cfg<GROUP>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -140,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int x_tiles;
     if constexpr (GROUPED) {
         rt = route_tables(a.group, a.S, a.E);
-        x_tiles = tile_prefix<kRows, kThreads>(rt, a.E, ctl.prefix, ctl.warp_tot);
+        x_tiles = tile_prefix<kRows, kThreads<GROUPED>>(rt, a.E, ctl.prefix, ctl.warp_tot);
     } else {
         x_tiles = (a.M + kRows * GROUP - 1) / (kRows * GROUP);
     }
@@ -171,10 +173,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
 
     if (warp >= kPromoWarps) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp == kTmaWarp || (GROUPED && warp == kGatherWarp)) {
-        // One warp for the boxes; grouped, another for the rows of x: a gather of four rows is an instruction of its own, 32 of them a
-        // block of K would hold up the weights.
+        if constexpr (GROUPED) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == kTmaWarp || (GROUPED && warp >= kGatherWarp)) {
+        // One warp for the boxes; grouped, five more for the rows of x: a gather of four rows is an instruction of its own, ~50 clocks
+        // of its thread's warp each (4096 tokens x 10 of 512 experts: 298 us with one gathering warp, 257 with two).
+        const int quad = (warp - kGatherWarp) + kGatherWarps * lane;  // gathering: rows 4 * quad .. of the tile
         uint32_t it = 0;
         bool ok = true;
         for (int p = blockIdx.x / GROUP; p < n_tiles && ok; p += step) {
@@ -185,16 +189,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // rows beyond the list's end repeat its last one; whole quads beyond it are not fetched, and what their lanes compute is
                 // not stored
                 bytes = C::BTile + (uint32_t)((t.n + 3) / 4) * 4 * kBK;
-                if (warp == kGatherWarp)
-                    for (int j = 0; j < 4; ++j) rows[j] = rt.slots[t.first + min(lane * 4 + j, t.n - 1)] / a.div;
+                if (warp >= kGatherWarp)
+                    for (int j = 0; j < 4; ++j) rows[j] = rt.slots[t.first + min(quad * 4 + j, t.n - 1)] / a.div;
             }
             for (int kb = 0; kb < a.KB; ++kb, ++it) {
                 const int s = it % C::Stages;
                 ok = __all_sync(0xffffffffu, mbar_wait(&ctl.empty[s], ((it / C::Stages) & 1u) ^ 1u, abort_flag));
                 if (!ok) break;
                 uint8_t *dst = base + s * C::StageBytes;
-                if (GROUPED && warp == kGatherWarp) {
-                    if (lane * 4 < t.n) tma_gather4(dst + lane * 4 * kBK, &x_map, kb * kBK, rows[0], rows[1], rows[2], rows[3], &ctl.full[s]);
+                if (GROUPED && warp >= kGatherWarp) {
+                    if (quad < kRows / 4 && quad * 4 < t.n) tma_gather4(dst + quad * 4 * kBK, &x_map, kb * kBK, rows[0], rows[1], rows[2], rows[3], &ctl.full[s]);
                 } else if (elect_one()) {
                     if constexpr (GROUP == 2) {
                         // the leader's barrier counts both CTAs' bytes; this CTA's weight rows are the rank-th 64 of each half, so that a
@@ -261,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
     }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int h = warp >> 2, r = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + h * kHalf;
         uint8_t *strip = strips + warp * kStrip;
@@ -349,9 +353,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int64_t out_row = row;
             fetch(p + step);
             // y: 64 bytes of every row at a time through the strip; then 4 lanes write a row's 64 bytes, 8 rows an instruction
-            const int es = a.out_f32 ? 4 : 2, per = 64 / es;  // columns of a strip
+            const int es = a.out_f32 ? 4 : 2;
             const bool wide = ((int64_t)a.N * es) % 16 == 0 && reinterpret_cast<uintptr_t>(a.y) % 16 == 0;
-            auto flush = [&](int col) {  // columns col .. col + per of the half
+            auto flush = [&](int col) {  // the strip's 64 / es columns from col on
                 __syncwarp();
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -428,7 +432,7 @@ int launch(const char *fn, const uint8_t *w, int64_t w_rows, const uint8_t *x, i
     const int64_t all = tiles * a.NT, room = sm_count() / GROUP;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(std::min(all, room) * GROUP));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(kThreads<GROUPED>);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
