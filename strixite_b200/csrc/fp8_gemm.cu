@@ -6,14 +6,17 @@
 // FP32), the outer sum an FP32 FMA of that accumulator, taken from tensor memory, into registers: a scale per 128 columns cannot be
 // applied inside the accumulation.
 //
-// Weight rows are the M axis of the MMA (128 lanes: one block row of scales) and the rows of x its N axis, up to TOK at a time: a few
-// rows (decode) cost a narrow instruction, and an expert's ragged slot list is padded to 16. Warp roles of a CTA:
+// This file: few rows (decode, verify, a few rows an expert). Weight rows are the M axis of the MMA (128 lanes: one block row of scales) and
+// the rows of x its N axis, up to TOK = 16, 32 or 64 at a time: a few rows cost a narrow instruction, and an expert's ragged slot list is
+// padded to 16. fp8_gemm_wide.cu has the form for many rows. What bounds it is the stream of the weights. Warp roles of a CTA:
 //   promotion warps   tcgen05.ld of a finished block accumulator, acc = fma(scale, block, acc); at the end the store of y
-//   TMA warp          weight boxes [128 rows x 128 bytes] and rows of x (a box, or gathered by slot for the experts), 128-byte swizzle
-//   MMA warp          four K = 32 instructions per block into one of NBUF accumulators, two commits
-//   scale warp        xs * ws of the block for the TOK columns, through a ring in shared memory
-// CTAs walk the (x tile, weight tile) pairs; where there are fewer pairs than SMs the blocks of K are split over the CTAs of a cluster,
-// whose register sums meet in distributed shared memory and are added in rank order (the same result on every run).
+//   TMA warp          weight boxes [128 rows x 128 bytes], 128-byte swizzle, and the box of x rows
+//   gather warp       rows of x by slot (the experts)
+//   MMA warp          four K = 32 instructions per block into one of NBuf accumulators, two commits
+//   scale warp        xs * ws of the block for the TOK columns, into the accumulator's slot of shared memory
+// CTAs walk the (x tile, weight tile) pairs; where there are fewer pairs than SMs the blocks of K are split over the CTAs of a cluster:
+// every CTA pushes its sums into the shared memory of the CTA that owns the column, which adds them in rank order (the same result on
+// every run).
 // Every mbarrier wait is bounded: on expiry the CTA raises the abort counter, waits for its copies, frees its tensor memory, returns.
 #include <cuda.h>
 
@@ -34,35 +37,36 @@ __device__ unsigned int g_fp8_aborts = 0;
 __device__ unsigned int g_fp8_refusals = 0;
 
 constexpr int kATile = kTileM * kBK;      // 16 KB of weights
-constexpr int kScaleSlots = 4;
-constexpr int kMaxSplit = 8;              // portable cluster size
+constexpr int kPromoWarps = 4, kTmaWarp = 4, kMmaWarp = 5, kScaleWarp = 6, kGatherWarp = 7;
+constexpr int kThreads = 8 * 32;
+// CTAs that share a pair's K blocks at most. Clusters of 8 CTAs with most of an SM's shared memory did not all start together (16 of them:
+// the last ones 4.3 us after the first, measured), clusters of 4 do.
+constexpr int kMaxSplit = 4;
 
 template <int TOK>
 struct Cfg {
-    static constexpr int BTile = TOK * kBK;
-    static constexpr int Stages = TOK >= 256 ? 4 : TOK >= 128 ? 6 : TOK >= 64 ? 8 : TOK >= 32 ? 9 : 10;
-    static constexpr int NBuf = TOK >= 256 ? 2 : 4;                // accumulators in tensor memory
-    static constexpr int TmemCols = NBuf * TOK < 32 ? 32 : NBuf * TOK;
-    static constexpr int PromoWarps = TOK >= 128 ? 8 : 4;
-    static constexpr int Cols = TOK / (PromoWarps / 4);            // columns a promotion thread holds
-    static constexpr int Threads = (PromoWarps + 3) * 32;
-    static constexpr int StageBytes = kATile + BTile;
+    static constexpr int BTile = TOK * kBK, StageBytes = kATile + BTile;
+    static constexpr int Stages = TOK >= 64 ? 7 : TOK >= 32 ? 9 : 10;
+    static constexpr int NBuf = TOK >= 64 ? 4 : 8;  // accumulators in tensor memory, and slots of scales
+    static constexpr int TmemCols = NBuf * TOK;
+    static constexpr int RedBytes = TOK * kTileM * 4;  // the columns' parts from the CTAs of a cluster
 };
 
 template <int TOK>
 struct Ctl {
     using C = Cfg<TOK>;
-    uint64_t full[C::Stages], empty[C::Stages], acc_full[C::NBuf], acc_empty[C::NBuf], sc_full[kScaleSlots], sc_empty[kScaleSlots];
+    // acc_full: the block's MMAs have completed (a commit) and its scales are there (the scale warp)
+    uint64_t full[C::Stages], empty[C::Stages], acc_full[C::NBuf], acc_empty[C::NBuf];
     uint32_t tmem_base;
     int abort_flag;
     int warp_tot[32];
-    alignas(16) float scales[kScaleSlots][TOK];  // read as float4
-    int prefix[kMaxE + 1 + 1];  // grouped: first tile of each bucket
+    alignas(16) float scales[C::NBuf][TOK];  // read as float4
+    int prefix[kMaxE + 1 + 1];               // grouped: first tile of each bucket
 };
 
 template <int TOK>
 constexpr size_t smem_bytes() {
-    return (size_t)Cfg<TOK>::Stages * Cfg<TOK>::StageBytes + sizeof(Ctl<TOK>) + 1024;
+    return (size_t)Cfg<TOK>::Stages * Cfg<TOK>::StageBytes + Cfg<TOK>::RedBytes + sizeof(Ctl<TOK>) + 1024;
 }
 
 __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
@@ -73,12 +77,8 @@ __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t da, uint64_t d
         ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(0u)
         : "memory");
 }
-__device__ __forceinline__ float ld_peer(uint32_t addr, uint32_t rank) {
-    uint32_t p;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(p) : "memory");
-    return v;
+__device__ __forceinline__ void st_peer(uint32_t cluster_addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
 }
 
 // One (x tile, weight tile) pair: its first row of the weight stack, first weight row and block row inside its matrix, and its columns -
@@ -88,97 +88,127 @@ struct Pair {
 };
 
 template <int TOK, bool GROUPED>
-__global__ void __launch_bounds__(Cfg<TOK>::Threads, 1)
+__global__ void __launch_bounds__(kThreads, 1)
     fp8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const GemmArgs a) {
     using C = Cfg<TOK>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    Ctl<TOK> &ctl = *reinterpret_cast<Ctl<TOK> *>(base + C::Stages * C::StageBytes);
+    float *red = reinterpret_cast<float *>(base + C::Stages * C::StageBytes);
+    Ctl<TOK> &ctl = *reinterpret_cast<Ctl<TOK> *>(base + C::Stages * C::StageBytes + C::RedBytes);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    constexpr int kTmaWarp = C::PromoWarps, kMmaWarp = kTmaWarp + 1, kScaleWarp = kTmaWarp + 2;
-    if (GROUPED && !ws_is_for(a.group, a.S, a.E, &g_fp8_refusals)) return;  // the whole grid leaves
-    if (tid == 0) {
-        for (int i = 0; i < C::Stages; ++i) mbar_init(&ctl.full[i], 1), mbar_init(&ctl.empty[i], 1);
-        for (int i = 0; i < C::NBuf; ++i) mbar_init(&ctl.acc_full[i], 1), mbar_init(&ctl.acc_empty[i], C::PromoWarps);
-        for (int i = 0; i < kScaleSlots; ++i) mbar_init(&ctl.sc_full[i], 1), mbar_init(&ctl.sc_empty[i], C::PromoWarps);
-        ctl.abort_flag = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    RouteTables rt{};
+    if constexpr (GROUPED) {
+        if (!ws_is_for(a.group, a.S, a.E, &g_fp8_refusals)) return;  // the whole grid leaves
+        rt = route_tables(a.group, a.S, a.E);
     }
-    if (warp == kMmaWarp) {
+    if (a.split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    const int rank = a.split > 1 ? (int)cluster_rank() : 0;
+    const int sh = a.split == 4 ? 2 : a.split == 2 ? 1 : 0;  // split is 1, 2 or 4
+    const int kb0 = a.KB * rank >> sh, kb1 = a.KB * (rank + 1) >> sh;
+    volatile int *abort_flag = &ctl.abort_flag;
+
+    // A CTA walks neighbouring pairs: the weight tiles of one x tile, so what belongs to the rows is looked up once. With a split, a cluster
+    // has one pair (or none).
+    auto first_of = [&](int n_pairs) { return a.split > 1 ? (int)blockIdx.x >> sh : (int)((int64_t)n_pairs * blockIdx.x / gridDim.x); };
+    auto end_of = [&](int n_pairs) { return a.split > 1 ? min(n_pairs, ((int)blockIdx.x >> sh) + 1) : (int)((int64_t)n_pairs * (blockIdx.x + 1) / gridDim.x); };
+    // Block kb of a pair into stage s: the weights, and (dense) the rows of x.
+    auto load = [&](int s, int kb, int wrow, int first, uint32_t bytes) {
+        uint8_t *dst = base + s * C::StageBytes;
+        mbar_expect_tx(&ctl.full[s], bytes);
+        tma_load_2d(dst, &w_map, kb * kBK, wrow, &ctl.full[s]);
+        if constexpr (!GROUPED) tma_load_2d(dst + kATile, &x_map, kb * kBK, first, &ctl.full[s]);
+    };
+    int early = 0;  // dense: blocks of the first pair that are on their way before anything else is set up
+    if (warp == kTmaWarp) {
+        if (elect_one()) {
+            for (int i = 0; i < C::Stages; ++i) mbar_init(&ctl.full[i], 1), mbar_init(&ctl.empty[i], 1);
+            for (int i = 0; i < C::NBuf; ++i) mbar_init(&ctl.acc_full[i], 2), mbar_init(&ctl.acc_empty[i], kPromoWarps);
+            ctl.abort_flag = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // this thread's copies may signal them at once
+            if constexpr (!GROUPED) {
+                const int p = first_of(((a.M + TOK - 1) / TOK) * a.NT), xt = p / a.NT;
+                for (int kb = kb0; kb < kb1 && kb - kb0 < C::Stages; ++kb) load(kb - kb0, kb, (p - xt * a.NT) * kTileM, xt * TOK, C::StageBytes);
+            }
+        }
+        if (!GROUPED) early = min(kb1 - kb0, C::Stages);
+        __syncwarp();
+    } else if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem_base)), "r"((uint32_t)C::TmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    RouteTables rt{};
     int x_tiles;
     if constexpr (GROUPED) {
-        rt = route_tables(a.group, a.S, a.E);
-        x_tiles = tile_prefix<TOK, C::Threads>(rt, a.E, ctl.prefix, ctl.warp_tot);
+        x_tiles = tile_prefix<TOK, kThreads>(rt, a.E, ctl.prefix, ctl.warp_tot);
     } else {
         x_tiles = (a.M + TOK - 1) / TOK;
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (a.split > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // the peers run: their shared memory may be written
     const uint32_t tmem = ctl.tmem_base;
-    volatile int *abort_flag = &ctl.abort_flag;
-    const int rank = a.split > 1 ? (int)cluster_rank() : 0;
-    const int n_pairs = x_tiles * a.NT, first_pair = blockIdx.x / a.split, pair_step = gridDim.x / a.split;
-    const int kb0 = (int)((int64_t)a.KB * rank / a.split), kb1 = (int)((int64_t)a.KB * (rank + 1) / a.split);
+    const int n_pairs = x_tiles * a.NT, p_first = first_of(n_pairs), p_end = end_of(n_pairs);
 
-    auto pair_of = [&](int p) {  // warp-uniform
-        const int xt = p / a.NT, nt = p - xt * a.NT;
-        Pair r;
-        r.n0 = nt * kTileM;
-        if constexpr (GROUPED) {
-            const int lo = bucket_of(ctl.prefix, a.E, xt);
-            const int begin = rt.offsets[lo] + (xt - ctl.prefix[lo]) * TOK;
-            r.wrow = lo * a.N + r.n0, r.ws_row = lo * a.NB + nt;
-            r.first = begin, r.n = min(TOK, rt.offsets[lo + 1] - begin);
-        } else {
-            r.wrow = r.n0, r.ws_row = nt;
-            r.first = xt * TOK, r.n = min(TOK, a.M - r.first);
+    Pair t{};  // of this thread's walk; warp-uniform
+    int xt = -1, nt = 0;
+    auto pair_at = [&](int p) {  // for p = p_first, p_first + 1, ..; whether the rows are others than before
+        if (xt >= 0 && ++nt < a.NT) {
+            t.n0 += kTileM, t.wrow += kTileM, ++t.ws_row;
+            return false;
         }
-        return r;
+        if (xt < 0) xt = p / a.NT, nt = p - xt * a.NT;
+        else ++xt, nt = 0;
+        t.n0 = nt * kTileM;
+        if constexpr (GROUPED) {
+            const int e = bucket_of(ctl.prefix, a.E, xt);
+            t.first = rt.offsets[e] + (xt - ctl.prefix[e]) * TOK;
+            t.n = min(TOK, rt.offsets[e + 1] - t.first);
+            t.wrow = e * a.N + t.n0, t.ws_row = e * a.NB + nt;
+        } else {
+            t.wrow = t.n0, t.ws_row = nt;
+            t.first = xt * TOK, t.n = min(TOK, a.M - t.first);
+        }
+        return true;
     };
-    auto row_of = [&](const Pair &p, int j) {  // the row of x behind column j < p.n
-        if constexpr (GROUPED) return rt.slots[p.first + j] / a.div;
-        else return p.first + j;
+    auto row_of = [&](int j) {  // the row of x behind column j < t.n
+        if constexpr (GROUPED) return rt.slots[t.first + j] / a.div;
+        else return t.first + j;
+    };
+    auto put = [&](int j, int r, float v) {  // y of column j, weight row r of the tile
+        int64_t row = t.first + j;
+        if constexpr (GROUPED) row = rt.slots[row];
+        const int64_t o = row * a.N + t.n0 + r;
+        if (a.out_f32) static_cast<float *>(a.y)[o] = v;
+        else static_cast<uint16_t *>(a.y)[o] = f32_to_bf16_bits(v);
     };
 
-    if (warp == kTmaWarp) {
-        constexpr int kQuads = TOK / 4, kPerLane = (kQuads + 31) / 32;
+    if (warp == kTmaWarp || (GROUPED && warp == kGatherWarp)) {
         uint32_t it = 0;
         bool ok = true;
-        for (int p = first_pair; p < n_pairs && ok; p += pair_step) {
-            const Pair t = pair_of(p);
-            int rows[kPerLane][4];
+        int rows[4] = {0, 0, 0, 0};
+        for (int p = p_first; p < p_end && ok; ++p) {
+            const bool other = pair_at(p);
             uint32_t bytes = C::StageBytes;
             if constexpr (GROUPED) {
                 // columns beyond the list's end repeat its last row; whole quads beyond it are not fetched, and what their columns
                 // compute is not stored
-                for (int i = 0; i < kPerLane; ++i)
-                    for (int j = 0; j < 4; ++j) rows[i][j] = row_of(t, min((lane + 32 * i) * 4 + j, t.n - 1));
                 bytes = kATile + (uint32_t)((t.n + 3) / 4) * 4 * kBK;
+                if (warp == kGatherWarp && other)
+                    for (int j = 0; j < 4; ++j) rows[j] = row_of(min(lane * 4 + j, t.n - 1));
             }
             for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                if ((int)it < early) continue;
                 const int s = it % C::Stages;
-                ok = __all_sync(0xffffffffu, mbar_wait(&ctl.empty[s], ((it / C::Stages) & 1u) ^ 1u, abort_flag));
+                if (it >= C::Stages) ok = __all_sync(0xffffffffu, mbar_wait(&ctl.empty[s], ((it / C::Stages) & 1u) ^ 1u, abort_flag));
                 if (!ok) break;
-                uint8_t *dst = base + s * C::StageBytes;
-                if (elect_one()) {
-                    mbar_expect_tx(&ctl.full[s], bytes);
-                    tma_load_2d(dst, &w_map, kb * kBK, t.wrow, &ctl.full[s]);
-                    if constexpr (!GROUPED) tma_load_2d(dst + kATile, &x_map, kb * kBK, t.first, &ctl.full[s]);
+                if (GROUPED && warp == kGatherWarp) {
+                    if (lane < TOK / 4 && lane * 4 < t.n)
+                        tma_gather4(base + s * C::StageBytes + kATile + lane * 4 * kBK, &x_map, kb * kBK, rows[0], rows[1], rows[2], rows[3], &ctl.full[s]);
+                } else if (elect_one()) {
+                    load(s, kb, t.wrow, t.first, bytes);
                 }
                 __syncwarp();
-                if constexpr (GROUPED) {
-#pragma unroll
-                    for (int i = 0; i < kPerLane; ++i) {
-                        const int quad = lane + 32 * i;
-                        if (quad < kQuads && quad * 4 < t.n)
-                            tma_gather4(dst + kATile + quad * 4 * kBK, &x_map, kb * kBK, rows[i][0], rows[i][1], rows[i][2], rows[i][3], &ctl.full[s]);
-                    }
-                }
             }
         }
         // The last blocks' MMAs have read their stages and signalled it; after an abandoned wait, the copies in flight have landed.
@@ -190,37 +220,39 @@ __global__ void __launch_bounds__(Cfg<TOK>::Threads, 1)
         }
         __syncwarp();
     } else if (warp == kMmaWarp) {
-        uint32_t it = 0;
-        bool ok = true;
-        for (int p = first_pair; p < n_pairs && ok; p += pair_step) {
-            const Pair t = pair_of(p);
-            const uint32_t idesc = idesc_e4m3(kTileM, (t.n + 15) & ~15);
-            for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                const int s = it % C::Stages, b = it % C::NBuf;
-                ok = mbar_wait(&ctl.acc_empty[b], ((it / C::NBuf) & 1u) ^ 1u, abort_flag) && mbar_wait(&ctl.full[s], (it / C::Stages) & 1u, abort_flag);
-                if (!__all_sync(0xffffffffu, ok)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                if (elect_one()) {
+        // One thread; the barriers of a block are asked about under the MMAs of the block in front of it (a probe takes ~100 clocks).
+        if (elect_one()) {
+            uint32_t it = 0;
+            bool ok = true, full = false, free = true;
+            for (int p = p_first; p < p_end && ok; ++p) {
+                pair_at(p);
+                const uint32_t idesc = idesc_e4m3(kTileM, (t.n + 15) & ~15);
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    const int s = it % C::Stages, b = it % C::NBuf;
+                    if (!free) ok = mbar_wait(&ctl.acc_empty[b], ((it / C::NBuf) & 1u) ^ 1u, abort_flag);
+                    if (ok && !full) ok = mbar_wait(&ctl.full[s], (it / C::Stages) & 1u, abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
                     const uint32_t at = smem_u32(base + s * C::StageBytes);
                     const uint64_t da = umma_desc(at), db = umma_desc(at + kATile);
 #pragma unroll
                     for (int k = 0; k < kBK / 32; ++k) umma_f8(tmem + b * TOK, da + 2 * k, db + 2 * k, idesc, k != 0);
-                    umma_commit(&ctl.empty[s]);
+                    ++it;
+                    free = it < C::NBuf || mbar_test(&ctl.acc_empty[it % C::NBuf], ((it / C::NBuf) & 1u) ^ 1u);
+                    full = mbar_test(&ctl.full[it % C::Stages], (it / C::Stages) & 1u);
                     umma_commit(&ctl.acc_full[b]);
+                    umma_commit(&ctl.empty[s]);
                 }
-                __syncwarp();
             }
         }
+        __syncwarp();
     } else if (warp == kScaleWarp) {
         constexpr int kPerLane = (TOK + 31) / 32;
         uint32_t it = 0;
         bool ok = true;
-        for (int p = first_pair; p < n_pairs && ok; p += pair_step) {
-            const Pair t = pair_of(p);
-            const float *xp[kPerLane];
+        const float *xp[kPerLane];
+        for (int p = p_first; p < p_end && ok; ++p) {
+            const bool other = pair_at(p);
             // four blocks at a time: a row's four scales share a 32-byte sector, and a round of loads is under way while the round before
             // it is handed over
             float cur[kPerLane][4], nxt[kPerLane][4];
@@ -234,22 +266,24 @@ __global__ void __launch_bounds__(Cfg<TOK>::Threads, 1)
                     for (int i = 0; i < kPerLane; ++i) to[i][q] = in && xp[i] != nullptr ? xp[i][kb + q] * w : 0.f;
                 }
             };
+            if (other) {
 #pragma unroll
-            for (int i = 0; i < kPerLane; ++i) xp[i] = lane + 32 * i < t.n ? a.xs + (int64_t)row_of(t, lane + 32 * i) * a.KB : nullptr;
+                for (int i = 0; i < kPerLane; ++i) xp[i] = lane + 32 * i < t.n ? a.xs + (int64_t)row_of(lane + 32 * i) * a.KB : nullptr;
+            }
             fetch(cur, kb0);
             for (int kb = kb0; kb < kb1 && ok; kb += 4) {
                 fetch(nxt, kb + 4);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     if (kb + q >= kb1 || !ok) continue;
-                    const int s = it % kScaleSlots;
-                    ok = __all_sync(0xffffffffu, mbar_wait(&ctl.sc_empty[s], ((it / kScaleSlots) & 1u) ^ 1u, abort_flag));
+                    const int b = it % C::NBuf;
+                    if (it >= C::NBuf) ok = __all_sync(0xffffffffu, mbar_wait(&ctl.acc_empty[b], ((it / C::NBuf) & 1u) ^ 1u, abort_flag));
                     if (!ok) continue;
 #pragma unroll
                     for (int i = 0; i < kPerLane; ++i)
-                        if (lane + 32 * i < TOK) ctl.scales[s][lane + 32 * i] = cur[i][q];
+                        if (lane + 32 * i < TOK) ctl.scales[b][lane + 32 * i] = cur[i][q];
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&ctl.sc_full[s]);
+                    if (lane == 0) mbar_arrive(&ctl.acc_full[b]);
                     ++it;
                 }
 #pragma unroll
@@ -258,90 +292,77 @@ __global__ void __launch_bounds__(Cfg<TOK>::Threads, 1)
                     for (int q = 0; q < 4; ++q) cur[i][q] = nxt[i][q];
             }
         }
-    } else {
-        // ---- promotion ----
-        constexpr int kChunk = C::Cols < 32 ? C::Cols : 32;
-        const int col0 = (warp / 4) * C::Cols, r = (warp & 3) * 32 + lane;
-        const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16) + col0;
+    } else if (warp < kPromoWarps) {
+        constexpr int kChunk = TOK < 32 ? TOK : 32;
+        const int r = warp * 32 + lane;
+        const uint32_t lane_base = tmem + ((uint32_t)(warp * 32) << 16);
         uint32_t it = 0;
         bool ok = true;
-        for (int p = first_pair; p < n_pairs && ok; p += pair_step) {
-            const Pair t = pair_of(p);
-            float acc[C::Cols];
+        for (int p = p_first; p < p_end && ok; ++p) {
+            pair_at(p);
+            float acc[TOK];
 #pragma unroll
-            for (int j = 0; j < C::Cols; ++j) acc[j] = 0.f;
+            for (int j = 0; j < TOK; ++j) acc[j] = 0.f;
             for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                const int b = it % C::NBuf, s = it % kScaleSlots;
-                ok = mbar_wait(&ctl.sc_full[s], (it / kScaleSlots) & 1u, abort_flag) && mbar_wait(&ctl.acc_full[b], (it / C::NBuf) & 1u, abort_flag);
-                if (!__all_sync(0xffffffffu, ok)) {
-                    ok = false;
-                    break;
-                }
+                const int b = it % C::NBuf;
+                ok = __all_sync(0xffffffffu, mbar_wait(&ctl.acc_full[b], (it / C::NBuf) & 1u, abort_flag));
+                if (!ok) break;
                 tc_fence_after();
 #pragma unroll
-                for (int c = 0; c < C::Cols; c += kChunk) {
-                    if (col0 + c >= t.n) continue;  // warp-uniform
+                for (int c = 0; c < TOK; c += kChunk) {
+                    if (c >= t.n) continue;  // warp-uniform
                     uint32_t v[kChunk];
                     if constexpr (kChunk == 32) tmem_ld32(lane_base + b * TOK + c, v);
                     else tmem_ld16(lane_base + b * TOK + c, v);
+                    float4 f[kChunk / 4];
+#pragma unroll
+                    for (int j = 0; j < kChunk / 4; ++j) f[j] = *reinterpret_cast<const float4 *>(&ctl.scales[b][c + 4 * j]);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < kChunk; j += 4) {
-                        const float4 f = *reinterpret_cast<const float4 *>(&ctl.scales[s][col0 + c + j]);
-                        acc[c + j] = fmaf(f.x, __uint_as_float(v[j]), acc[c + j]);
-                        acc[c + j + 1] = fmaf(f.y, __uint_as_float(v[j + 1]), acc[c + j + 1]);
-                        acc[c + j + 2] = fmaf(f.z, __uint_as_float(v[j + 2]), acc[c + j + 2]);
-                        acc[c + j + 3] = fmaf(f.w, __uint_as_float(v[j + 3]), acc[c + j + 3]);
+                    for (int j = 0; j < kChunk / 4; ++j) {
+                        acc[c + 4 * j] = fmaf(f[j].x, __uint_as_float(v[4 * j]), acc[c + 4 * j]);
+                        acc[c + 4 * j + 1] = fmaf(f[j].y, __uint_as_float(v[4 * j + 1]), acc[c + 4 * j + 1]);
+                        acc[c + 4 * j + 2] = fmaf(f[j].z, __uint_as_float(v[4 * j + 2]), acc[c + 4 * j + 2]);
+                        acc[c + 4 * j + 3] = fmaf(f[j].w, __uint_as_float(v[4 * j + 3]), acc[c + 4 * j + 3]);
                     }
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&ctl.acc_empty[b]), mbar_arrive(&ctl.sc_empty[s]);
+                if (lane == 0) mbar_arrive(&ctl.acc_empty[b]);
             }
             if (!ok) break;
             if (a.split > 1) {
-                // the sums go to this CTA's own shared memory (its stages are spent: every block's MMAs have completed)
-                float *red = reinterpret_cast<float *>(base);
+                // column j belongs to the CTA of rank j % split: part `rank` of its (j / split)-th column
+                const uint32_t at = smem_u32(red + rank * kTileM + r);
 #pragma unroll
-                for (int j = 0; j < C::Cols; ++j)
-                    if (col0 + j < t.n) red[(col0 + j) * kTileM + r] = acc[j];
+                for (int j = 0; j < TOK; ++j) {
+                    if (j >= t.n) continue;
+                    uint32_t dst;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(at + (uint32_t)(j & ~(a.split - 1)) * kTileM * 4), "r"(j & (a.split - 1)));
+                    st_peer(dst, acc[j]);
+                }
             } else if (t.n0 + r < a.N) {
 #pragma unroll
-                for (int j = 0; j < C::Cols; ++j) {
-                    if (col0 + j < t.n) {
-                        int64_t row = t.first + col0 + j;
-                        if constexpr (GROUPED) row = rt.slots[row];
-                        const int64_t o = row * a.N + t.n0 + r;
-                        if (a.out_f32) static_cast<float *>(a.y)[o] = acc[j];
-                        else static_cast<uint16_t *>(a.y)[o] = f32_to_bf16_bits(acc[j]);
-                    }
-                }
+                for (int j = 0; j < TOK; ++j)
+                    if (j < t.n) put(j, r, acc[j]);
             }
         }
     }
 
-    if (a.split > 1) {  // the grid has at most one pair per cluster
+    if (a.split > 1) {  // at most one pair per cluster
         __syncwarp();
         cluster_sync();
-        if (warp < C::PromoWarps && first_pair < n_pairs) {
-            const Pair t = pair_of(first_pair);
-            const int r = (warp & 3) * 32 + lane;
-            const uint32_t red = smem_u32(base);
-            for (int j = rank + (warp / 4) * a.split; j < t.n; j += a.split * (C::PromoWarps / 4)) {
-                float v = 0.f;
-                for (int q = 0; q < a.split; ++q) v += ld_peer(red + (uint32_t)(j * kTileM + r) * 4, q);
-                if (t.n0 + r < a.N) {
-                    int64_t row = t.first + j;
-                    if constexpr (GROUPED) row = rt.slots[row];
-                    const int64_t o = row * a.N + t.n0 + r;
-                    if (a.out_f32) static_cast<float *>(a.y)[o] = v;
-                    else static_cast<uint16_t *>(a.y)[o] = f32_to_bf16_bits(v);
-                }
+        if (warp < kPromoWarps && p_first < p_end) {
+            const int r = warp * 32 + lane;
+            for (int j = rank; j < t.n; j += a.split) {
+                const float *part = red + (j - rank) * kTileM + r;
+                float v = part[0] + part[kTileM];
+                if (a.split == 4) v = v + part[2 * kTileM] + part[3 * kTileM];
+                if (t.n0 + r < a.N) put(j, r, v);
             }
         }
-        __syncwarp();
-        cluster_sync();  // nobody's shared memory goes while a peer reads it
     }
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -410,7 +431,7 @@ int launch(const char *fn, const uint8_t *w, int64_t w_rows, const uint8_t *x, i
     while (a.split < kMaxSplit && a.split * 2 <= a.KB && pairs * a.split * 2 <= sms) a.split *= 2;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(a.split > 1 ? pairs * a.split : std::min(pairs, sms)));
-    cfg.blockDim = dim3(Cfg<TOK>::Threads);
+    cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
