@@ -59,9 +59,8 @@ struct Ctl {
     uint64_t full[C::Stages], empty[C::Stages], acc_full[C::NBuf], acc_empty[C::NBuf];
     uint32_t tmem_base;
     int abort_flag;
-    int warp_tot[32];
     alignas(16) float scales[C::NBuf][TOK];  // read as float4
-    int prefix[kMaxE + 1 + 1];               // grouped: first tile of each bucket
+    Buckets buckets;                         // grouped
 };
 
 template <int TOK>
@@ -96,10 +95,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     float *red = reinterpret_cast<float *>(base + C::Stages * C::StageBytes);
     Ctl<TOK> &ctl = *reinterpret_cast<Ctl<TOK> *>(base + C::Stages * C::StageBytes + C::RedBytes);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    if (warp == kTmaWarp && elect_one()) prefetch_map(&w_map), prefetch_map(&x_map);
     RouteTables rt{};
+    BucketScan<TOK, kThreads> scan;
     if constexpr (GROUPED) {
-        if (!ws_is_for(a.group, a.S, a.E, &g_fp8_refusals)) return;  // the whole grid leaves
         rt = route_tables(a.group, a.S, a.E);
+        if (!scan.load(a.group, rt, a.S, a.E, &g_fp8_refusals)) return;  // the whole grid leaves
     }
     if (a.split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     const int rank = a.split > 1 ? (int)cluster_rank() : 0;
@@ -109,8 +110,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     // A CTA walks neighbouring pairs: the weight tiles of one x tile, so what belongs to the rows is looked up once. With a split, a cluster
     // has one pair (or none).
-    auto first_of = [&](int n_pairs) { return a.split > 1 ? (int)blockIdx.x >> sh : (int)((int64_t)n_pairs * blockIdx.x / gridDim.x); };
-    auto end_of = [&](int n_pairs) { return a.split > 1 ? min(n_pairs, ((int)blockIdx.x >> sh) + 1) : (int)((int64_t)n_pairs * (blockIdx.x + 1) / gridDim.x); };
+    const int cluster = (int)blockIdx.x >> sh, clusters = (int)gridDim.x >> sh;
+    auto first_of = [&](int n_pairs) {  // the first n_pairs % clusters walks are one pair longer
+        const int each = n_pairs / clusters;
+        return each * cluster + min(cluster, n_pairs - each * clusters);
+    };
     // Block kb of a pair into stage s: the weights, and (dense) the rows of x.
     auto load = [&](int s, int kb, int wrow, int first, uint32_t bytes) {
         uint8_t *dst = base + s * C::StageBytes;
@@ -139,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     int x_tiles;
     if constexpr (GROUPED) {
-        x_tiles = tile_prefix<TOK, kThreads>(rt, a.E, ctl.prefix, ctl.warp_tot);
+        x_tiles = scan.scan(a.E, ctl.buckets, [&](int tiles) { return first_of(tiles * a.NT) / a.NT; });
     } else {
         x_tiles = (a.M + TOK - 1) / TOK;
     }
@@ -148,7 +152,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     if (a.split > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // the peers run: their shared memory may be written
     const uint32_t tmem = ctl.tmem_base;
-    const int n_pairs = x_tiles * a.NT, p_first = first_of(n_pairs), p_end = end_of(n_pairs);
+    const int n_pairs = x_tiles * a.NT, p_first = first_of(n_pairs), each = n_pairs / clusters, p_end = p_first + each + (cluster < n_pairs - each * clusters ? 1 : 0);
 
     Pair t{};  // of this thread's walk; warp-uniform
     int xt = -1, nt = 0;
@@ -157,13 +161,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             t.n0 += kTileM, t.wrow += kTileM, ++t.ws_row;
             return false;
         }
-        if (xt < 0) xt = p / a.NT, nt = p - xt * a.NT;
+        const bool begin = xt < 0;
+        if (begin) xt = p / a.NT, nt = p - xt * a.NT;
         else ++xt, nt = 0;
         t.n0 = nt * kTileM;
         if constexpr (GROUPED) {
-            const int e = bucket_of(ctl.prefix, a.E, xt);
-            t.first = rt.offsets[e] + (xt - ctl.prefix[e]) * TOK;
-            t.n = min(TOK, rt.offsets[e + 1] - t.first);
+            const int e = begin ? ctl.buckets.first : bucket_of(ctl.buckets.prefix, a.E, xt);
+            t.first = ctl.buckets.start[e] + (xt - ctl.buckets.prefix[e]) * TOK;
+            t.n = min(TOK, ctl.buckets.start[e + 1] - t.first);
             t.wrow = e * a.N + t.n0, t.ws_row = e * a.NB + nt;
         } else {
             t.wrow = t.n0, t.ws_row = nt;

@@ -86,42 +86,59 @@ __device__ __forceinline__ uint32_t peer_addr(const void *p, uint32_t rank) {
     return r;
 }
 
-// The tiles of TILE slots that the buckets of a grouping workspace are cut into: prefix[e] = first tile of bucket e, prefix[E] = their
-// number, which is returned. All threads of the block; warp_tot: 32 ints of shared memory. Ends with the prefix visible after the
-// caller's next __syncthreads().
+// What a grouped kernel knows of the buckets, in shared memory.
+struct Buckets {
+    int warp_tot[32];
+    int first;              // the bucket of this block's first tile
+    int prefix[kMaxE + 2];  // first tile of each bucket; [E]: their number
+    int start[kMaxE + 2];   // first position of each bucket in the slot list
+};
+
+// Cuts the buckets of a grouping workspace into tiles of TILE slots; all THREADS threads of the block. The offsets are read together
+// with the header that says whether the workspace is for these sizes (they lie inside it either way), so their latencies overlap.
 template <int TILE, int THREADS>
-__device__ __forceinline__ int tile_prefix(const RouteTables &rt, int E, int *prefix, int *warp_tot) {
-    constexpr int kPer = (kMaxE + THREADS) / THREADS;  // neighbouring buckets of a thread
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    int nt[kPer], sum = 0;
+struct BucketScan {
+    static constexpr int kPer = (kMaxE + THREADS) / THREADS;  // neighbouring buckets of a thread
+    int off[kPer + 1];
+    __device__ __forceinline__ bool load(const int32_t *ws, const RouteTables &rt, int64_t S, int E, unsigned int *refusals) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int e = tid * kPer + i;
-        nt[i] = e < E ? (rt.offsets[e + 1] - rt.offsets[e] + TILE - 1) / TILE : 0;
-        sum += nt[i];
+        for (int i = 0; i <= kPer; ++i) off[i] = rt.offsets[min((int)threadIdx.x * kPer + i, E)];
+        return ws_is_for(ws, S, E, refusals);
     }
-    int incl = sum;
+    // Returns the number of tiles. `first_tile` (of that number) says which tile's bucket goes to b.first. The caller's next
+    // __syncthreads() makes all of it visible.
+    template <typename F>
+    __device__ __forceinline__ int scan(int E, Buckets &b, F first_tile) const {
+        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+        int nt[kPer], sum = 0;
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, incl, off);
-        if (lane >= off) incl += o;
-    }
-    if (lane == 31) warp_tot[warp] = incl;
-    __syncthreads();
-    int before = incl - sum, total = 0;
-    for (int i = 0; i < THREADS / 32; ++i) {
-        const int t = warp_tot[i];
-        before += i < warp ? t : 0;
-        total += t;
-    }
+        for (int i = 0; i < kPer; ++i) nt[i] = (off[i + 1] - off[i] + TILE - 1) / TILE, sum += nt[i];
+        int incl = sum;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int e = tid * kPer + i;
-        if (e <= E) prefix[e] = before;
-        before += nt[i];
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (lane == 31) b.warp_tot[warp] = incl;
+        __syncthreads();
+        int before = incl - sum, total = 0;
+#pragma unroll
+        for (int i = 0; i < THREADS / 32; ++i) {
+            const int v = b.warp_tot[i];
+            before += i < warp ? v : 0;
+            total += v;
+        }
+        const int mine = first_tile(total);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int e = tid * kPer + i;
+            if (e <= E) b.prefix[e] = before, b.start[e] = off[i];
+            if (before <= mine && mine < before + nt[i]) b.first = e;
+            before += nt[i];
+        }
+        return total;
     }
-    return total;
-}
+};
 // The bucket of tile t: prefix[b] <= t < prefix[b + 1].
 __device__ __forceinline__ int bucket_of(const int *prefix, int E, int t) {
     int lo = 0, hi = E;
@@ -132,6 +149,7 @@ __device__ __forceinline__ int bucket_of(const int *prefix, int E, int t) {
     }
     return lo;
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *m) { asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory"); }
 #endif
 
 }  // namespace fp8

@@ -10,7 +10,7 @@
 // bounds the one-CTA form. GROUP = 1 (the experts' slots, gathered by row): an expert has seldom more than 128 rows.
 //
 // Roles: warps 0-3 / 4-7 promote column half 0 / 1 (each half has two accumulators, so the tensor cores run up to three half blocks
-// ahead), warp 8 issues TMA, warps 9 and 10 the MMAs of half 0 and 1 (those of CTA 0 for both CTAs), warps 11-15 gather rows of x. The sums leave through a 64-byte-wide staging strip per warp so that a
+// ahead), warp 8 issues TMA, warps 9 and 10 the MMAs of half 0 and 1 (those of CTA 0 for both CTAs), warps 11-13 gather rows of x. The sums leave through a 64-byte-wide staging strip per warp so that a
 // store covers whole sectors of a row.
 // Every mbarrier wait is bounded: on expiry the CTA raises the abort counter, waits for its copies, frees its tensor memory, returns.
 #include <algorithm>
@@ -37,7 +37,7 @@ constexpr int kStrip = 32 * kStripPitch;
 // sums: 2 * 128 * 208 + 128 * 64 <= 3 * 128 * 168 and 2 * 128 * 208 + 2 * 128 * 48 = 4 * 128 * 128, what the block is launched with.
 template <bool GROUPED>
 constexpr int kThreads = (GROUPED ? 16 : 12) * 32;
-constexpr int kGatherWarps = 5;
+constexpr int kGatherWarps = 3;
 
 template <int GROUP>
 struct Cfg {
@@ -51,8 +51,7 @@ struct Ctl {
     uint64_t full[Cfg<GROUP>::Stages], empty[Cfg<GROUP>::Stages], acc_full[2][2], acc_empty[2][2];  // [half][buffer]
     uint32_t tmem_base;
     int abort_flag;
-    int warp_tot[32];
-    int prefix[kMaxE + 1 + 1];  // grouped: first tile of each bucket
+    Buckets buckets;  // grouped
 };
 
 template <int GROUP>
@@ -121,7 +120,13 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
     uint8_t *strips = base + C::Stages * C::StageBytes;
     Ctl<GROUP> &ctl = *reinterpret_cast<Ctl<GROUP> *>(strips + kPromoWarps * kStrip);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    if (GROUPED && !ws_is_for(a.group, a.S, a.E, &g_wide_refusals)) return;  // the whole grid leaves
+    if (warp == kTmaWarp && elect_one()) prefetch_map(&w_map), prefetch_map(&x_map);
+    RouteTables rt{};
+    BucketScan<kRows, kThreads<GROUPED>> scan;
+    if constexpr (GROUPED) {
+        rt = route_tables(a.group, a.S, a.E);
+        if (!scan.load(a.group, rt, a.S, a.E, &g_wide_refusals)) return;  // the whole grid leaves
+    }
     const uint32_t rank = GROUP == 2 ? cluster_rank() : 0;
     if (tid == 0) {
         for (int i = 0; i < C::Stages; ++i) mbar_init(&ctl.full[i], 1), mbar_init(&ctl.empty[i], 2);  // empty: both halves' MMAs
@@ -138,11 +143,9 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
         }
     }
-    RouteTables rt{};
     int x_tiles;
     if constexpr (GROUPED) {
-        rt = route_tables(a.group, a.S, a.E);
-        x_tiles = tile_prefix<kRows, kThreads<GROUPED>>(rt, a.E, ctl.prefix, ctl.warp_tot);
+        x_tiles = scan.scan(a.E, ctl.buckets, [&](int) { return (int)blockIdx.x / a.NT; });
     } else {
         x_tiles = (a.M + kRows * GROUP - 1) / (kRows * GROUP);
     }
@@ -160,9 +163,9 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
         t.n0 = nt * kColTile;
         t.halves = a.N - t.n0 > kHalf ? 2 : 1;
         if constexpr (GROUPED) {
-            const int e = bucket_of(ctl.prefix, a.E, xt);
-            t.first = rt.offsets[e] + (xt - ctl.prefix[e]) * kRows;
-            t.n = min(kRows, rt.offsets[e + 1] - t.first);
+            const int e = p == (int)blockIdx.x ? ctl.buckets.first : bucket_of(ctl.buckets.prefix, a.E, xt);
+            t.first = ctl.buckets.start[e] + (xt - ctl.buckets.prefix[e]) * kRows;
+            t.n = min(kRows, ctl.buckets.start[e + 1] - t.first);
             t.wrow = e * a.N + t.n0, t.ws_row = e * a.NB + nt * 2;
         } else {
             t.first = (xt * GROUP + (int)rank) * kRows;
@@ -175,8 +178,8 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
     if (warp >= kPromoWarps) {
         if constexpr (GROUPED) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
         else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp == kTmaWarp || (GROUPED && warp >= kGatherWarp)) {
-        // One warp for the boxes; grouped, five more for the rows of x: a gather of four rows is an instruction of its own, ~50 clocks
+    if (warp == kTmaWarp || (GROUPED && warp >= kGatherWarp && warp < kGatherWarp + kGatherWarps)) {
+        // One warp for the boxes; grouped, three more for the rows of x: a gather of four rows is an instruction of its own, ~50 clocks
         // of its thread's warp each (4096 tokens x 10 of 512 experts: 298 us with one gathering warp, 257 with two).
         const int quad = (warp - kGatherWarp) + kGatherWarps * lane;  // gathering: rows 4 * quad .. of the tile
         uint32_t it = 0;
@@ -185,10 +188,13 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
             const Tile t = tile_of(p);
             int rows[4] = {0, 0, 0, 0};
             uint32_t bytes = (uint32_t)C::StageBytes * GROUP;
+            int quads = 0;
             if constexpr (GROUPED) {
-                // rows beyond the list's end repeat its last one; whole quads beyond it are not fetched, and what their lanes compute is
-                // not stored
-                bytes = C::BTile + (uint32_t)((t.n + 3) / 4) * 4 * kBK;
+                // Rows beyond the list's end repeat its last one; whole quads beyond it are not fetched, but for the first of every
+                // gathering warp: a warp without a part in a block could fall a round of the ring behind and wait for a phase long over.
+                // What the lanes of such rows compute is not stored.
+                quads = max((t.n + 3) / 4, kGatherWarps);
+                bytes = C::BTile + (uint32_t)quads * 4 * kBK;
                 if (warp >= kGatherWarp)
                     for (int j = 0; j < 4; ++j) rows[j] = rt.slots[t.first + min(quad * 4 + j, t.n - 1)] / a.div;
             }
@@ -198,7 +204,7 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
                 if (!ok) break;
                 uint8_t *dst = base + s * C::StageBytes;
                 if (GROUPED && warp >= kGatherWarp) {
-                    if (quad < kRows / 4 && quad * 4 < t.n) tma_gather4(dst + quad * 4 * kBK, &x_map, kb * kBK, rows[0], rows[1], rows[2], rows[3], &ctl.full[s]);
+                    if (quad < quads) tma_gather4(dst + quad * 4 * kBK, &x_map, kb * kBK, rows[0], rows[1], rows[2], rows[3], &ctl.full[s]);
                 } else if (elect_one()) {
                     if constexpr (GROUP == 2) {
                         // the leader's barrier counts both CTAs' bytes; this CTA's weight rows are the rank-th 64 of each half, so that a

@@ -243,6 +243,10 @@ def some_ids(g, M, A, E, kind):
     ids = torch.rand((M, E), generator=g, device="cuda").topk(A, dim=1).indices.int() if A <= E else torch.randint(0, E, (M, A), generator=g, device="cuda").int()
     if kind == "one":  # every token to the same expert first: one long list, some empty ones
         ids[:, 0] = E - 1
+    if kind == "steep":  # lists of one slot next to lists of hundreds, several tiles of each for every block of threads
+        share = torch.arange(1, E + 1, device="cuda").float() ** -1.5
+        ids = torch.multinomial(share.expand(M, E), A, generator=g).int()
+        ids = torch.randperm(E, generator=g, device="cuda").int()[ids.long()]
     if kind == "bad":
         ids[0, 0], ids[M - 1, A - 1] = -1, E
     if kind == "none":
@@ -252,7 +256,8 @@ def some_ids(g, M, A, E, kind):
 
 @pytest.mark.parametrize("M,A,E,N,Kd,kind", [(1, 1, 1, 128, 128, ""), (1, 8, 64, 1024, 512, ""), (6, 10, 64, 512, 640, "bad"), (1, 3, 5, 100, 144, "bad"), (40, 4, 16, 256, 256, "one"),
                                              (300, 2, 8, 136, 1040, "bad"), (700, 3, 6, 257, 272, "one"), (9, 2, 1023, 16, 16, ""), (33, 64, 7, 128, 128, ""), (5, 4, 8, 128, 256, "none"),
-                                             (600, 8, 16, 640, 384, ""), (1000, 6, 300, 128, 128, "bad")])
+                                             (600, 8, 16, 640, 384, ""), (1000, 6, 300, 128, 128, "bad"), (4000, 4, 96, 1000, 640, "steep"), (700, 2, 64, 2048, 512, "steep"), (200, 4, 100, 2048, 512, "steep"),
+                                             (6, 10, 512, 2048, 512, "steep")])
 def test_experts(M, A, E, N, Kd, kind):
     g = gen(M * A + E + N)
     ids = some_ids(g, M, A, E, kind)
