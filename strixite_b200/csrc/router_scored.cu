@@ -13,6 +13,7 @@
 
 #include "strixite_b200.h"
 
+#include <cfloat>
 #include <climits>
 
 namespace {
@@ -61,7 +62,22 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
-// A token in 64 bits, one warp, finite logits and bias. Lane `sub` of group g holds the group's experts sub, sub + L, .. Seldom run, so its
+// A score in 64 bits (softmax: top and sum of the token's exponentials).
+__device__ __noinline__ double score_64(float l, float top, double sum, int kind) {
+    const double e = exp(kind == kSigmoid ? -(double)l : (double)l - (double)top);
+    return kind == kSigmoid ? 1.0 / (1.0 + e) : e / sum;
+}
+// sum of exp(l - top) over a token's experts, one warp.
+template <typename T>
+__device__ __noinline__ double softmax_sum_64(const T *row, int E, float top) {
+    double sum = 0.0;
+#pragma unroll 4
+    for (int e = threadIdx.x & 31; e < E; e += 32) sum += exp((double)ld_act(row, e) - (double)top);
+    return warp_sum_d(sum);
+}
+
+// A token in 64 bits from end to end, one warp, finite logits and bias: for what the FP32 path leaves (scores outside FP32's range, hundreds
+// of candidates). Lane `sub` of group g holds the group's experts sub, sub + L, .. Seldom run, so its
 // loops are not unrolled and its values live in local memory: it must not cost the FP32 path registers.
 template <typename T>
 __device__ __noinline__ void route_64(const T *row, const RouteArgs &a, int64_t m) {
@@ -70,18 +86,15 @@ __device__ __noinline__ void route_64(const T *row, const RouteArgs &a, int64_t 
     const int n = g < a.G && sub < a.per ? (a.per - sub + a.L - 1) / a.L : 0;
     double c[64];  // of the lane's experts: what they are chosen by
     auto expert = [&](int j) { return g * a.per + sub + a.L * j; };
-    double top = -INFINITY, sum = 1.0;
+    float top = -INFINITY;
+    double sum = 1.0;
     if (a.score == kSoftmax) {
 #pragma unroll 1
-        for (int j = 0; j < n; ++j) top = fmax(top, (double)ld_act(row, expert(j)));
-#pragma unroll 1
-        for (int off = 16; off > 0; off >>= 1) top = fmax(top, __shfl_xor_sync(full, top, off));
-        sum = 0.0;
-#pragma unroll 1
-        for (int j = 0; j < n; ++j) sum += exp((double)ld_act(row, expert(j)) - top);
-        sum = warp_sum_d(sum);
+        for (int j = 0; j < n; ++j) top = fmaxf(top, ld_act(row, expert(j)));
+        top = warp_max(top);
+        sum = softmax_sum_64(row, a.E, top);
     }
-    auto score = [&](float l) { return a.score == kSigmoid ? 1.0 / (1.0 + exp(-(double)l)) : exp((double)l - top) / sum; };
+    auto score = [&](float l) { return score_64(l, top, sum, a.score); };
     const bool biased = a.bias != nullptr;
 #pragma unroll 1
     for (int j = 0; j < n; ++j) {
@@ -147,18 +160,27 @@ __device__ __forceinline__ float4 load4(const uint16_t *p) {
 // One warp per token. The lanes are dealt to the groups (a group's L neighbouring lanes hold its experts, NV a lane, in runs of four where
 // VEC), so a group's value is a reduction over L lanes and a closed group is a lane that drops out.
 // The choice: the k-th largest lane maximum bounds the k-th largest value from below, what reaches it are the candidates (about 1.3 k of
-// them), they meet in shared memory and each counts those in front of it: no k rounds of warp-wide maxima.
+// them), they meet in shared memory and each counts those in front of it: no k rounds of warp-wide maxima. Where neighbours in that
+// order are closer than the error, the candidates are valued again in 64 bits (one token in a thousand).
 //
-// The FP32 errors that the choice allows for (documented bounds: expf 2 ulp, __expf 2 + 1.17 |x| ulp, __fdividef 2 ulp):
-//   sigmoid  e = __expf(-l): p moves by p (1 - p) (2 + 1.17 |l|) 2^-23 <= 0.77 * 2^-23, 1 + e by 2^-24, the quotient by 2^-22: 3.3 * 2^-23, for
-//            two values 6.6 * 2^-23 < 2^-20
+// The FP32 errors that the choice allows for (documented bounds: expf 2 ulp; ex2.approx 2^-22, rcp.approx 2^-23 relative):
+//   sigmoid  e = 2^(-l log2 e): the argument's roundings move e by 1.5 |l| 2^-24, so p by p (1 - p) (2^-22 + 1.5 |l| 2^-24) <= 0.7 * 2^-23; 1 + e
+//            and the reciprocal by 1.5 * 2^-23: 2.2 * 2^-23, for two values 4.4 * 2^-23 < 2^-20
 //   softmax  e = expf(l - top): (2 + |x| / 2) 2^-23 of e; the sum of up to 64 a lane and 5 steps: 35 * 2^-23 and the terms' mean, at most
 //            2 + ln(1024) / 2; p by at most 45 * 2^-23 of the largest p, for two values 90 * 2^-23 < 2^-16
 //   c = p + bias one rounding each, 2^-24 |c|: 2^-22 (|c| + |c'|) is above both
+__device__ __forceinline__ float fast_sigmoid(float l) {
+    float e, p;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(l * -1.44269504f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(1.0f + e));
+    return p;
+}
+
 template <typename T, int NV, bool VEC>
 __global__ void __launch_bounds__(kWarps * 32) router_scored_kernel(const T *logits, const T *shared, const RouteArgs a) {
-    __shared__ uint64_t cand[kWarps][kMaxCand];
-    __shared__ uint64_t sorted[kWarps][40];
+    __shared__ float2 cand[kWarps][kMaxCand];  // value, expert (as bits)
+    __shared__ double exact[kWarps][kMaxCand];  // of a close token: the candidates' values in 64 bits
+    __shared__ float2 sorted[kWarps][40];
     const unsigned full = 0xffffffffu;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t m = (int64_t)blockIdx.x * kWarps + warp;
@@ -207,23 +229,23 @@ __global__ void __launch_bounds__(kWarps * 32) router_scored_kernel(const T *log
     if (biased) {
         const float inv = 1.0f / sum;
         base = a.score == kSigmoid ? 0x1p-20f : 0x1p-16f * inv;
+        auto choose_by = [&](auto score) {
 #pragma unroll
-        for (int j = 0; j < NV; j += VEC ? 4 : 1) {
-            if (!holds(j)) continue;
-            float b[4];
-            if constexpr (VEC) {
-                const float4 v = load4(a.bias + expert(j));
-                b[0] = v.x, b[1] = v.y, b[2] = v.z, b[3] = v.w;
-            } else {
-                b[0] = a.bias[expert(j)];
+            for (int j = 0; j < NV; j += VEC ? 4 : 1) {
+                if (!holds(j)) continue;
+                if constexpr (VEC) {
+                    const float4 v = load4(a.bias + expert(j));
+                    chk = fmaf(v.x, 0.f, fmaf(v.y, 0.f, fmaf(v.z, 0.f, fmaf(v.w, 0.f, chk))));
+                    c[j] = score(c[j]) + v.x, c[j + 1] = score(c[j + 1]) + v.y, c[j + 2] = score(c[j + 2]) + v.z, c[j + 3] = score(c[j + 3]) + v.w;
+                } else {
+                    const float v = a.bias[expert(j)];
+                    chk = fmaf(v, 0.f, chk);
+                    c[j] = score(c[j]) + v;
+                }
             }
-#pragma unroll
-            for (int i = 0; i < (VEC ? 4 : 1); ++i) {
-                chk = fmaf(b[i], 0.f, chk);
-                const float l = c[j + i];
-                c[j + i] = (a.score == kSigmoid ? __fdividef(1.0f, 1.0f + __expf(-l)) : expf(l - top) * inv) + b[i];
-            }
-        }
+        };
+        if (a.score == kSigmoid) choose_by([](float l) { return fast_sigmoid(l); });
+        else choose_by([&](float l) { return expf(l - top) * inv; });
     }
     if (__any_sync(full, !(chk == 0.f))) {  // a non-finite logit or bias fails the token: ids -1, coefficients NaN
         unsigned bad = UINT_MAX;
@@ -236,7 +258,7 @@ __global__ void __launch_bounds__(kWarps * 32) router_scored_kernel(const T *log
         return;
     }
 
-    bool close = false;  // two values that the choice tells apart lie within the error
+    double sum64 = 0.0;  // of the softmax, where something is done in 64 bits
     if (a.topk_group < a.G) {
         float b1 = -INFINITY, b2 = -INFINITY;  // the two largest of the lane, then of the group
 #pragma unroll
@@ -252,7 +274,7 @@ __global__ void __launch_bounds__(kWarps * 32) router_scored_kernel(const T *log
         float value = b1, tol = 0.f;
         if (a.group_top == 2 && a.per > 1) {
             if (biased) value = b1 + b2, tol = 2.f * base + 0x1p-21f * (fabsf(b1) + fabsf(b2));
-            else if (a.score == kSigmoid) value = __fdividef(1.0f, 1.0f + __expf(-b1)) + __fdividef(1.0f, 1.0f + __expf(-b2)), tol = 0x1p-18f;
+            else if (a.score == kSigmoid) value = fast_sigmoid(b1) + fast_sigmoid(b2), tol = 0x1p-18f;
             else value = expf(b1 - top) + expf(b2 - top), tol = 0x1p-18f;
         } else if (biased) {
             tol = base + 0x1p-21f * fabsf(b1);
@@ -262,40 +284,66 @@ __global__ void __launch_bounds__(kWarps * 32) router_scored_kernel(const T *log
             const float o = __shfl_sync(full, value, h * L);
             rank += o > value || (o == value && h < g);
         }
-        const bool open = g < a.G && rank < a.topk_group;
-        if (!open) {
-#pragma unroll
-            for (int j = 0; j < NV; ++j) c[j] = -INFINITY;
-        }
+        bool open = g < a.G && rank < a.topk_group;
         if (biased || (a.group_top == 2 && a.per > 1)) {  // else the values are exact
             const float worst = __uint_as_float(__reduce_max_sync(full, g < a.G ? __float_as_uint(tol) : 0u));
             const float least_open = key_value(__reduce_min_sync(full, open ? order_key(value) : UINT_MAX));
             const float most_shut = key_value(__reduce_max_sync(full, g < a.G && !open ? order_key(value) : order_key(-INFINITY)));
-            close = !(least_open - most_shut > worst);
+            if (!(least_open - most_shut > worst)) {
+                // Too close to tell: the groups' values in 64 bits, from the experts that FP32 does not rule out as one of their largest.
+                if (a.score == kSoftmax) sum64 = softmax_sum_64(row, a.E, top);
+                const float least = a.group_top == 2 && a.per > 1 ? b2 : b1, reach = biased ? least - (base + 0x1p-21f * fabsf(least)) : least;
+                uint64_t mask = 0;
+#pragma unroll
+                for (int j = 0; j < NV; ++j) mask |= (uint64_t)(c[j] >= reach && c[j] > -INFINITY) << j;
+                double d1 = -INFINITY, d2 = -INFINITY;
+#pragma unroll 1
+                while (mask != 0) {
+                    const int e = expert(__ffsll((long long)mask) - 1);
+                    mask &= mask - 1;
+                    const double v = score_64(ld_act(row, e), top, sum64, a.score) + (biased ? (double)a.bias[e] : 0.0);
+                    d2 = fmax(d2, fmin(d1, v)), d1 = fmax(d1, v);
+                }
+                __syncwarp();
+#pragma unroll 1
+                for (int off = L / 2; off > 0; off >>= 1) {
+                    const double o1 = __shfl_xor_sync(full, d1, off), o2 = __shfl_xor_sync(full, d2, off);
+                    d2 = fmax(fmax(d2, o2), fmin(d1, o1)), d1 = fmax(d1, o1);
+                }
+                const double exact_value = a.group_top == 2 && a.per > 1 ? d1 + d2 : d1;
+                rank = 0;
+#pragma unroll 1
+                for (int h = 0; h < a.G; ++h) {
+                    const double o = __shfl_sync(full, exact_value, h * L);
+                    rank += o > exact_value || (o == exact_value && h < g);
+                }
+                open = g < a.G && rank < a.topk_group;
+            }
+        }
+        if (!open) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) c[j] = -INFINITY;
         }
     }
 
     int n = 0;  // candidates
-    if (!close) {
+    {
         float lm = -INFINITY;
 #pragma unroll
         for (int j = 0; j < NV; ++j) lm = fmaxf(lm, c[j]);
-        // the lane maxima in descending order (a bitonic network over the lanes), of which the k-th
-#pragma unroll
-        for (int size = 2; size <= 32; size *= 2) {
-#pragma unroll
-            for (int off = size / 2; off > 0; off /= 2) {
-                const float o = __shfl_xor_sync(full, lm, off);
-                const bool larger = ((lane & off) == 0) == ((lane & size) == 0);  // this lane keeps the larger of the two
-                lm = larger ? fmaxf(lm, o) : fminf(lm, o);
-            }
+        // the k-th largest lane maximum: k rounds of the warp's maximum (a hardware reduction of the ordered bits), the lane that held it out
+        uint32_t key = order_key(lm), kth_key = 0;
+        for (int r = 0; r < a.k; ++r) {
+            kth_key = __reduce_max_sync(full, key);
+            if (key == kth_key) key = 0;  // equal maxima go together: the bound is only lower
         }
-        const float kth = __shfl_sync(full, lm, a.k - 1);
-        // what lies below the k-th by no more than the error is a candidate too: nothing that is left out can belong to the picks
-        const float bound = biased ? kth - (base + 0x1p-21f * fabsf(kth)) : kth;
+        const float kth = kth_key == 0 ? -INFINITY : key_value(kth_key);
+        // what lies below the k-th by no more than the error is a candidate too: nothing that is left out can belong to the picks.
+        // -FLT_MAX: every finite value where fewer than k lanes are open.
+        const float bound = fmaxf(biased ? kth - (base + 0x1p-21f * fabsf(kth)) : kth, -FLT_MAX);
         int mine = 0;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) mine += c[j] >= bound && c[j] > -INFINITY;
+        for (int j = 0; j < NV; ++j) mine += c[j] >= bound;
         int at = mine;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -306,36 +354,62 @@ __global__ void __launch_bounds__(kWarps * 32) router_scored_kernel(const T *log
         at -= mine;
         if (n <= kMaxCand) {
 #pragma unroll
-            for (int j = 0; j < NV; ++j)
-                if (c[j] >= bound && c[j] > -INFINITY) cand[warp][at++] = ((uint64_t)order_key(c[j]) << 32) | (uint32_t)~expert(j);
+            for (int j = 0; j < NV; ++j) {
+                const bool in = c[j] >= bound;
+                if (in) cand[warp][at] = make_float2(c[j], __int_as_float(expert(j)));
+                at += in;
+            }
             __syncwarp();
-            // a larger key is in front: larger value, then lower expert; the keys differ, so the ranks are 0 .. n - 1
+            // in front: a larger value, then the lower expert; no two candidates are equal in both, so the ranks are 0 .. n - 1
             for (int i = lane; i < n; i += 32) {
-                const uint64_t key = cand[warp][i];
+                const float2 own = cand[warp][i];
                 int rank = 0;
-                for (int q = 0; q < n; ++q) rank += cand[warp][q] > key;
-                if (rank <= a.k) sorted[warp][rank] = key;
+#pragma unroll 4
+                for (int q = 0; q < n; ++q) {
+                    const float2 o = cand[warp][q];
+                    rank += o.x > own.x || (o.x == own.x && __float_as_int(o.y) < __float_as_int(own.y));
+                }
+                if (rank <= a.k) sorted[warp][rank] = own;
             }
             __syncwarp();
         }
     }
     int pick = -1;
-    float l = 0.f, value = 0.f;
-    if (!close && n <= kMaxCand) {
-        if (lane < a.k) {
-            const uint64_t key = sorted[warp][lane];
-            pick = (int)~(uint32_t)key, value = key_value((uint32_t)(key >> 32));
-            if (biased && lane + 1 < n) {
-                const float next = key_value((uint32_t)(sorted[warp][lane + 1] >> 32));
-                close = !(value - next > base + 0x1p-22f * (fabsf(value) + fabsf(next)));
-            }
-            l = ld_act(row, pick);
-            close |= (a.score == kSigmoid ? l : l - top) < -80.f;  // the score leaves FP32's normal range
+    float l = 0.f;
+    bool out = n > kMaxCand;  // for the 64-bit path
+    if (!out) {
+        bool near = false;
+        if (biased && lane < a.k && lane + 1 < n) {
+            const float value = sorted[warp][lane].x, next = sorted[warp][lane + 1].x;
+            near = !(value - next > base + 0x1p-22f * (fabsf(value) + fabsf(next)));
         }
-    } else {
-        close = true;
+        if (__any_sync(full, near)) {
+            // the candidates once more, in 64 bits
+            if (a.score == kSoftmax && sum64 == 0.0) sum64 = softmax_sum_64(row, a.E, top);
+#pragma unroll 1
+            for (int i = lane; i < n; i += 32) {
+                const int e = __float_as_int(cand[warp][i].y);
+                exact[warp][i] = score_64(ld_act(row, e), top, sum64, a.score) + (double)a.bias[e];
+            }
+            __syncwarp();
+#pragma unroll 1
+            for (int i = lane; i < n; i += 32) {
+                const float2 own = cand[warp][i];
+                const double v = exact[warp][i];
+                int rank = 0;
+#pragma unroll 1
+                for (int q = 0; q < n; ++q) rank += exact[warp][q] > v || (exact[warp][q] == v && __float_as_int(cand[warp][q].y) < __float_as_int(own.y));
+                if (rank <= a.k) sorted[warp][rank] = own;
+            }
+            __syncwarp();
+        }
+        if (lane < a.k) {
+            pick = __float_as_int(sorted[warp][lane].y);
+            l = ld_act(row, pick);
+            out = (a.score == kSigmoid ? l : l - top) < -80.f;  // the score leaves FP32's normal range
+        }
     }
-    if (__any_sync(full, close)) {
+    if (__any_sync(full, out)) {
         route_64(row, a, m);
     } else {
         float p = 0.f;
