@@ -18,9 +18,8 @@ __device__ __forceinline__ float max_abs(float a, float v) {
     return r;
 }
 
-// The scale of a block from its largest magnitude: 448 (the largest e4m3 value) stands for it. The floor 2^-100 gives a block of
-// zeros a scale that divides and keeps the quotient away from the subnormals; a NaN stays one.
-__device__ __forceinline__ float fp8_scale(float amax) { return max_abs(0x1p-100f, amax) / 448.0f; }
+// The scale of a block is its largest magnitude / 448 (the largest e4m3 value stands for it), at least 2^-100 / 448: a block of zeros has
+// a scale that divides. A NaN stays one.
 
 // Two values in e4m3, round to nearest even, saturating at +-448 (NaN -> the NaN code); `lo` in the low byte.
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
@@ -29,48 +28,60 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     return r;
 }
 
-// v / d to the last bit or the one next to it: the hardware's approximate reciprocal r of d (1 ulp), the quotient v * r (2 ulp) and one
-// correction by its remainder, which the FMA gives exactly (Markstein's step). d and v / d well inside FP32's range.
-__device__ __forceinline__ float fast_rcp(float d) {
+__device__ __forceinline__ float fast_rcp(float d) {  // 1 ulp; 1 / d inside FP32's normal range
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
     return r;
 }
-__device__ __forceinline__ float quotient(float v, float d, float r) {
-    const float q = v * r;
-    return fmaf(fmaf(-q, d, v), r, q);
-}
 
-// 8 values of one block -> 8 e4m3 bytes of v / scale. A product with the reciprocal alone would move values that lie next to a
-// rounding border; 8 IEEE divisions cost as many instructions as the rest of the kernels that use this.
-__device__ __forceinline__ uint2 fp8_pack8(const float (&v)[8], float scale) {
+// What the 8 values of a thread are to the block that they belong to: v = hi + lo unevaluated, so that a product's rounding does not reach
+// the codes. An e4m3 code changes where the value crosses the middle between two neighbours; every FP32 rounding in front of it
+// moves a value across with a chance of about 2^-21, and a matrix has tens of millions of them.
+struct Block8 {
+    float hi[8], lo[8];
+};
+
+// The 8 values (times `unit`, a factor that the block shares) as e4m3 bytes of v / scale, scale = max(amax * unit, 2^-100) / 448. The quotient
+// is taken against the unrounded block maximum, in which the unit cancels: 448 / amax as two floats, three FMAs a value.
+__device__ __forceinline__ uint2 fp8_pack8(const Block8 &v, float amax, float unit, float &scale) {
     uint32_t h[4];
-    if (scale < 0x1p100f) {
-        const float r = fast_rcp(scale);
+    const float top = amax * unit;
+    if (top >= 0x1p-100f && amax > 0x1p-60f && amax < 0x1p60f) {
+        const float s = top * (1.0f / 448.0f);
+        scale = fmaf(fmaf(-s, 448.0f, top), 1.0f / 448.0f, s);
+        float r = fast_rcp(amax);
+        r = fmaf(fmaf(-r, amax, 1.0f), r, r);
+        const float inv = 448.0f * r, rest = fmaf(-inv, amax, 448.0f) * r;  // 448 / amax = inv + rest
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = e4m3x2(quotient(v[2 * i], scale, r), quotient(v[2 * i + 1], scale, r));
-    } else {  // near FP32's end, infinite or NaN
+        for (int i = 0; i < 4; ++i) {
+            const float a = fmaf(v.hi[2 * i], inv, fmaf(v.hi[2 * i], rest, v.lo[2 * i] * inv));
+            const float b = fmaf(v.hi[2 * i + 1], inv, fmaf(v.hi[2 * i + 1], rest, v.lo[2 * i + 1] * inv));
+            h[i] = e4m3x2(a, b);
+        }
+    } else {  // near FP32's ends, zero, infinite or NaN: word for word
+        scale = __fdiv_rn(max_abs(0x1p-100f, top), 448.0f);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = e4m3x2(__fdiv_rn(v[2 * i], scale), __fdiv_rn(v[2 * i + 1], scale));
+        for (int i = 0; i < 4; ++i) h[i] = e4m3x2(__fdiv_rn(v.hi[2 * i] * unit, scale), __fdiv_rn(v.hi[2 * i + 1] * unit, scale));
     }
     return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
 }
 
-// silu(g) * u of 8 pairs with the same division; where a gate is near the ends of the exponential's range (or infinite), as the
-// definition says.
-__device__ __forceinline__ void swiglu8(const float (&g)[8], const float (&u)[8], float (&h)[8]) {
+// silu(g) * u of 8 pairs: g / (1 + e) by the approximate reciprocal and one correction by the exact remainder (Markstein's step). Where a
+// gate is near the ends of the exponential's range (or infinite), as the definition says.
+__device__ __forceinline__ void swiglu8(const float (&g)[8], const float (&u)[8], Block8 &h) {
     float most = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(g[j]));
     if (most < 80.0f) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float d = 1.0f + expf(-g[j]);
-            h[j] = quotient(g[j], d, fast_rcp(d)) * u[j];
+            const float d = 1.0f + expf(-g[j]), r = fast_rcp(d), q = g[j] * r, silu = fmaf(fmaf(-q, d, g[j]), r, q);
+            h.hi[j] = silu * u[j];
+            h.lo[j] = fmaf(silu, u[j], -h.hi[j]);
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) h[j] = silu_f(g[j]) * u[j];
+        for (int j = 0; j < 8; ++j) h.hi[j] = silu_f(g[j]) * u[j], h.lo[j] = 0.f;
     }
 }
 

@@ -17,8 +17,10 @@ constexpr int kNormMaxVec = 8;  // 8-element pieces a thread can hold: d <= 256 
 // Bound by memory: nothing is read twice, and the row's values never leave the registers.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kNormMaxThreads)
-    rmsnorm_fp8_kernel(const T *x, const T *y, const float *w, float w_add, float eps, int d, T *x_out, T *h_out, uint8_t *q, float *scale, int blocks) {
-    __shared__ float part[kNormMaxThreads / 32];
+    rmsnorm_fp8_kernel(const T *x, const T *y, const float *w, float w_add, float eps, int d, float inv_d, T *x_out, T *h_out, uint8_t *q, float *scale,
+                       int blocks) {
+    constexpr int kWarps = kNormMaxThreads / 32;
+    __shared__ alignas(16) float part[kWarps];
     const int64_t row = blockIdx.x, base = row * d;
     float v[VEC][8];
     float sq = 0.f;
@@ -44,27 +46,45 @@ __global__ void __launch_bounds__(kNormMaxThreads)
     sq = warp_sum(sq);
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sq;
     __syncthreads();
+    // every thread adds the warps' sums in the same order; a root of the mean by the approximate instruction and one Newton step
     float total = 0.f;
-    for (int i = 0; i < (int)blockDim.x / 32; ++i) total += part[i];
-    const float r = 1.0f / sqrtf(total / (float)d + eps);
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) total += i < (int)blockDim.x / 32 ? part[i] : 0.f;
+    const float mean = fmaf(total, inv_d, eps);
+    float r;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(mean));
+    if (mean > 0x1p-100f && mean < 0x1p100f) r = fmaf(r * 0.5f, fmaf(-mean * r, r, 1.0f), r);
+    else r = 1.0f / sqrtf(mean);
+    const bool plain = !(r > 0x1p-60f && r < 0x1p60f);  // a row near FP32's ends (or with an infinity, a NaN): h first, then its codes
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
         const int c = (threadIdx.x + i * blockDim.x) * 8;
         float top = 0.f;
+        Block8 p;  // x' g in two parts (h / r), or h
         if (c < d) {
-            float g[8];
+            float g[8], h[8];
             load8(w + c, g);
+            if (!plain) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[i][j] = v[i][j] * r * (g[j] + w_add);
-                top = max_abs(top, v[i][j]);
+                for (int j = 0; j < 8; ++j) {
+                    const float gain = g[j] + w_add;
+                    p.hi[j] = v[i][j] * gain;
+                    p.lo[j] = fmaf(v[i][j], gain, -p.hi[j]);
+                    h[j] = p.hi[j] * r;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) h[j] = p.hi[j] = v[i][j] * r * (g[j] + w_add), p.lo[j] = 0.f;
             }
-            if (h_out != nullptr) store8(h_out + base + c, v[i]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = max_abs(top, p.hi[j]);
+            if (h_out != nullptr) store8(h_out + base + c, h);
         }
         if (q != nullptr) {  // the same for the whole grid; the reduction runs on full warps
-            const float s = fp8_scale(half_warp_max(top));
+            top = half_warp_max(top);
             if (c < d) {
-                *reinterpret_cast<uint2 *>(q + base + c) = fp8_pack8(v[i], s);
+                float s;
+                *reinterpret_cast<uint2 *>(q + base + c) = fp8_pack8(p, top, plain ? 1.0f : r, s);
                 if ((c & (kFp8Block - 1)) == 0) scale[row * blocks + c / kFp8Block] = s;
             }
         }
@@ -80,7 +100,7 @@ void launch_norm(const void *x, const void *y, const float *w, float w_add, floa
     const int threads = ((pieces + vec - 1) / vec + 31) / 32 * 32;
     const int blocks = (int)fp8_blocks(d);
 #define SB_NORM(V) \
-    rmsnorm_fp8_kernel<T, V><<<(unsigned)M, threads, 0, st>>>((const T *)x, (const T *)y, w, w_add, eps, (int)d, (T *)x_out, (T *)h, q, scale, blocks)
+    rmsnorm_fp8_kernel<T, V><<<(unsigned)M, threads, 0, st>>>((const T *)x, (const T *)y, w, w_add, eps, (int)d, 1.0f / (float)d, (T *)x_out, (T *)h, q, scale, blocks)
     if (vec == 1) SB_NORM(1);
     else if (vec == 2) SB_NORM(2);
     else if (vec == 4) SB_NORM(4);
@@ -90,16 +110,23 @@ void launch_norm(const void *x, const void *y, const float *w, float w_add, floa
 
 // A half warp per (row, 128-column block) of h = silu(gate) * up, 8 elements a thread. Gate and up stay FP32 until the one rounding
 // to e4m3.
-template <typename T, typename Index>
-__global__ void __launch_bounds__(256) swiglu_fp8_kernel(const T *gu, uint8_t *q, float *scale, int64_t rows, int I, int blocks) {
+// u / blocks for u < 2^31: (u * mul) >> shift with mul = ceil(2^shift / blocks), shift = 31 + ceil(log2 blocks) (the excess of mul * blocks
+// over 2^shift is below blocks <= 2^(shift - 31), so u times it stays below 2^shift). mul = 0: by division.
+struct RowOf {
+    uint32_t mul;
+    int shift;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256, 6) swiglu_fp8_kernel(const T *gu, uint8_t *q, float *scale, int64_t rows, int I, int blocks, RowOf row_of) {
     const int64_t units = rows * blocks, stride = (int64_t)gridDim.x * (blockDim.x / 16);
     const int t = threadIdx.x & 15;
     for (int64_t u0 = (int64_t)blockIdx.x * (blockDim.x / 16); u0 < units; u0 += stride) {
         const int64_t u = u0 + threadIdx.x / 16;
-        const int64_t row = (Index)u / (Index)blocks;  // 32 bits where they hold it: a 64-bit division is 80 instructions
+        const int64_t row = row_of.mul != 0 ? (int64_t)((uint64_t)(uint32_t)u * row_of.mul >> row_of.shift) : u / blocks;
         const int b = (int)(u - row * blocks), c = b * kFp8Block + t * 8;
         const bool live = u < units && c < I;
-        float h[8];
+        Block8 h;
         float top = 0.f;
         if (live) {
             float g[8], up[8];
@@ -107,11 +134,12 @@ __global__ void __launch_bounds__(256) swiglu_fp8_kernel(const T *gu, uint8_t *q
             load8(gu + row * 2 * I + I + c, up);
             swiglu8(g, up, h);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = max_abs(top, h[j]);
+            for (int j = 0; j < 8; ++j) top = max_abs(top, h.hi[j]);
         }
-        const float s = fp8_scale(half_warp_max(top));
+        top = half_warp_max(top);
         if (live) {
-            *reinterpret_cast<uint2 *>(q + row * I + c) = fp8_pack8(h, s);
+            float s;
+            *reinterpret_cast<uint2 *>(q + row * I + c) = fp8_pack8(h, top, 1.0f, s);
             if (t == 0) scale[u] = s;
         }
     }
@@ -172,13 +200,15 @@ int strix_swiglu_fp8(const void *gu, uint8_t *q, float *scale, int64_t rows, int
     const int64_t units = rows * blocks, want = (units + 15) / 16, cap = (int64_t)sm_count() * 32;
     const unsigned grid = (unsigned)(want < cap ? want : cap);
     auto st = static_cast<cudaStream_t>(stream);
-    const bool small = units + cap * 16 < (1ll << 31);
-#define SB_SWIGLU(T, INDEX) swiglu_fp8_kernel<T, INDEX><<<grid, 256, 0, st>>>((const T *)gu, q, scale, rows, (int)I, blocks)
-    if (act == kF32 && small) SB_SWIGLU(float, uint32_t);
-    else if (act == kF32) SB_SWIGLU(float, int64_t);
-    else if (small) SB_SWIGLU(uint16_t, uint32_t);
-    else SB_SWIGLU(uint16_t, int64_t);
-#undef SB_SWIGLU
+    RowOf row_of{0, 0};
+    if (units + cap * 16 < (1ll << 31)) {
+        int log = 0;
+        while ((1 << log) < blocks) ++log;
+        row_of.shift = 31 + log;
+        row_of.mul = (uint32_t)(((1ull << row_of.shift) + blocks - 1) / blocks);
+    }
+    if (act == kF32) swiglu_fp8_kernel<float><<<grid, 256, 0, st>>>((const float *)gu, q, scale, rows, (int)I, blocks, row_of);
+    else swiglu_fp8_kernel<uint16_t><<<grid, 256, 0, st>>>((const uint16_t *)gu, q, scale, rows, (int)I, blocks, row_of);
     SB_LAUNCH_OK(fn, " ", act_name(act), " rows=", rows, " I=", I);
     return 0;
 }
