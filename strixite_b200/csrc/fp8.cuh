@@ -11,11 +11,19 @@ constexpr int kFp8Block = 128;
 inline int64_t fp8_blocks(int64_t n) { return (n + kFp8Block - 1) / kFp8Block; }
 
 #ifdef __CUDACC__
-// The larger of a and |v|; a NaN in either stays one (fmaxf would drop it).
+// The largest magnitude of a, v and w; a NaN in any stays one (fmaxf would drop it).
+__device__ __forceinline__ float max_abs(float a, float v, float w) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(v), "f"(w));
+    return r;
+}
 __device__ __forceinline__ float max_abs(float a, float v) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(v)));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(v)));
     return r;
+}
+__device__ __forceinline__ float max_abs8(const float (&v)[8]) {
+    return max_abs(max_abs(v[0], v[1], v[2]), max_abs(v[3], v[4], v[5]), max_abs(v[6], v[7]));
 }
 
 // The scale of a block is its largest magnitude / 448 (the largest e4m3 value stands for it), at least 2^-100 / 448: a block of zeros has
@@ -66,16 +74,22 @@ __device__ __forceinline__ uint2 fp8_pack8(const Block8 &v, float amax, float un
     return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
 }
 
+// e^-g for |g| < 80: 2^t with t = -g log2(e) in two parts (log2(e) = 1.44269502 + 1.93e-8), the second applied to first order. Off by the
+// 2^-22 of ex2.approx and two roundings.
+__device__ __forceinline__ float exp_neg(float g) {
+    const float t = g * -1.44269502f, rest = fmaf(g, -1.92596299e-8f, fmaf(g, -1.44269502f, -t));
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+    return fmaf(e * 0.693147181f, rest, e);
+}
+
 // silu(g) * u of 8 pairs: g / (1 + e) by the approximate reciprocal and one correction by the exact remainder (Markstein's step). Where a
-// gate is near the ends of the exponential's range (or infinite), as the definition says.
+// gate is near the ends of the exponential's range (or infinite, or NaN), as the definition says.
 __device__ __forceinline__ void swiglu8(const float (&g)[8], const float (&u)[8], Block8 &h) {
-    float most = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(g[j]));
-    if (most < 80.0f) {
+    if (max_abs8(g) < 80.0f) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float d = 1.0f + expf(-g[j]), r = fast_rcp(d), q = g[j] * r, silu = fmaf(fmaf(-q, d, g[j]), r, q);
+            const float d = 1.0f + exp_neg(g[j]), r = fast_rcp(d), q = g[j] * r, silu = fmaf(fmaf(-q, d, g[j]), r, q);
             h.hi[j] = silu * u[j];
             h.lo[j] = fmaf(silu, u[j], -h.hi[j]);
         }

@@ -76,8 +76,7 @@ __global__ void __launch_bounds__(kNormMaxThreads)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) h[j] = p.hi[j] = v[i][j] * r * (g[j] + w_add), p.lo[j] = 0.f;
             }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) top = max_abs(top, p.hi[j]);
+            top = max_abs8(p.hi);
             if (h_out != nullptr) store8(h_out + base + c, h);
         }
         if (q != nullptr) {  // the same for the whole grid; the reduction runs on full warps
@@ -133,8 +132,7 @@ __global__ void __launch_bounds__(256, 6) swiglu_fp8_kernel(const T *gu, uint8_t
             load8(gu + row * 2 * I + c, g);
             load8(gu + row * 2 * I + I + c, up);
             swiglu8(g, up, h);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) top = max_abs(top, h.hi[j]);
+            top = max_abs8(h.hi);
         }
         top = half_warp_max(top);
         if (live) {
