@@ -13,6 +13,7 @@
 #include <sstream>
 #include <string>
 #include <type_traits>
+#include <utility>
 
 #define STRIX_OK 0
 #define STRIX_ERR_CHECK 1
@@ -89,6 +90,26 @@ inline bool bits_ok(int b) { return b == 4 || b == 5 || b == 6 || b == 8; }
 inline bool group_ok(int64_t G) { return G == 32 || G == 64 || G == 128; }
 
 int sm_count();  // of the current device, cached (api.cu)
+
+#ifdef __CUDACC__
+// A launch that may begin before the kernel in front of it on the stream has ended (programmatic dependent launch): its blocks are set up
+// while that one drains, and kernel code calls wait_for_previous() before it touches global memory. cluster: blocks per cluster.
+template <typename... Params, typename... Args>
+inline cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster, Args &&...args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization, attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr, cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+// Lets the next kernel on the stream be set up, if it was launched that way; then waits until everything in front of this kernel has
+// completed and is visible. Both are nothing where the launch was an ordinary one.
+__device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+#endif
 
 // ---- device helpers --------------------------------------------------------------------------------------------
 #ifdef __CUDACC__

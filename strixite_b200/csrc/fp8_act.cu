@@ -19,6 +19,8 @@ template <typename T, int VEC>
 __global__ void __launch_bounds__(kNormMaxThreads)
     rmsnorm_fp8_kernel(const T *x, const T *y, const float *w, float w_add, float eps, int d, float inv_d, T *x_out, T *h_out, uint8_t *q, float *scale,
                        int blocks) {
+    let_next_begin();
+    wait_for_previous();
     constexpr int kWarps = kNormMaxThreads / 32;
     __shared__ alignas(16) float part[kWarps];
     const int64_t row = blockIdx.x, base = row * d;
@@ -91,7 +93,7 @@ __global__ void __launch_bounds__(kNormMaxThreads)
 }
 
 template <typename T>
-void launch_norm(const void *x, const void *y, const float *w, float w_add, float eps, int64_t M, int64_t d, void *x_out, void *h, uint8_t *q, float *scale,
+cudaError_t launch_norm(const void *x, const void *y, const float *w, float w_add, float eps, int64_t M, int64_t d, void *x_out, void *h, uint8_t *q, float *scale,
                  cudaStream_t st) {
     const int pieces = (int)(d / 8);
     int vec = 1;
@@ -99,11 +101,9 @@ void launch_norm(const void *x, const void *y, const float *w, float w_add, floa
     const int threads = ((pieces + vec - 1) / vec + 31) / 32 * 32;
     const int blocks = (int)fp8_blocks(d);
 #define SB_NORM(V) \
-    rmsnorm_fp8_kernel<T, V><<<(unsigned)M, threads, 0, st>>>((const T *)x, (const T *)y, w, w_add, eps, (int)d, 1.0f / (float)d, (T *)x_out, (T *)h, q, scale, blocks)
-    if (vec == 1) SB_NORM(1);
-    else if (vec == 2) SB_NORM(2);
-    else if (vec == 4) SB_NORM(4);
-    else SB_NORM(8);
+    launch_after(rmsnorm_fp8_kernel<T, V>, dim3((unsigned)M), dim3(threads), 0, st, 1, (const T *)x, (const T *)y, w, w_add, eps, (int)d, 1.0f / (float)d, \
+                 (T *)x_out, (T *)h, q, scale, blocks)
+    return vec == 1 ? SB_NORM(1) : vec == 2 ? SB_NORM(2) : vec == 4 ? SB_NORM(4) : SB_NORM(8);
 #undef SB_NORM
 }
 
@@ -118,6 +118,8 @@ struct RowOf {
 
 template <typename T>
 __global__ void __launch_bounds__(256, 6) swiglu_fp8_kernel(const T *gu, uint8_t *q, float *scale, int64_t rows, int I, int blocks, RowOf row_of) {
+    let_next_begin();
+    wait_for_previous();
     const int64_t units = rows * blocks, stride = (int64_t)gridDim.x * (blockDim.x / 16);
     const int t = threadIdx.x & 15;
     for (int64_t u0 = (int64_t)blockIdx.x * (blockDim.x / 16); u0 < units; u0 += stride) {
@@ -178,9 +180,9 @@ int strix_residual_rmsnorm_fp8(const void *x, const void *y, const float *w, int
     }
     auto st = static_cast<cudaStream_t>(stream);
     const float w_add = centered ? 1.0f : 0.0f;
-    if (act == kF32) launch_norm<float>(x, y, w, w_add, eps, M, d, x_out, h, q, scale, st);
-    else launch_norm<uint16_t>(x, y, w, w_add, eps, M, d, x_out, h, q, scale, st);
-    SB_LAUNCH_OK(fn, " ", act_name(act), " M=", M, " d=", d);
+    SB_CUDA((act == kF32 ? launch_norm<float>(x, y, w, w_add, eps, M, d, x_out, h, q, scale, st)
+                         : launch_norm<uint16_t>(x, y, w, w_add, eps, M, d, x_out, h, q, scale, st)),
+            fn, " ", act_name(act), " M=", M, " d=", d);
     return 0;
 }
 
@@ -205,9 +207,9 @@ int strix_swiglu_fp8(const void *gu, uint8_t *q, float *scale, int64_t rows, int
         row_of.shift = 31 + log;
         row_of.mul = (uint32_t)(((1ull << row_of.shift) + blocks - 1) / blocks);
     }
-    if (act == kF32) swiglu_fp8_kernel<float><<<grid, 256, 0, st>>>((const float *)gu, q, scale, rows, (int)I, blocks, row_of);
-    else swiglu_fp8_kernel<uint16_t><<<grid, 256, 0, st>>>((const uint16_t *)gu, q, scale, rows, (int)I, blocks, row_of);
-    SB_LAUNCH_OK(fn, " ", act_name(act), " rows=", rows, " I=", I);
+    SB_CUDA((act == kF32 ? launch_after(swiglu_fp8_kernel<float>, dim3(grid), dim3(256), 0, st, 1, (const float *)gu, q, scale, rows, (int)I, blocks, row_of)
+                         : launch_after(swiglu_fp8_kernel<uint16_t>, dim3(grid), dim3(256), 0, st, 1, (const uint16_t *)gu, q, scale, rows, (int)I, blocks, row_of)),
+            fn, " ", act_name(act), " rows=", rows, " I=", I);
     return 0;
 }
 

@@ -7,7 +7,7 @@
 // applied inside the accumulation.
 //
 // This file: few rows (decode, verify, a few rows an expert). Weight rows are the M axis of the MMA (128 lanes: one block row of scales) and
-// the rows of x its N axis, up to TOK = 16, 32 or 64 at a time: a few rows cost a narrow instruction, and an expert's ragged slot list is
+// the rows of x its N axis, up to TOK = 16 or 32 at a time: a few rows cost a narrow instruction, and an expert's ragged slot list is
 // padded to 16. fp8_gemm_wide.cu has the form for many rows. What bounds it is the stream of the weights. Warp roles of a CTA:
 //   promotion warps   tcgen05.ld of a finished block accumulator, acc = fma(scale, block, acc); at the end the store of y
 //   TMA warp          weight boxes [128 rows x 128 bytes], 128-byte swizzle, and the box of x rows
@@ -45,9 +45,10 @@ constexpr int kMaxSplit = 4;
 
 template <int TOK>
 struct Cfg {
+    static_assert(TOK <= 32, "a lane of the scale warp per column");
     static constexpr int BTile = TOK * kBK, StageBytes = kATile + BTile;
-    static constexpr int Stages = TOK >= 64 ? 7 : TOK >= 32 ? 9 : 10;
-    static constexpr int NBuf = TOK >= 64 ? 4 : 8;  // accumulators in tensor memory, and slots of scales
+    static constexpr int Stages = TOK >= 32 ? 9 : 10;
+    static constexpr int NBuf = 8;  // accumulators in tensor memory, and slots of scales
     static constexpr int TmemCols = NBuf * TOK;
     static constexpr int RedBytes = TOK * kTileM * 4;  // the columns' parts from the CTAs of a cluster
 };
@@ -95,13 +96,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     float *red = reinterpret_cast<float *>(base + C::Stages * C::StageBytes);
     Ctl<TOK> &ctl = *reinterpret_cast<Ctl<TOK> *>(base + C::Stages * C::StageBytes + C::RedBytes);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    if (warp == kTmaWarp && elect_one()) prefetch_map(&w_map), prefetch_map(&x_map);
-    RouteTables rt{};
-    BucketScan<TOK, kThreads> scan;
-    if constexpr (GROUPED) {
-        rt = route_tables(a.group, a.S, a.E);
-        if (!scan.load(a.group, rt, a.S, a.E, &g_fp8_refusals)) return;  // the whole grid leaves
-    }
+    let_next_begin();
     if (a.split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     const int rank = a.split > 1 ? (int)cluster_rank() : 0;
     const int sh = a.split == 4 ? 2 : a.split == 2 ? 1 : 0;  // split is 1, 2 or 4
@@ -125,12 +120,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     int early = 0;  // dense: blocks of the first pair that are on their way before anything else is set up
     if (warp == kTmaWarp) {
         if (elect_one()) {
+            prefetch_map(&w_map), prefetch_map(&x_map);
             for (int i = 0; i < C::Stages; ++i) mbar_init(&ctl.full[i], 1), mbar_init(&ctl.empty[i], 1);
             for (int i = 0; i < C::NBuf; ++i) mbar_init(&ctl.acc_full[i], 2), mbar_init(&ctl.acc_empty[i], kPromoWarps);
             ctl.abort_flag = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // this thread's copies may signal them at once
             if constexpr (!GROUPED) {
+                wait_for_previous();
                 const int p = first_of(((a.M + TOK - 1) / TOK) * a.NT), xt = p / a.NT;
                 for (int kb = kb0; kb < kb1 && kb - kb0 < C::Stages; ++kb) load(kb - kb0, kb, (p - xt * a.NT) * kTileM, xt * TOK, C::StageBytes);
             }
@@ -141,8 +138,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem_base)), "r"((uint32_t)C::TmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    wait_for_previous();  // nothing in front of this has read or written global memory (but for the early loads, which waited too)
+    RouteTables rt{};
     int x_tiles;
+    bool refused = false;
     if constexpr (GROUPED) {
+        rt = route_tables(a.group, a.S, a.E);
+        BucketScan<TOK, kThreads> scan;
+        refused = !scan.load(a.group, rt, a.S, a.E, &g_fp8_refusals);  // the whole grid: no tiles
         x_tiles = scan.scan(a.E, ctl.buckets, [&](int tiles) { return first_of(tiles * a.NT) / a.NT; });
     } else {
         x_tiles = (a.M + TOK - 1) / TOK;
@@ -152,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     if (a.split > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // the peers run: their shared memory may be written
     const uint32_t tmem = ctl.tmem_base;
-    const int n_pairs = x_tiles * a.NT, p_first = first_of(n_pairs), each = n_pairs / clusters, p_end = p_first + each + (cluster < n_pairs - each * clusters ? 1 : 0);
+    const int n_pairs = refused ? 0 : x_tiles * a.NT, p_first = first_of(n_pairs), each = n_pairs / clusters, p_end = p_first + each + (cluster < n_pairs - each * clusters ? 1 : 0);
 
     Pair t{};  // of this thread's walk; warp-uniform
     int xt = -1, nt = 0;
@@ -252,29 +255,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
     } else if (warp == kScaleWarp) {
-        constexpr int kPerLane = (TOK + 31) / 32;
         uint32_t it = 0;
         bool ok = true;
-        const float *xp[kPerLane];
+        const float *xp = nullptr;  // lane j: the scales of column j's row; null beyond the columns
         for (int p = p_first; p < p_end && ok; ++p) {
-            const bool other = pair_at(p);
+            if (pair_at(p)) xp = lane < t.n ? a.xs + (int64_t)row_of(lane) * a.KB : nullptr;
             // four blocks at a time: a row's four scales share a 32-byte sector, and a round of loads is under way while the round before
             // it is handed over
-            float cur[kPerLane][4], nxt[kPerLane][4];
+            float cur[4], nxt[4];
             const float *wp = a.ws + (int64_t)t.ws_row * a.KB;
-            auto fetch = [&](float(&to)[kPerLane][4], int kb) {
+            auto fetch = [&](float(&to)[4], int kb) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const bool in = kb + q < kb1;
-                    const float w = in ? wp[kb + q] : 0.f;
-#pragma unroll
-                    for (int i = 0; i < kPerLane; ++i) to[i][q] = in && xp[i] != nullptr ? xp[i][kb + q] * w : 0.f;
-                }
+                for (int q = 0; q < 4; ++q) to[q] = kb + q < kb1 && xp != nullptr ? xp[kb + q] * wp[kb + q] : 0.f;
             };
-            if (other) {
-#pragma unroll
-                for (int i = 0; i < kPerLane; ++i) xp[i] = lane + 32 * i < t.n ? a.xs + (int64_t)row_of(lane + 32 * i) * a.KB : nullptr;
-            }
             fetch(cur, kb0);
             for (int kb = kb0; kb < kb1 && ok; kb += 4) {
                 fetch(nxt, kb + 4);
@@ -284,17 +277,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int b = it % C::NBuf;
                     if (it >= C::NBuf) ok = __all_sync(0xffffffffu, mbar_wait(&ctl.acc_empty[b], ((it / C::NBuf) & 1u) ^ 1u, abort_flag));
                     if (!ok) continue;
-#pragma unroll
-                    for (int i = 0; i < kPerLane; ++i)
-                        if (lane + 32 * i < TOK) ctl.scales[b][lane + 32 * i] = cur[i][q];
+                    if (lane < TOK) ctl.scales[b][lane] = cur[q];
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&ctl.acc_full[b]);
                     ++it;
                 }
 #pragma unroll
-                for (int i = 0; i < kPerLane; ++i)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) cur[i][q] = nxt[i][q];
+                for (int q = 0; q < 4; ++q) cur[q] = nxt[q];
             }
         }
     } else if (warp < kPromoWarps) {
@@ -434,16 +423,9 @@ int launch(const char *fn, const uint8_t *w, int64_t w_rows, const uint8_t *x, i
     const int64_t pairs = most_tiles * a.NT, sms = sm_count();
     a.split = 1;
     while (a.split < kMaxSplit && a.split * 2 <= a.KB && pairs * a.split * 2 <= sms) a.split *= 2;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(a.split > 1 ? pairs * a.split : std::min(pairs, sms)));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)a.split, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr, cfg.numAttrs = 1;
-    SB_CUDA((cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<TOK, GROUPED>, wm, xm, a)), fn, " (", TOK, " columns, split ", a.split, ") N=", a.N, " K=", K);
+    const dim3 grid((unsigned)(a.split > 1 ? pairs * a.split : std::min(pairs, sms)));
+    SB_CUDA((launch_after(fp8_gemm_kernel<TOK, GROUPED>, grid, dim3(kThreads), smem, st, a.split, wm, xm, a)), fn, " (", TOK, " columns, split ", a.split,
+            ") N=", a.N, " K=", K);
     return 0;
 }
 
@@ -481,12 +463,12 @@ int grouped(const char *fn, const uint8_t *xq, const float *xs, const strix_fp8v
     a.xs = xs, a.ws = w->scale, a.group = static_cast<const int32_t *>(ws), a.y = y, a.out_f32 = out_act == kF32;
     a.M = (int)M, a.N = (int)N, a.KB = (int)fp8_blocks(w->K), a.NB = (int)fp8_blocks(N), a.E = (int)E, a.div = (int)(rows == S ? 1 : A), a.S = S;
     a.NT = (int)((N + kTileM - 1) / kTileM);
-    const int64_t mean = (S + E - 1) / E;
-    auto tiles = [&](int64_t tok) { return std::min(S, E + S / tok); };  // at most: every bucket may end in a partial tile
-    SB_CHECK(tiles(16) <= 0x7fffffff / a.NT, fn, ": ", S, " slots of N = ", N, " outputs are too many tiles");
-    if (mean <= 8) return launch<16, true>(fn, w->q, w->N, xq, rows, w->K, a, tiles(16), st);
-    if (mean <= 16) return launch<32, true>(fn, w->q, w->N, xq, rows, w->K, a, tiles(32), st);
-    if (mean <= 40) return launch<64, true>(fn, w->q, w->N, xq, rows, w->K, a, tiles(64), st);
+    // Below 8 slots an expert on average the narrow form, from there on the wide one. Measured (gate/up [1024, 2048] of 64 / 256 experts, us, narrow
+    // and wide): mean 4: 22 and 29 / 75 and 83; mean 8: 26 and 31 / 99 and 89; mean 16: 33 and 33 / 142 and 101. Tiles of 32 or 64 slots in the narrow
+    // form were never the fastest.
+    const int64_t tiles = std::min(S, E + S / 16);  // at most: every bucket may end in a partial tile
+    SB_CHECK(tiles <= 0x7fffffff / a.NT, fn, ": ", S, " slots of N = ", N, " outputs are too many tiles");
+    if (S < 8 * E) return launch<16, true>(fn, w->q, w->N, xq, rows, w->K, a, tiles, st);
     return wide_grouped(fn, w->q, w->N, xq, rows, w->K, a, st);
 }
 
@@ -513,7 +495,6 @@ int strix_linear_fp8(const uint8_t *xq, const float *xs, const strix_fp8view *w,
     const char *fn = "linear_fp8";
     SB_TRY(check_view(fn, w));
     SB_CHECK(M >= 1 && M <= 0x7fffff00, fn, ": M = ", M, " rows, expected 1..2^31-256");
-    SB_TRY(check_rows(fn, xq, xs, M, w->K, y, M * w->N * act_size(out_act), out_act));
     GemmArgs a{};
     a.xs = xs, a.ws = w->scale, a.y = y, a.out_f32 = out_act == kF32;
     a.M = (int)M, a.N = (int)w->N, a.KB = (int)fp8_blocks(w->K), a.NB = (int)fp8_blocks(w->N), a.E = 1, a.div = 1, a.S = M;
@@ -521,9 +502,13 @@ int strix_linear_fp8(const uint8_t *xq, const float *xs, const strix_fp8view *w,
     auto st = static_cast<cudaStream_t>(stream);
     auto tiles = [&](int64_t tok) { return (M + tok - 1) / tok; };
     SB_CHECK(tiles(16) <= 0x7fffffff / a.NT, fn, ": M = ", M, " rows of N = ", w->N, " outputs are too many tiles");
-    if (M <= 16) return launch<16, false>(fn, w->q, w->N, xq, M, w->K, a, tiles(16), st);
-    if (M <= 32) return launch<32, false>(fn, w->q, w->N, xq, M, w->K, a, tiles(32), st);
-    if (M <= 64) return launch<64, false>(fn, w->q, w->N, xq, M, w->K, a, tiles(64), st);
+    SB_TRY(check_rows(fn, xq, xs, M, w->K, y, M * w->N * act_size(out_act), out_act));
+    // Tiles of 16 rows while K can be split four ways over the SMs, of 32 while there is an SM for each, else the wide form. Measured
+    // ([N, K], M: us with 16 / 32 / wide): [1024, 2048], 64: 5.2 / 5.5 / 11.7, 128: 6.8 / 5.8 / 12.1, 512: 12.9 / 10.3 / 12.5, 1024: 20.9 / 15.9 / 12.7;
+    // [4096, 4096], 16: 7.7 / 8.1 / 18.0, 32: 9.6 / 8.9 / 18.5, 128: 20.7 / 14.3 / 19.9, 192: 28.5 / 23.2 / 19.8.
+    const int64_t sms = sm_count();
+    if (tiles(16) * a.NT * 4 <= sms) return launch<16, false>(fn, w->q, w->N, xq, M, w->K, a, tiles(16), st);
+    if (tiles(32) * a.NT <= sms) return launch<32, false>(fn, w->q, w->N, xq, M, w->K, a, tiles(32), st);
     return wide_dense(fn, w->q, w->N, xq, M, w->K, a, st);
 }
 
@@ -548,7 +533,7 @@ int strix_linear_fp8_experts_combine_grouped(const uint8_t *hq, const float *hs,
              ": y overlaps the rows or their scales");
     auto st = static_cast<cudaStream_t>(stream);
     SB_TRY(grouped(fn, hq, hs, w, E, ws, ws_bytes, M, A, M * A, partial, kF32, st));
-    return sb::combine_reduce(fn, partial, ids, coef, M, A, E, N, y, act, st);
+    return sb::combine_reduce(fn, partial, ids, coef, M, A, E, N, y, act, st, nullptr, false, true);
 }
 
 }  // extern "C"

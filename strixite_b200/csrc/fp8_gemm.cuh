@@ -1,4 +1,4 @@
-// Shared by the two forms of the FP8 products: narrow (fp8_gemm.cu: weight rows on the accumulator's lanes, up to 64 rows of x as its
+// Shared by the two forms of the FP8 products: narrow (fp8_gemm.cu: weight rows on the accumulator's lanes, up to 32 rows of x as its
 // columns - decode, few rows an expert) and wide (fp8_gemm_wide.cu: rows of x on the lanes, 256 weight rows as columns).
 #pragma once
 

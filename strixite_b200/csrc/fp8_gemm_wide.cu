@@ -120,13 +120,8 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
     uint8_t *strips = base + C::Stages * C::StageBytes;
     Ctl<GROUP> &ctl = *reinterpret_cast<Ctl<GROUP> *>(strips + kPromoWarps * kStrip);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    let_next_begin();
     if (warp == kTmaWarp && elect_one()) prefetch_map(&w_map), prefetch_map(&x_map);
-    RouteTables rt{};
-    BucketScan<kRows, kThreads<GROUPED>> scan;
-    if constexpr (GROUPED) {
-        rt = route_tables(a.group, a.S, a.E);
-        if (!scan.load(a.group, rt, a.S, a.E, &g_wide_refusals)) return;  // the whole grid leaves
-    }
     const uint32_t rank = GROUP == 2 ? cluster_rank() : 0;
     if (tid == 0) {
         for (int i = 0; i < C::Stages; ++i) mbar_init(&ctl.full[i], 1), mbar_init(&ctl.empty[i], 2);  // empty: both halves' MMAs
@@ -143,8 +138,14 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
         }
     }
+    wait_for_previous();  // nothing in front of this has read or written global memory
+    RouteTables rt{};
     int x_tiles;
+    bool refused = false;
     if constexpr (GROUPED) {
+        rt = route_tables(a.group, a.S, a.E);
+        BucketScan<kRows, kThreads<GROUPED>> scan;
+        refused = !scan.load(a.group, rt, a.S, a.E, &g_wide_refusals);  // the whole grid: no tiles
         x_tiles = scan.scan(a.E, ctl.buckets, [&](int) { return (int)blockIdx.x / a.NT; });
     } else {
         x_tiles = (a.M + kRows * GROUP - 1) / (kRows * GROUP);
@@ -155,7 +156,7 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
     tc_fence_after();
     const uint32_t tmem = ctl.tmem_base;
     volatile int *abort_flag = &ctl.abort_flag;
-    const int n_tiles = x_tiles * a.NT, step = gridDim.x / GROUP;
+    const int n_tiles = refused ? 0 : x_tiles * a.NT, step = gridDim.x / GROUP;
 
     auto tile_of = [&](int p) {  // warp-uniform
         const int xt = p / a.NT, nt = p - xt * a.NT;
@@ -436,16 +437,8 @@ int launch(const char *fn, const uint8_t *w, int64_t w_rows, const uint8_t *x, i
     SB_TRY(make_map(fn, &xm, x, x_rows, K, GROUPED ? 1 : kRows));
     a.NT = (a.N + kColTile - 1) / kColTile;
     const int64_t all = tiles * a.NT, room = sm_count() / GROUP;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(std::min(all, room) * GROUP));
-    cfg.blockDim = dim3(kThreads<GROUPED>);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = GROUP, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr, cfg.numAttrs = 1;
-    SB_CUDA((cudaLaunchKernelEx(&cfg, fp8_wide_kernel<GROUP, GROUPED>, wm, xm, a)), fn, " (wide) N=", a.N, " K=", K);
+    SB_CUDA((launch_after(fp8_wide_kernel<GROUP, GROUPED>, dim3((unsigned)(std::min(all, room) * GROUP)), dim3(kThreads<GROUPED>), smem, st, GROUP, wm, xm, a)), fn,
+            " (wide) N=", a.N, " K=", K);
     return 0;
 }
 

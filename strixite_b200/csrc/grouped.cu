@@ -108,6 +108,7 @@ template <bool CLUSTER>
 __global__ void __launch_bounds__(kRouteThreads)
     route_kernel(const int32_t *ids, int S, int E, int Tmax, int WTmax, int32_t *ws, uint32_t *err) {
     extern __shared__ int smem[];
+    let_next_begin();
     const int B = E + 1;
     int *cnt = smem;                      // [kRouteWarps][B]
     int *start = cnt + kRouteWarps * B;   // [B + 1] first slot position of each bucket
@@ -124,6 +125,7 @@ __global__ void __launch_bounds__(kRouteThreads)
     for (int i = t; i < live_warps * B; i += kRouteThreads) cnt[i] = 0;
     if (t == 0) first_bad = 0x7fffffff;
     __syncthreads();
+    wait_for_previous();
     for (int s0 = s_begin + lane; s0 < s_end; s0 += 128) {  // four ids in flight
         int32_t id[4];
 #pragma unroll
@@ -388,6 +390,7 @@ template <typename T>
 __global__ void __launch_bounds__(256)
     combine_reduce_kernel(const float *partial, const int32_t *ids, const float *coef, int64_t M, int64_t A, int64_t E,
                           int64_t N, T *y) {
+    wait_for_previous();
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= M * N) return;
     const int64_t m = i / N, n = i - m * N;
@@ -419,6 +422,7 @@ template <typename T, bool H>
 __global__ void __launch_bounds__(256)
     combine_reduce4_kernel(const void *partial, const int64_t *pos, const int32_t *ids, const float *coef, int64_t M, int64_t A, int64_t E,
                            int64_t N, T *y) {
+    wait_for_previous();
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, N4 = N / 4;
     if (i >= M * N4) return;
     const int64_t m = i / N4, n = (i - m * N4) * 4;
@@ -555,9 +559,16 @@ int combine_grouped(const char *fn, const void *h, const StackView &w, int64_t E
 }
 
 int combine_reduce(const char *fn, const void *partial, const int32_t *ids, const float *coef, int64_t M, int64_t A, int64_t E, int64_t N,
-                   void *y, int act, cudaStream_t st, const int64_t *pos, bool half_partial) {
+                   void *y, int act, cudaStream_t st, const int64_t *pos, bool half_partial, bool early) {
     const bool vec = N % 4 == 0 && reinterpret_cast<uintptr_t>(partial) % 16 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
     SB_CHECK((pos == nullptr && !half_partial) || vec, fn, ": the indexed combine and F16 partial sums need N % 4 == 0 and 16-byte aligned buffers");
+    if (early && vec && !half_partial) {
+        const dim3 blocks((unsigned)((M * (N / 4) + 255) / 256));
+        SB_CUDA((act == kF32 ? launch_after(combine_reduce4_kernel<float, false>, blocks, dim3(256), 0, st, 1, partial, pos, ids, coef, M, A, E, N, (float *)y)
+                             : launch_after(combine_reduce4_kernel<uint16_t, false>, blocks, dim3(256), 0, st, 1, partial, pos, ids, coef, M, A, E, N, (uint16_t *)y)),
+                fn, " reduce ", act_name(act), " M=", M, " A=", A, " N=", N);
+        return 0;
+    }
     if (vec) {
         const unsigned blocks = (unsigned)((M * (N / 4) + 255) / 256);
         if (half_partial) {
@@ -658,18 +669,10 @@ int strix_moe_group_routes(const int32_t *ids, int64_t M, int64_t A, int64_t E, 
     auto st = static_cast<cudaStream_t>(stream);
     auto *wi = static_cast<int32_t *>(ws);
     const int Tmax = (int)(S / 16 + E + 2), WTmax = (int)(S / 64 + E + 2);
-    if (S < kRouteClusterSlots) {
-        route_kernel<false><<<1, kRouteThreads, smem, st>>>(ids, (int)S, (int)E, Tmax, WTmax, wi, err);
-    } else {
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(kRouteBlocks), cfg.blockDim = dim3(kRouteThreads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = kRouteBlocks, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
-        cfg.attrs = attr, cfg.numAttrs = 1;
-        SB_CUDA(cudaLaunchKernelEx(&cfg, route_kernel<true>, ids, (int)S, (int)E, Tmax, WTmax, wi, err), fn, " M=", M, " A=", A, " E=", E);
-    }
-    SB_LAUNCH_OK(fn, " M=", M, " A=", A, " E=", E);
+    SB_CUDA((S < kRouteClusterSlots
+                 ? launch_after(route_kernel<false>, dim3(1), dim3(kRouteThreads), smem, st, 1, ids, (int)S, (int)E, Tmax, WTmax, wi, err)
+                 : launch_after(route_kernel<true>, dim3(kRouteBlocks), dim3(kRouteThreads), smem, st, kRouteBlocks, ids, (int)S, (int)E, Tmax, WTmax, wi, err)),
+            fn, " M=", M, " A=", A, " E=", E);
     return 0;
 }
 

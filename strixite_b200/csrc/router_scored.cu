@@ -184,6 +184,8 @@ __global__ void __launch_bounds__(kWarps * 32) router_scored_kernel(const T *log
     const unsigned full = 0xffffffffu;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t m = (int64_t)blockIdx.x * kWarps + warp;
+    let_next_begin();
+    wait_for_previous();
     if (m >= a.M) return;  // whole warps leave together; no block-level barrier below
     const int L = a.L, g = lane / L, sub = lane % L;
     const T *row = logits + m * a.ld;
@@ -433,15 +435,11 @@ __global__ void __launch_bounds__(kWarps * 32) router_scored_kernel(const T *log
 }
 
 template <typename T, bool VEC>
-void launch(const void *logits, const void *shared, const RouteArgs &a, cudaStream_t st) {
+cudaError_t launch(const void *logits, const void *shared, const RouteArgs &a, cudaStream_t st) {
     const int nv = (a.per + a.L - 1) / a.L;
     const unsigned blocks = (unsigned)((a.M + kWarps - 1) / kWarps);
-#define SB_ROUTE(NV) router_scored_kernel<T, NV, VEC><<<blocks, kWarps * 32, 0, st>>>((const T *)logits, (const T *)shared, a)
-    if (nv <= 4) SB_ROUTE(4);
-    else if (nv <= 8) SB_ROUTE(8);
-    else if (nv <= 16) SB_ROUTE(16);
-    else if (nv <= 32) SB_ROUTE(32);
-    else SB_ROUTE(64);
+#define SB_ROUTE(NV) launch_after(router_scored_kernel<T, NV, VEC>, dim3(blocks), dim3(kWarps * 32), 0, st, 1, (const T *)logits, (const T *)shared, a)
+    return nv <= 4 ? SB_ROUTE(4) : nv <= 8 ? SB_ROUTE(8) : nv <= 16 ? SB_ROUTE(16) : nv <= 32 ? SB_ROUTE(32) : SB_ROUTE(64);
 #undef SB_ROUTE
 }
 
@@ -485,11 +483,9 @@ int strix_moe_router_scored(const void *logits, int64_t ld, int64_t M, int64_t E
     // runs of four where they fill the lanes of a group evenly and every row starts aligned
     const bool vec = a.per % (4 * a.L) == 0 && ld % 4 == 0 && reinterpret_cast<uintptr_t>(logits) % (4 * act_size(act)) == 0 && aligned16(bias);
     auto st = static_cast<cudaStream_t>(stream);
-    if (act == kF32 && vec) launch<float, true>(logits, shared_logit, a, st);
-    else if (act == kF32) launch<float, false>(logits, shared_logit, a, st);
-    else if (vec) launch<uint16_t, true>(logits, shared_logit, a, st);
-    else launch<uint16_t, false>(logits, shared_logit, a, st);
-    SB_LAUNCH_OK(fn, " ", act_name(act), " M=", M, " E=", E, " k=", k, " groups=", n_group);
+    const cudaError_t rc = act == kF32 ? (vec ? launch<float, true>(logits, shared_logit, a, st) : launch<float, false>(logits, shared_logit, a, st))
+                                       : (vec ? launch<uint16_t, true>(logits, shared_logit, a, st) : launch<uint16_t, false>(logits, shared_logit, a, st));
+    SB_CUDA(rc, fn, " ", act_name(act), " M=", M, " E=", E, " k=", k, " groups=", n_group);
     return 0;
 }
 
