@@ -440,9 +440,9 @@ int check_view(const char *fn, const strix_fp8view *w) {
 
 int check_rows(const char *fn, const uint8_t *xq, const float *xs, int64_t rows, int64_t K, const void *y, int64_t y_bytes, int out_act) {
     SB_CHECK(xq != nullptr && xs != nullptr && y != nullptr, fn, ": null pointer (xq=", (const void *)xq, ", xs=", (const void *)xs, ", y=", y, ")");
-    SB_CHECK(aligned16(xq) && reinterpret_cast<uintptr_t>(xs) % 4 == 0 && reinterpret_cast<uintptr_t>(y) % 4 == 0, fn, ": xq ", (const void *)xq,
-             " must be 16-byte aligned, xs and y 4-byte");
     SB_CHECK(act_ok(out_act), fn, ": unsupported output dtype ", out_act);
+    SB_CHECK(aligned16(xq) && reinterpret_cast<uintptr_t>(xs) % 4 == 0 && reinterpret_cast<uintptr_t>(y) % act_size(out_act) == 0, fn, ": xq ", (const void *)xq,
+             " must be 16-byte aligned, xs 4-byte, y ", y, " aligned to its elements");
     SB_CHECK(apart(y, y_bytes, xq, rows * K) && apart(y, y_bytes, xs, rows * fp8_blocks(K) * 4), fn, ": output [", y, ", +", y_bytes,
              " B) overlaps the rows [", (const void *)xq, "] or their scales [", (const void *)xs, "]");
     return 0;

@@ -448,7 +448,7 @@ namespace sb {
 namespace fp8 {
 
 int wide_dense(const char *fn, const uint8_t *w, int64_t w_rows, const uint8_t *x, int64_t x_rows, int64_t K, const GemmArgs &a, cudaStream_t st) {
-    return launch<2, false>(fn, w, w_rows, x, x_rows, K, a, (a.M + 2 * kRows - 1) / (2 * kRows), st);
+    return launch<2, false>(fn, w, w_rows, x, x_rows, K, a, ((int64_t)a.M + 2 * kRows - 1) / (2 * kRows), st);
 }
 
 int wide_grouped(const char *fn, const uint8_t *w, int64_t w_rows, const uint8_t *x, int64_t x_rows, int64_t K, const GemmArgs &a, cudaStream_t st) {

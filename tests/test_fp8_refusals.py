@@ -103,6 +103,7 @@ def test_linear(mem):
     refused(call(q=C.c_void_p(mem(2).value + 8)), "aligned")
     refused(call(xq=C.c_void_p(mem(0).value + 8)), "aligned")
     refused(call(y=C.c_void_p(mem(4).value + 2)), "aligned")
+    refused(call(y=C.c_void_p(mem(4).value + 1), act=1), "aligned")
     refused(call(act=2), "dtype 2")
     refused(call(y=mem(0)), "overlaps")
     refused(call(y=mem(1)), "overlaps")

@@ -111,6 +111,29 @@ def test_route_extremes_shared_slot_and_failed_tokens():
     assert (ids == -1).all() and coef.isnan().all() and host_err(err)[2] == 3
 
 
+def test_route_hundreds_of_candidates_and_odd_views():
+    """Equal logits: every expert is a candidate and the lowest indices win. Logits that start and are spaced so that no vector load is
+    aligned give the same as a copy."""
+    for E, G, tg, k in ((1024, 1, 1, 32), (768, 3, 2, 20), (1023, 1, 1, 5)):
+        for score in ("softmax", "sigmoid"):
+            logits, bias = torch.full((5, E), 0.25, device="cuda"), torch.full((E,), 0.5, device="cuda")
+            for b in (None, bias):
+                ids, coef, _ = run_route(logits, k, score, b, G, tg, 2, True, 1.0, K.Act.F32)
+                assert torch.equal(ids.cpu(), torch.arange(k, dtype=torch.int32).expand(5, k)) and (coef - 1 / k).abs().max() < 1e-6 / k
+    g = gen(9)
+    wide = (rand(g, 33, 261) * 1.5).bfloat16()
+    bias = rand(g, 257)[1:] * 0.05  # 4 bytes past an aligned address
+    for act, base in ((K.Act.BF16, wide), (K.Act.F32, wide.float())):
+        view = base[:, 3:]  # 256 experts used, rows 261 apart
+        ids = torch.empty((33, 8), dtype=torch.int32, device="cuda")
+        coef, err = torch.empty((33, 8), device="cuda"), K.new_err()
+        K.moe_router_scored(view, 261, 33, 256, 8, "sigmoid", bias, 8, 4, 2, True, 2.5, None, 0, 0, ids, coef, act, err)
+        want, cw = route(base[:, 3:259].float(), 8, "sigmoid", bias, 8, 4, 2, True, 2.5)
+        assert torch.equal(ids.cpu(), want) and ((coef.cpu().double() - cw).abs() <= cw * 44 * 2.0**-24).all()
+        with pytest.raises(StrixError, match="ends before"):
+            K.moe_router_scored(base[1:, 3:], 261, 33, 256, 8, "sigmoid", bias, 8, 4, 2, True, 2.5, None, 0, 0, ids, coef, act, err)
+
+
 # ---- norm and SwiGLU -------------------------------------------------------------------------------------------------
 
 
@@ -225,6 +248,49 @@ def test_linear_fp8_nan_and_zero_rows_stay_apart():
     keep = torch.ones(N, dtype=torch.bool, device="cuda")
     keep[130] = False
     assert (y[5][keep] == 0).all()
+
+
+def test_rows_and_outputs_past_32_bit_offsets():
+    """More than 2^31 elements: the last rows are where they belong."""
+    g = gen(11)
+    M, d = 1100000, 2048
+    x = torch.zeros((M, d), dtype=torch.bfloat16, device="cuda")
+    x[0], x[-1] = rand(g, d), rand(g, d)
+    q, s, w = torch.empty((M, d), dtype=FP8, device="cuda"), torch.empty((M, 16), device="cuda"), torch.ones(d, device="cuda")
+    K.residual_rmsnorm_fp8(x, None, w, M, d, 1e-5, None, None, q, s, K.Act.BF16)
+    for r in (0, M - 1):
+        f = x[r : r + 1].double()
+        check_fp8_rows(q[r : r + 1], s[r : r + 1], f / torch.sqrt(f.pow(2).mean(1, keepdim=True) + 1e-5), 45 * 2.0**-24)
+    assert (q[M // 2].float() == 0).all()
+    gu = x.view(M // 2, 2 * d)  # the same elements as merged rows of I = d
+    q2, s2 = q.view(torch.uint8).view(-1)[: M // 2 * d].view(FP8).view(M // 2, d), s[: M // 2]
+    K.swiglu_fp8(gu, q2, s2, M // 2, d, K.Act.BF16)
+    last = gu[-1:].double()
+    check_fp8_rows(q2[-1:], s2[-1:], last[:, :d] * torch.sigmoid(last[:, :d]) * last[:, d:], 8 * 2.0**-24)
+    del x, gu, q, q2, s, s2
+    M, N, Kd = 66000, 33000, 128
+    xq, xs = rows_fp8(rand(g, M, Kd))
+    wq, ws = matrix_fp8(rand(g, N, Kd))
+    y = torch.empty((M, N), dtype=torch.bfloat16, device="cuda")
+    K.linear_fp8(xq, xs, K.Fp8Weight(wq, ws), y, M, K.Act.BF16)
+    for r in (0, 65070, M - 1):  # 65076 rows hold 2^31 elements
+        a, b = wide_rows(xq[r : r + 1], xs[r : r + 1]), wide_matrix(wq, ws)
+        y64 = a @ b.t()
+        assert ((y[r : r + 1].double() - y64).abs() <= product_bound(a.abs(), b.abs(), Kd, y64, True)).all()
+
+
+def test_linear_fp8_output_at_any_element():
+    g = gen(12)
+    for M, N, Kd in ((5, 130, 256), (600, 136, 384)):  # narrow and wide form, stores that are not aligned to vectors
+        xq, xs = rows_fp8(rand(g, M, Kd))
+        W = K.Fp8Weight(*matrix_fp8(rand(g, N, Kd)))
+        for act in ACTS:
+            want = torch.empty((M, N), dtype=DT[act], device="cuda")
+            K.linear_fp8(xq, xs, W, want, M, act)
+            room = torch.full((M * N + 9,), 3.0, dtype=DT[act], device="cuda")
+            y = room[1 : 1 + M * N].view(M, N)
+            K.linear_fp8(xq, xs, W, y, M, act)
+            assert torch.equal(y, want) and room[0] == 3.0 and (room[1 + M * N :] == 3.0).all()
 
 
 # ---- the experts' products -------------------------------------------------------------------------------------------
