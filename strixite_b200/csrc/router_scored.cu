@@ -339,9 +339,32 @@ __global__ void __launch_bounds__(kWarps * 32) router_scored_kernel(const T *log
             kth_key = __reduce_max_sync(full, key);
             if (key == kth_key) key = 0;  // equal maxima go together: the bound is only lower
         }
-        const float kth = kth_key == 0 ? -INFINITY : key_value(kth_key);
+        float kth = kth_key == 0 ? -INFINITY : key_value(kth_key);
+        if (kth == -INFINITY && a.topk_group * a.per > 96) {
+            // Fewer lanes than k are open, and they hold many experts: the k-th largest value itself, by k rounds in which the lane that
+            // holds the largest drops it (16384 tokens, 16 of 256 open experts: 857 -> 185 us; of 63: 131 -> 216, so there all are candidates)
+            uint64_t gone = 0;
+            float best = lm;
+#pragma unroll 1
+            for (int r = 0; r < a.k; ++r) {
+                const uint32_t own = order_key(best);
+                kth_key = __reduce_max_sync(full, own);
+                if (own == kth_key) {
+                    float next = -INFINITY;
+                    bool dropped = false;
+#pragma unroll
+                    for (int j = 0; j < NV; ++j) {
+                        if (gone >> j & 1) continue;
+                        if (!dropped && c[j] == best) gone |= 1ull << j, dropped = true;
+                        else next = fmaxf(next, c[j]);
+                    }
+                    best = next;
+                }
+            }
+            kth = key_value(kth_key);
+        }
         // what lies below the k-th by no more than the error is a candidate too: nothing that is left out can belong to the picks.
-        // -FLT_MAX: every finite value where fewer than k lanes are open.
+        // -FLT_MAX: every finite value.
         const float bound = fmaxf(biased ? kth - (base + 0x1p-21f * fabsf(kth)) : kth, -FLT_MAX);
         int mine = 0;
 #pragma unroll
