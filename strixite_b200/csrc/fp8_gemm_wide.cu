@@ -361,26 +361,33 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
             fetch(p + step);
             // y: 64 bytes of every row at a time through the strip; then 4 lanes write a row's 64 bytes, 8 rows an instruction
             const int es = a.out_f32 ? 4 : 2;
-            const bool wide = ((int64_t)a.N * es) % 16 == 0 && reinterpret_cast<uintptr_t>(a.y) % 16 == 0;
+            const uint64_t at = reinterpret_cast<uint64_t>(a.y) | (uint64_t)a.N * es;  // what every row's start is a multiple of
+            const int unit = at % 16 == 0 ? 16 : at % 4 == 0 ? 4 : 2;
             auto flush = [&](int col) {  // the strip's 64 / es columns from col on
                 __syncwarp();
+                if (unit == 16) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int rr = i * 8 + (lane >> 2), n = n_base + col + (lane & 3) * (16 / es);
-                    const int64_t orow = __shfl_sync(0xffffffffu, out_row, rr);
-                    const bool live = (warp & 3) * 32 + rr < n_rows;
-                    const uint4 q = *reinterpret_cast<const uint4 *>(strip + rr * kStripPitch + (lane & 3) * 16);
-                    uint8_t *dst = static_cast<uint8_t *>(a.y) + (orow * a.N + n) * es;
-                    if (!live) continue;
-                    if (wide) {
-                        if (n < a.N) *reinterpret_cast<uint4 *>(dst) = q;
-                    } else {
-                        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-                        for (int e = 0; e < 16 / es; ++e) {
-                            if (n + e >= a.N) break;
-                            if (es == 4) reinterpret_cast<uint32_t *>(dst)[e] = w[e];
-                            else reinterpret_cast<uint16_t *>(dst)[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        const int rr = i * 8 + (lane >> 2), n = n_base + col + (lane & 3) * (16 / es);
+                        const int64_t orow = __shfl_sync(0xffffffffu, out_row, rr);
+                        const bool live = (warp & 3) * 32 + rr < n_rows;
+                        const uint4 q = *reinterpret_cast<const uint4 *>(strip + rr * kStripPitch + (lane & 3) * 16);
+                        uint8_t *dst = static_cast<uint8_t *>(a.y) + (orow * a.N + n) * es;
+                        if (live && n < a.N) *reinterpret_cast<uint4 *>(dst) = q;
+                    }
+                } else {
+                    // rows that start anywhere: neighbouring lanes write neighbouring words (16 a row, two rows an instruction) or halves.
+                    // 2293 x 656 against 2112 (vectors), 2116 (words), 2115 (halves) rows: 13.2, 18.5, 26.5 us; each lane its own row: 43 us.
+                    const int per = 64 / unit, mine = lane & (per - 1), n = n_base + col + mine * unit / es;
+#pragma unroll 8
+                    for (int i = 0; i < per; ++i) {
+                        const int rr = unit == 4 ? i * 2 + (lane >> 4) : i;
+                        const int64_t orow = __shfl_sync(0xffffffffu, out_row, rr);
+                        if ((warp & 3) * 32 + rr >= n_rows || n >= a.N) continue;
+                        uint8_t *dst = static_cast<uint8_t *>(a.y) + (orow * a.N + n) * es;
+                        const uint8_t *src = strip + rr * kStripPitch + mine * unit;
+                        if (unit == 4) *reinterpret_cast<uint32_t *>(dst) = *reinterpret_cast<const uint32_t *>(src);
+                        else *reinterpret_cast<uint16_t *>(dst) = *reinterpret_cast<const uint16_t *>(src);
                     }
                 }
                 __syncwarp();

@@ -461,8 +461,16 @@ template <typename T, bool VEC>
 cudaError_t launch(const void *logits, const void *shared, const RouteArgs &a, cudaStream_t st) {
     const int nv = (a.per + a.L - 1) / a.L;
     const unsigned blocks = (unsigned)((a.M + kWarps - 1) / kWarps);
+    // a lane's scores stay in NV registers: the steps between powers of two pay (13665 tokens, 524 experts, nv = 17: 38.7 us with
+    // 24, 44.6 with 32)
 #define SB_ROUTE(NV) launch_after(router_scored_kernel<T, NV, VEC>, dim3(blocks), dim3(kWarps * 32), 0, st, 1, (const T *)logits, (const T *)shared, a)
-    return nv <= 4 ? SB_ROUTE(4) : nv <= 8 ? SB_ROUTE(8) : nv <= 16 ? SB_ROUTE(16) : nv <= 32 ? SB_ROUTE(32) : SB_ROUTE(64);
+    return nv <= 4    ? SB_ROUTE(4)
+           : nv <= 8  ? SB_ROUTE(8)
+           : nv <= 12 ? SB_ROUTE(12)
+           : nv <= 16 ? SB_ROUTE(16)
+           : nv <= 24 ? SB_ROUTE(24)
+           : nv <= 32 ? SB_ROUTE(32)
+                      : SB_ROUTE(64);
 #undef SB_ROUTE
 }
 
