@@ -26,9 +26,6 @@ __device__ __forceinline__ float max_abs8(const float (&v)[8]) {
     return max_abs(max_abs(v[0], v[1], v[2]), max_abs(v[3], v[4], v[5]), max_abs(v[6], v[7]));
 }
 
-// The scale of a block is its largest magnitude / 448 (the largest e4m3 value stands for it), at least 2^-100 / 448: a block of zeros has
-// a scale that divides. A NaN stays one.
-
 // Two values in e4m3, round to nearest even, saturating at +-448 (NaN -> the NaN code); `lo` in the low byte.
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     uint16_t r;
@@ -49,8 +46,8 @@ struct Block8 {
     float hi[8], lo[8];
 };
 
-// The 8 values (times `unit`, a factor that the block shares) as e4m3 bytes of v / scale, scale = max(amax * unit, 2^-100) / 448. The quotient
-// is taken against the unrounded block maximum, in which the unit cancels: 448 / amax as two floats, three FMAs a value.
+// The 8 values (times `unit`, a factor that the block shares) as e4m3 bytes of v / scale, scale = max(amax * unit, 2^-100) / 448: the largest
+// magnitude gets the largest e4m3 value, and a block of zeros has a scale that divides. A NaN stays one. The quotient is taken against the unrounded block maximum, in which the unit cancels: 448 / amax as two floats, three FMAs a value.
 __device__ __forceinline__ uint2 fp8_pack8(const Block8 &v, float amax, float unit, float &scale) {
     uint32_t h[4];
     const float top = amax * unit;

@@ -107,8 +107,6 @@ cudaError_t launch_norm(const void *x, const void *y, const float *w, float w_ad
 #undef SB_NORM
 }
 
-// A half warp per (row, 128-column block) of h = silu(gate) * up, 8 elements a thread. Gate and up stay FP32 until the one rounding
-// to e4m3.
 // u / blocks for u < 2^31: (u * mul) >> shift with mul = ceil(2^shift / blocks), shift = 31 + ceil(log2 blocks) (the excess of mul * blocks
 // over 2^shift is below blocks <= 2^(shift - 31), so u times it stays below 2^shift). mul = 0: by division.
 struct RowOf {
@@ -116,6 +114,8 @@ struct RowOf {
     int shift;
 };
 
+// A half warp per (row, 128-column block) of h = silu(gate) * up, 8 elements a thread. Gate and up stay FP32 until the one rounding
+// to e4m3.
 template <typename T>
 __global__ void __launch_bounds__(256, 6) swiglu_fp8_kernel(const T *gu, uint8_t *q, float *scale, int64_t rows, int I, int blocks, RowOf row_of) {
     let_next_begin();

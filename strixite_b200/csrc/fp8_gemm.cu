@@ -68,6 +68,7 @@ template <int TOK>
 constexpr size_t smem_bytes() {
     return (size_t)Cfg<TOK>::Stages * Cfg<TOK>::StageBytes + Cfg<TOK>::RedBytes + sizeof(Ctl<TOK>) + 1024;
 }
+static_assert(smem_bytes<16>() > kOnePerSm && smem_bytes<32>() > kOnePerSm);
 
 __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -521,9 +522,12 @@ int strix_linear_fp8_experts_combine_grouped(const uint8_t *hq, const float *hs,
                                              const void *ws, size_t ws_bytes, float *partial, int64_t M, int64_t A, void *y, int act, void *stream) {
     const char *fn = "linear_fp8_experts_combine_grouped";
     SB_CHECK(ids != nullptr && coef != nullptr && y != nullptr, fn, ": null pointer (ids=", (const void *)ids, ", coef=", (const void *)coef, ", y=", y, ")");
+    SB_CHECK(reinterpret_cast<uintptr_t>(ids) % 4 == 0 && reinterpret_cast<uintptr_t>(coef) % 4 == 0, fn, ": ids ", (const void *)ids, " and coef ",
+             (const void *)coef, " must be 4-byte aligned");
     SB_CHECK(act_ok(act), fn, ": unsupported activation dtype ", act);
     SB_CHECK(M >= 1 && A >= 1 && A <= 64 && M <= (1 << 20) && M * A <= (1 << 20), fn, ": M = ", M, ", A = ", A, " (A <= 64, M * A <= 2^20)");
-    SB_CHECK(w != nullptr && E >= 1 && E <= kMaxE && w->N >= 1 && w->N % E == 0, fn, ": null weight view, or its rows are not those of E = ", E, " experts (1..1023)");
+    SB_TRY(check_view(fn, w));
+    SB_CHECK(E >= 1 && E <= kMaxE && w->N % E == 0, fn, ": weight has ", w->N, " rows for E = ", E, " experts (E must be 1..1023 and divide the rows)");
     const int64_t N = w->N / E, yb = M * N * act_size(act), pb = M * A * N * 4;
     SB_CHECK(partial != nullptr && apart(y, yb, partial, pb), fn, ": null partial, or it overlaps y");
     SB_CHECK(apart(y, yb, ids, M * A * 4) && apart(y, yb, coef, M * A * 4) && apart(partial, pb, ids, M * A * 4) && apart(partial, pb, coef, M * A * 4), fn,

@@ -13,6 +13,9 @@ namespace fp8 {
 
 constexpr int kBK = 128;  // K per stage: one scale block, one 128-byte swizzle row
 constexpr int kMaxE = 1023;
+// More shared memory than this and an SM holds one block of these kernels at a time. That is a condition, not only a consequence: they
+// let the next kernel begin before they have their tensor memory, and a block of that one must not hold it while it waits for them.
+constexpr size_t kOnePerSm = 114 * 1024;
 
 struct GemmArgs {
     const float *xs, *ws;    // scales of x rows [.., KB] and of the weight blocks [(E *) NB, KB]

@@ -58,6 +58,7 @@ template <int GROUP>
 constexpr size_t smem_bytes() {
     return (size_t)Cfg<GROUP>::Stages * Cfg<GROUP>::StageBytes + kPromoWarps * kStrip + sizeof(Ctl<GROUP>) + 1024;
 }
+static_assert(smem_bytes<1>() > kOnePerSm && smem_bytes<2>() > kOnePerSm);
 
 template <int GROUP>
 __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {

@@ -495,6 +495,8 @@ int strix_moe_router_scored(const void *logits, int64_t ld, int64_t M, int64_t E
              " experts in open groups)");
     SB_CHECK(ld >= E, fn, ": logits row stride ld = ", ld, " < E = ", E);
     SB_CHECK(route_scale == route_scale && route_scale - route_scale == 0.0f, fn, ": route_scale = ", route_scale, ", expected a finite number");
+    SB_CHECK(M == 1 || (ld <= (1 << 28) && (shared_logit == nullptr || shared_ld <= (1 << 28))), fn, ": row strides ", ld, " and ", shared_ld,
+             ", expected up to 2^28");
     if (shared_logit != nullptr) {
         SB_CHECK(shared_ld >= 1, fn, ": shared_ld = ", shared_ld, ", expected >= 1");
         SB_CHECK(shared_id >= 0, fn, ": shared_id = ", shared_id, ", expected >= 0 (its expert row block)");
@@ -504,6 +506,9 @@ int strix_moe_router_scored(const void *logits, int64_t ld, int64_t M, int64_t E
     SB_CHECK(apart(ids, ob, coef, ob), fn, ": ids [", (const void *)ids, "] and coef [", (const void *)coef, "] (", ob, " B each) overlap");
     const int64_t lb = ((M - 1) * ld + E) * act_size(act);
     SB_CHECK(apart(ids, ob, logits, lb) && apart(coef, ob, logits, lb), fn, ": ids or coef overlaps the logits [", logits, ", +", lb, " B)");
+    SB_CHECK(bias == nullptr || (apart(ids, ob, bias, E * 4) && apart(coef, ob, bias, E * 4)), fn, ": ids or coef overlaps the bias");
+    const int64_t shb = ((M - 1) * shared_ld + 1) * act_size(act);
+    SB_CHECK(shared_logit == nullptr || (apart(ids, ob, shared_logit, shb) && apart(coef, ob, shared_logit, shb)), fn, ": ids or coef overlaps the shared logits");
     RouteArgs a{};
     a.ld = ld, a.M = M, a.E = (int)E, a.k = (int)k, a.score = score, a.G = (int)n_group, a.topk_group = (int)topk_group, a.group_top = (int)group_top;
     a.renorm = renorm != 0, a.route_scale = route_scale, a.bias = bias, a.shared_ld = shared_ld, a.shared_id = shared_id, a.ids = ids, a.coef = coef;

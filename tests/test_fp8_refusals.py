@@ -21,8 +21,8 @@ def refused(rc, text):
 
 
 def test_router_scored(mem):
-    def call(M=4, E=64, k=8, ld=64, score=1, G=8, tg=4, gt=2, scale=1.0, shared=None, shared_ld=1, shared_id=0, act=0, ids=mem(1), coef=mem(2), logits=mem(0), err=mem(3)):
-        return lib.strix_moe_router_scored(logits, ld, M, E, k, score, None, G, tg, gt, 1, scale, shared, shared_ld, shared_id, ids, coef, act, err, None)
+    def call(M=4, E=64, k=8, ld=64, score=1, G=8, tg=4, gt=2, scale=1.0, shared=None, shared_ld=1, shared_id=0, act=0, ids=mem(1), coef=mem(2), logits=mem(0), err=mem(3), bias=None):
+        return lib.strix_moe_router_scored(logits, ld, M, E, k, score, bias, G, tg, gt, 1, scale, shared, shared_ld, shared_id, ids, coef, act, err, None)
 
     refused(call(logits=None), "null pointer")
     refused(call(err=None), "null pointer")
@@ -46,6 +46,10 @@ def test_router_scored(mem):
     refused(call(shared=mem(4), shared_id=-1), "shared_id")
     refused(call(coef=mem(1)), "overlap")
     refused(call(ids=mem(0)), "overlaps the logits")
+    refused(call(coef=mem(4), bias=mem(4)), "overlaps the bias")
+    refused(call(coef=mem(4), shared=mem(4)), "overlaps the shared logits")
+    refused(call(ld=1 << 40), "row strides")
+    refused(call(shared=mem(4), shared_ld=1 << 40), "row strides")
 
 
 def test_norm(mem):
@@ -145,6 +149,8 @@ def test_experts(mem):
     refused(combine(E=3), "E = 3")
     refused(combine(n=8), "needs %d" % need)
     refused(combine(hq=None), "null pointer")
+    refused(combine(ids=C.c_void_p(mem(6).value + 2)), "4-byte aligned")
+    refused(combine(coef=C.c_void_p(mem(7).value + 2)), "4-byte aligned")
 
 
 def test_weight_object():

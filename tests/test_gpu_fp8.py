@@ -512,6 +512,49 @@ def test_ffn_in_a_graph_on_streams_and_side_by_side():
     assert all(torch.equal(v, bits(f)[k]) for k, v in want_f.items())
 
 
+def test_ffn_with_the_shared_expert_on_a_second_stream():
+    """The shared expert beside the routed ones, forked and joined by events, eager and captured: the bits of the run on one stream."""
+    f = Ffn(3, 600, 512, 256, 16, 4, K.Act.BF16)
+    f.forward()
+    torch.cuda.synchronize()
+    keys = [k for k in f.b if k != "partial"]
+    want = {k: f.b[k].clone().view(torch.uint8) for k in keys}
+    side = torch.cuda.Stream()
+
+    def forked():
+        b, M, d, I, E, k, act = f.b, f.M, f.d, f.I, f.E, f.k, f.act
+        K.residual_rmsnorm_fp8(f.x, f.y, f.gain, M, d, 1e-6, b["x_out"], b["h"], b["q"], b["s"], act)
+        side.wait_stream(torch.cuda.current_stream())
+        K.linear_fp8(b["q"], b["s"], f.sgu, b["sg"], M, act, stream=side)
+        K.swiglu_fp8(b["sg"], b["sq"], b["ss"], M, I, act, stream=side)
+        K.linear_fp8(b["sq"], b["ss"], f.sdn, b["sy"], M, act, stream=side)
+        K.linear_bf16w(b["h"], f.router, b["logits"], M, E, d, act, K.Act.F32)
+        K.moe_router_scored(b["logits"], E, M, E, k, "sigmoid", f.bias, 4, 2, 2, True, 2.5, None, 0, 0, b["ids"], b["coef"], K.Act.F32, b["err"])
+        K.moe_group_routes(b["ids"], M, k, E, f.ws, f.n, b["err"])
+        K.linear_fp8_experts_gather_grouped(b["q"], b["s"], f.gu, E, f.ws, f.n, M, k, b["g1"], act)
+        K.swiglu_fp8(b["g1"], b["hq"], b["hs"], M * k, I, act)
+        K.linear_fp8_experts_combine_grouped(b["hq"], b["hs"], f.dn, E, b["ids"], b["coef"], f.ws, f.n, b["partial"], M, k, b["out"], act)
+        torch.cuda.current_stream().wait_stream(side)
+        K.residual_add(b["out"], b["sy"], M * d, act)
+
+    def wipe():
+        for k in keys:
+            f.b[k].view(torch.uint8).zero_()
+
+    wipe()
+    forked()
+    torch.cuda.synchronize()
+    assert all(torch.equal(v, f.b[k].view(torch.uint8)) for k, v in want.items())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        forked()
+    for _ in range(2):
+        wipe()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(v, f.b[k].view(torch.uint8)) for k, v in want.items())
+
+
 def test_wrappers_refuse_wrong_tensors():
     x = torch.zeros((4, 256), device="cuda")
     q, s = torch.zeros((4, 256), dtype=FP8, device="cuda"), torch.zeros((4, 2), device="cuda")
