@@ -46,10 +46,30 @@ struct Block8 {
     float hi[8], lo[8];
 };
 
-// The 8 values (times `unit`, a factor that the block shares) as e4m3 bytes of v / scale, scale = max(amax * unit, 2^-100) / 448: the largest
+// Two FP32 values in one register pair: an instruction for both, each half rounded as the scalar one rounds it.
+using Pair2 = uint64_t;
+__device__ __forceinline__ Pair2 two(float a, float b) {
+    Pair2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ Pair2 both(float a) { return two(a, a); }
+__device__ __forceinline__ void halves(Pair2 p, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ Pair2 mul2(Pair2 a, Pair2 b) {
+    Pair2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Pair2 fma2(Pair2 a, Pair2 b, Pair2 c) {
+    Pair2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// The 8 N values (times `unit`, a factor that the block shares) as e4m3 bytes of v / scale, scale = max(amax * unit, 2^-100) / 448: the largest
 // magnitude gets the largest e4m3 value, and a block of zeros has a scale that divides. A NaN stays one. The quotient is taken against the unrounded block maximum, in which the unit cancels: 448 / amax as two floats, three FMAs a value.
-__device__ __forceinline__ uint2 fp8_pack8(const Block8 &v, float amax, float unit, float &scale) {
-    uint32_t h[4];
+template <int N>
+__device__ __forceinline__ void fp8_pack(const Block8 (&v)[N], float amax, float unit, float &scale, uint2 (&codes)[N]) {
     const float top = amax * unit;
     if (top >= 0x1p-100f && amax > 0x1p-60f && amax < 0x1p60f) {
         const float s = top * (1.0f / 448.0f);
@@ -58,37 +78,51 @@ __device__ __forceinline__ uint2 fp8_pack8(const Block8 &v, float amax, float un
         r = fmaf(fmaf(-r, amax, 1.0f), r, r);
         const float inv = 448.0f * r, rest = fmaf(-inv, amax, 448.0f) * r;  // 448 / amax = inv + rest
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float a = fmaf(v.hi[2 * i], inv, fmaf(v.hi[2 * i], rest, v.lo[2 * i] * inv));
-            const float b = fmaf(v.hi[2 * i + 1], inv, fmaf(v.hi[2 * i + 1], rest, v.lo[2 * i + 1] * inv));
-            h[i] = e4m3x2(a, b);
+        for (int n = 0; n < N; ++n) {
+            uint32_t h[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const Pair2 hi = two(v[n].hi[2 * i], v[n].hi[2 * i + 1]), lo = two(v[n].lo[2 * i], v[n].lo[2 * i + 1]);
+                float a, b;
+                halves(fma2(hi, both(inv), fma2(hi, both(rest), mul2(lo, both(inv)))), a, b);
+                h[i] = e4m3x2(a, b);
+            }
+            codes[n] = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
         }
     } else {  // near FP32's ends, zero, infinite or NaN: word for word
         scale = __fdiv_rn(max_abs(0x1p-100f, top), 448.0f);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = e4m3x2(__fdiv_rn(v.hi[2 * i] * unit, scale), __fdiv_rn(v.hi[2 * i + 1] * unit, scale));
+        for (int n = 0; n < N; ++n) {
+            uint32_t h[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[i] = e4m3x2(__fdiv_rn(v[n].hi[2 * i] * unit, scale), __fdiv_rn(v[n].hi[2 * i + 1] * unit, scale));
+            codes[n] = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+        }
     }
-    return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
 }
 
-// e^-g for |g| < 80: 2^t with t = -g log2(e) in two parts (log2(e) = 1.44269502 + 1.93e-8), the second applied to first order. Off by the
-// 2^-22 of ex2.approx and two roundings.
-__device__ __forceinline__ float exp_neg(float g) {
-    const float t = g * -1.44269502f, rest = fmaf(g, -1.92596299e-8f, fmaf(g, -1.44269502f, -t));
-    float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-    return fmaf(e * 0.693147181f, rest, e);
-}
-
-// silu(g) * u of 8 pairs: g / (1 + e) by the approximate reciprocal and one correction by the exact remainder (Markstein's step). Where a
-// gate is near the ends of the exponential's range (or infinite, or NaN), as the definition says.
+// silu(g) * u of 8 pairs. e^-g for |g| < 80 is 2^t with t = -g log2(e) in two parts (log2(e) = 1.44269502 + 1.93e-8), the second applied to
+// first order: off by the 2^-22 of ex2.approx and two roundings. g / (1 + e) by the approximate reciprocal and one correction by the
+// exact remainder (Markstein's step). Where a gate is near the ends of the exponential's range (or infinite, or NaN), as the definition
+// says. In pairs, because the kernel is bound by the instructions that it issues.
 __device__ __forceinline__ void swiglu8(const float (&g)[8], const float (&u)[8], Block8 &h) {
     if (max_abs8(g) < 80.0f) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float d = 1.0f + exp_neg(g[j]), r = fast_rcp(d), q = g[j] * r, silu = fmaf(fmaf(-q, d, g[j]), r, q);
-            h.hi[j] = silu * u[j];
-            h.lo[j] = fmaf(silu, u[j], -h.hi[j]);
+        for (int j = 0; j < 8; j += 2) {
+            const Pair2 gg = two(g[j], g[j + 1]), uu = two(u[j], u[j + 1]);
+            const Pair2 t = mul2(gg, both(1.44269502f)), rest = fma2(gg, both(-1.92596299e-8f), fma2(gg, both(-1.44269502f), t));  // -t is 2's exponent
+            float t0, t1, e0, e1, d0, d1;
+            halves(t, t0, t1);
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(-t0));
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(-t1));
+            Pair2 e = two(e0, e1);
+            e = fma2(mul2(e, both(0.693147181f)), rest, e);
+            const Pair2 minus_d = fma2(e, both(-1.0f), both(-1.0f));
+            halves(minus_d, d0, d1);
+            const Pair2 r = two(fast_rcp(-d0), fast_rcp(-d1)), q = mul2(gg, r), silu = fma2(fma2(q, minus_d, gg), r, q);
+            const Pair2 hi = mul2(silu, uu);
+            halves(hi, h.hi[j], h.hi[j + 1]);
+            halves(fma2(silu, uu, mul2(hi, both(-1.0f))), h.lo[j], h.lo[j + 1]);
         }
     } else {
 #pragma unroll
@@ -103,10 +137,11 @@ __device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
     return r;
 }
 
-// The largest of the 16 lanes of a half warp (the 16 x 8 values of a block); NaN if one is.
-__device__ __forceinline__ float half_warp_max(float v) {
+// The largest of LANES neighbouring lanes (those that hold the 128 values of a block); NaN if one is.
+template <int LANES>
+__device__ __forceinline__ float lanes_max(float v) {
 #pragma unroll
-    for (int off = 8; off > 0; off >>= 1) v = max_abs(v, __shfl_xor_sync(0xffffffffu, v, off));
+    for (int off = LANES / 2; off > 0; off >>= 1) v = max_abs(v, __shfl_xor_sync(0xffffffffu, v, off));
     return v;
 }
 

@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(kNormMaxThreads)
     for (int i = 0; i < VEC; ++i) {
         const int c = (threadIdx.x + i * blockDim.x) * 8;
         float top = 0.f;
-        Block8 p;  // x' g in two parts (h / r), or h
+        Block8 part8[1], &p = part8[0];  // x' g in two parts (h / r), or h
         if (c < d) {
             float g[8], h[8];
             load8(w + c, g);
@@ -82,10 +82,12 @@ __global__ void __launch_bounds__(kNormMaxThreads)
             if (h_out != nullptr) store8(h_out + base + c, h);
         }
         if (q != nullptr) {  // the same for the whole grid; the reduction runs on full warps
-            top = half_warp_max(top);
+            top = lanes_max<16>(top);
             if (c < d) {
                 float s;
-                *reinterpret_cast<uint2 *>(q + base + c) = fp8_pack8(p, top, plain ? 1.0f : r, s);
+                uint2 codes[1];
+                fp8_pack(part8, top, plain ? 1.0f : r, s, codes);
+                *reinterpret_cast<uint2 *>(q + base + c) = codes[0];
                 if ((c & (kFp8Block - 1)) == 0) scale[row * blocks + c / kFp8Block] = s;
             }
         }
@@ -114,32 +116,37 @@ struct RowOf {
     int shift;
 };
 
-// A half warp per (row, 128-column block) of h = silu(gate) * up, 8 elements a thread. Gate and up stay FP32 until the one rounding
-// to e4m3.
+// Eight lanes per (row, 128-column block) of h = silu(gate) * up, 16 elements a thread. Gate and up stay FP32 until the one rounding
+// to e4m3. FP32 rows are bound by memory (40960 x 512: 28.6 us, 6.6 TB/s), BF16 rows by the instructions issued (21.9 us, 4.8 TB/s; with
+// 8 elements a thread, whose index, maximum and scale cost as much as those of 16: 25.1 us, and with scalar arithmetic 26.5).
+constexpr int kSwigluThreads = 256, kSwigluUnits = kSwigluThreads / 8;  // of a block
 template <typename T>
-__global__ void __launch_bounds__(256, 6) swiglu_fp8_kernel(const T *gu, uint8_t *q, float *scale, int64_t rows, int I, int blocks, RowOf row_of) {
+__global__ void __launch_bounds__(kSwigluThreads, 4) swiglu_fp8_kernel(const T *gu, uint8_t *q, float *scale, int64_t rows, int I, int blocks, RowOf row_of) {
     let_next_begin();
     wait_for_previous();
-    const int64_t units = rows * blocks, stride = (int64_t)gridDim.x * (blockDim.x / 16);
-    const int t = threadIdx.x & 15;
-    for (int64_t u0 = (int64_t)blockIdx.x * (blockDim.x / 16); u0 < units; u0 += stride) {
-        const int64_t u = u0 + threadIdx.x / 16;
+    const int64_t units = rows * blocks, stride = (int64_t)gridDim.x * kSwigluUnits;
+    const int t = threadIdx.x & 7;
+    for (int64_t u0 = (int64_t)blockIdx.x * kSwigluUnits; u0 < units; u0 += stride) {
+        const int64_t u = u0 + threadIdx.x / 8;
         const int64_t row = row_of.mul != 0 ? (int64_t)((uint64_t)(uint32_t)u * row_of.mul >> row_of.shift) : u / blocks;
-        const int b = (int)(u - row * blocks), c = b * kFp8Block + t * 8;
-        const bool live = u < units && c < I;
-        Block8 h;
+        const int b = (int)(u - row * blocks), c = b * kFp8Block + t * 16;
+        const bool live = u < units && c < I;  // I % 16 == 0
+        Block8 h[2];
         float top = 0.f;
         if (live) {
-            float g[8], up[8];
-            load8(gu + row * 2 * I + c, g);
-            load8(gu + row * 2 * I + I + c, up);
-            swiglu8(g, up, h);
-            top = max_abs8(h.hi);
+            const T *gate = gu + row * 2 * I + c, *up = gate + I;
+            float g[2][8], v[2][8];
+            load8(gate, g[0]), load8(gate + 8, g[1]);
+            load8(up, v[0]), load8(up + 8, v[1]);
+            swiglu8(g[0], v[0], h[0]), swiglu8(g[1], v[1], h[1]);
+            top = max_abs(max_abs8(h[0].hi), max_abs8(h[1].hi));
         }
-        top = half_warp_max(top);
+        top = lanes_max<8>(top);
         if (live) {
             float s;
-            *reinterpret_cast<uint2 *>(q + row * I + c) = fp8_pack8(h, top, 1.0f, s);
+            uint2 codes[2];
+            fp8_pack(h, top, 1.0f, s, codes);
+            *reinterpret_cast<uint4 *>(q + row * I + c) = make_uint4(codes[0].x, codes[0].y, codes[1].x, codes[1].y);
             if (t == 0) scale[u] = s;
         }
     }
@@ -197,18 +204,18 @@ int strix_swiglu_fp8(const void *gu, uint8_t *q, float *scale, int64_t rows, int
     SB_CHECK(apart(q, qb, gu, gb) && apart(scale, sb_, gu, gb) && apart(q, qb, scale, sb_), fn, ": q [", (const void *)q, "], scale [", (const void *)scale,
              "] and gu [", gu, "] overlap");
     const int blocks = (int)fp8_blocks(I);
-    const int64_t units = rows * blocks, want = (units + 15) / 16, cap = (int64_t)sm_count() * 32;
+    const int64_t units = rows * blocks, want = (units + kSwigluUnits - 1) / kSwigluUnits, cap = (int64_t)sm_count() * 32;
     const unsigned grid = (unsigned)(want < cap ? want : cap);
     auto st = static_cast<cudaStream_t>(stream);
     RowOf row_of{0, 0};
-    if (units + cap * 16 < (1ll << 31)) {
+    if (units + cap * kSwigluUnits < (1ll << 31)) {
         int log = 0;
         while ((1 << log) < blocks) ++log;
         row_of.shift = 31 + log;
         row_of.mul = (uint32_t)(((1ull << row_of.shift) + blocks - 1) / blocks);
     }
-    SB_CUDA((act == kF32 ? launch_after(swiglu_fp8_kernel<float>, dim3(grid), dim3(256), 0, st, 1, (const float *)gu, q, scale, rows, (int)I, blocks, row_of)
-                         : launch_after(swiglu_fp8_kernel<uint16_t>, dim3(grid), dim3(256), 0, st, 1, (const uint16_t *)gu, q, scale, rows, (int)I, blocks, row_of)),
+    SB_CUDA((act == kF32 ? launch_after(swiglu_fp8_kernel<float>, dim3(grid), dim3(kSwigluThreads), 0, st, 1, (const float *)gu, q, scale, rows, (int)I, blocks, row_of)
+                         : launch_after(swiglu_fp8_kernel<uint16_t>, dim3(grid), dim3(kSwigluThreads), 0, st, 1, (const uint16_t *)gu, q, scale, rows, (int)I, blocks, row_of)),
             fn, " ", act_name(act), " rows=", rows, " I=", I);
     return 0;
 }
