@@ -35,7 +35,7 @@ struct RouteArgs {
     int32_t *ids;
     float *coef;
     int A;
-    int per, L;  // experts of a group; lanes of a group: 32 / (G rounded up to a power of two)
+    int per, L, log_L;  // experts of a group; lanes of a group: 32 / (G rounded up to a power of two)
     uint32_t *err;
 };
 
@@ -162,13 +162,16 @@ __device__ __forceinline__ float4 load4(const uint16_t *p) {
 // The choice: the k-th largest lane maximum bounds the k-th largest value from below, what reaches it are the candidates (about 1.3 k of
 // them), they meet in shared memory and each counts those in front of it: no k rounds of warp-wide maxima. Where neighbours in that
 // order are closer than the error, the candidates are valued again in 64 bits (one token in a thousand).
+// Bound by the instructions issued: 16384 x 512 experts, 10 of 4 of 8 groups, 23.4 us, of which the loads are 4.9, scores 2.9, groups
+// 3.5, candidates and their order 7, the last step 4.
 //
 // The FP32 errors that the choice allows for (documented bounds: expf 2 ulp; ex2.approx 2^-22, rcp.approx 2^-23 relative):
 //   sigmoid  e = 2^(-l log2 e): the argument's roundings move e by 1.5 |l| 2^-24, so p by p (1 - p) (2^-22 + 1.5 |l| 2^-24) <= 0.7 * 2^-23; 1 + e
 //            and the reciprocal by 1.5 * 2^-23: 2.2 * 2^-23, for two values 4.4 * 2^-23 < 2^-20
 //   softmax  e = expf(l - top): (2 + |x| / 2) 2^-23 of e; the sum of up to 64 a lane and 5 steps: 35 * 2^-23 and the terms' mean, at most
 //            2 + ln(1024) / 2; p by at most 45 * 2^-23 of the largest p, for two values 90 * 2^-23 < 2^-16
-//   c = p + bias one rounding each, 2^-24 |c|: 2^-22 (|c| + |c'|) is above both
+//            relative to p itself: its exponential's error with |x| < 88 and the sum's, below 2^-16 p
+//   c = p + bias one rounding each, 2^-24 |c|: 2^-22 (|c| + |c'|) is above both; 2^-120 is above what is lost where a score is flushed to zero
 __device__ __forceinline__ float fast_sigmoid(float l) {
     float e, p;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(l * -1.44269504f));
@@ -176,18 +179,28 @@ __device__ __forceinline__ float fast_sigmoid(float l) {
     return p;
 }
 
+struct PerToken {
+    union {
+        struct {
+            float2 cand[kMaxCand];   // value, expert (as bits)
+            double exact[kMaxCand];  // of a close token: the candidates' values in 64 bits
+        };
+        float dealt[kMaxCand * 4];
+    };
+};
+
 template <typename T, int NV, bool VEC>
-__global__ void __launch_bounds__(kWarps * 32) router_scored_kernel(const T *logits, const T *shared, const RouteArgs a) {
-    __shared__ float2 cand[kWarps][kMaxCand];  // value, expert (as bits)
-    __shared__ double exact[kWarps][kMaxCand];  // of a close token: the candidates' values in 64 bits
+__global__ void __launch_bounds__(kWarps * 32, NV <= 8 ? 7 : 0) router_scored_kernel(const T *logits, const T *shared, const RouteArgs a) {
+    __shared__ PerToken tokens[kWarps];
     __shared__ float2 sorted[kWarps][40];
     const unsigned full = 0xffffffffu;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    PerToken &tok = tokens[warp];
     const int64_t m = (int64_t)blockIdx.x * kWarps + warp;
     let_next_begin();
     wait_for_previous();
     if (m >= a.M) return;  // whole warps leave together; no block-level barrier below
-    const int L = a.L, g = lane / L, sub = lane % L;
+    const int L = a.L, g = lane >> a.log_L, sub = lane & (L - 1);
     const T *row = logits + m * a.ld;
     auto expert = [&](int j) { return VEC ? g * a.per + (j >> 2) * 4 * L + sub * 4 + (j & 3) : g * a.per + sub + L * j; };
     auto holds = [&](int j) { return g < a.G && (VEC ? (j >> 2) * 4 * L + sub * 4 : sub + L * j) < a.per; };
@@ -261,6 +274,8 @@ __global__ void __launch_bounds__(kWarps * 32) router_scored_kernel(const T *log
     }
 
     double sum64 = 0.0;  // of the softmax, where something is done in 64 bits
+    float lm = -INFINITY;  // the lane's largest; -inf in a closed group
+    bool open = g < a.G;
     if (a.topk_group < a.G) {
         float b1 = -INFINITY, b2 = -INFINITY;  // the two largest of the lane, then of the group
 #pragma unroll
@@ -268,6 +283,7 @@ __global__ void __launch_bounds__(kWarps * 32) router_scored_kernel(const T *log
             b2 = fmaxf(b2, fminf(b1, c[j]));
             b1 = fmaxf(b1, c[j]);
         }
+        lm = b1;
         for (int off = L / 2; off > 0; off >>= 1) {
             const float o1 = __shfl_xor_sync(full, b1, off), o2 = __shfl_xor_sync(full, b2, off);
             b2 = fmaxf(fmaxf(b2, o2), fminf(b1, o1));
@@ -281,12 +297,11 @@ __global__ void __launch_bounds__(kWarps * 32) router_scored_kernel(const T *log
         } else if (biased) {
             tol = base + 0x1p-21f * fabsf(b1);
         }
-        int rank = 0;  // groups in front of this lane's
-        for (int h = 0; h < a.G; ++h) {
-            const float o = __shfl_sync(full, value, h * L);
-            rank += o > value || (o == value && h < g);
-        }
-        bool open = g < a.G && rank < a.topk_group;
+        int rank = 0;  // groups in front of this lane's: a larger value, or the same and a lower group
+        const uint32_t key = order_key(value);
+#pragma unroll 4
+        for (int h = 0; h < a.G; ++h) rank += __shfl_sync(full, key, h << a.log_L) + (h < g) > key;  // no value's key is the largest integer
+        open = g < a.G && rank < a.topk_group;
         if (biased || (a.group_top == 2 && a.per > 1)) {  // else the values are exact
             const float worst = __uint_as_float(__reduce_max_sync(full, g < a.G ? __float_as_uint(tol) : 0u));
             const float least_open = key_value(__reduce_min_sync(full, open ? order_key(value) : UINT_MAX));
@@ -322,50 +337,40 @@ __global__ void __launch_bounds__(kWarps * 32) router_scored_kernel(const T *log
                 open = g < a.G && rank < a.topk_group;
             }
         }
-        if (!open) {
+        if (!open) lm = -INFINITY;
+    } else {
 #pragma unroll
-            for (int j = 0; j < NV; ++j) c[j] = -INFINITY;
-        }
+        for (int j = 0; j < NV; ++j) lm = fmaxf(lm, c[j]);
     }
 
     int n = 0;  // candidates
     {
-        float lm = -INFINITY;
+        const unsigned lanes = __ballot_sync(full, open);
+        const int many = __popc(lanes);
+        if (many * 4 < a.k * 5 && many < 32 && a.topk_group * a.per > 32) {
+            // Few lanes are open and hold the experts of all: these are dealt anew, to every lane its share, or the bound would let most of them
+            // in (16384 tokens: 16 picks of 512 experts in 16 open lanes 68 -> 27 us, of 256 in 8 lanes 185 -> 46; below the rule, 6 of 64 in
+            // 8 lanes, 17.1 -> 17.0, 10 of 256 in 16 lanes 23.4 -> 24.6).
+            const int total = min(many * ((a.per + L - 1) >> a.log_L), kMaxCand * 4);  // what is not dealt only lowers the bound
+            int at = __popc(lanes & ((1u << lane) - 1));
 #pragma unroll
-        for (int j = 0; j < NV; ++j) lm = fmaxf(lm, c[j]);
+            for (int j = 0; j < NV; ++j, at += many)
+                if (open && at < total) tok.dealt[at] = c[j];
+            __syncwarp();
+            lm = -INFINITY;
+            for (int i = lane; i < total; i += 32) lm = fmaxf(lm, tok.dealt[i]);
+            __syncwarp();
+        }
         // the k-th largest lane maximum: k rounds of the warp's maximum (a hardware reduction of the ordered bits), the lane that held it out
         uint32_t key = order_key(lm), kth_key = 0;
         for (int r = 0; r < a.k; ++r) {
             kth_key = __reduce_max_sync(full, key);
             if (key == kth_key) key = 0;  // equal maxima go together: the bound is only lower
         }
-        float kth = kth_key == 0 ? -INFINITY : key_value(kth_key);
-        if (kth == -INFINITY && a.topk_group * a.per > 96) {
-            // Fewer lanes than k are open, and they hold many experts: the k-th largest value itself, by k rounds in which the lane that
-            // holds the largest drops it (16384 tokens, 16 of 256 open experts: 857 -> 185 us; of 63: 131 -> 216, so there all are candidates)
-            uint64_t gone = 0;
-            float best = lm;
-#pragma unroll 1
-            for (int r = 0; r < a.k; ++r) {
-                const uint32_t own = order_key(best);
-                kth_key = __reduce_max_sync(full, own);
-                if (own == kth_key) {
-                    float next = -INFINITY;
-                    bool dropped = false;
-#pragma unroll
-                    for (int j = 0; j < NV; ++j) {
-                        if (gone >> j & 1) continue;
-                        if (!dropped && c[j] == best) gone |= 1ull << j, dropped = true;
-                        else next = fmaxf(next, c[j]);
-                    }
-                    best = next;
-                }
-            }
-            kth = key_value(kth_key);
-        }
+        const float kth = kth_key == 0 ? -INFINITY : key_value(kth_key);
         // what lies below the k-th by no more than the error is a candidate too: nothing that is left out can belong to the picks.
         // -FLT_MAX: every finite value.
-        const float bound = fmaxf(biased ? kth - (base + 0x1p-21f * fabsf(kth)) : kth, -FLT_MAX);
+        const float bound = open ? fmaxf(biased ? kth - (base + 0x1p-21f * fabsf(kth)) : kth, -FLT_MAX) : INFINITY;
         int mine = 0;
 #pragma unroll
         for (int j = 0; j < NV; ++j) mine += c[j] >= bound;
@@ -381,17 +386,29 @@ __global__ void __launch_bounds__(kWarps * 32) router_scored_kernel(const T *log
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const bool in = c[j] >= bound;
-                if (in) cand[warp][at] = make_float2(c[j], __int_as_float(expert(j)));
+                if (in) tok.cand[at] = make_float2(c[j], __int_as_float(expert(j)));
                 at += in;
             }
             __syncwarp();
-            // in front: a larger value, then the lower expert; no two candidates are equal in both, so the ranks are 0 .. n - 1
-            for (int i = lane; i < n; i += 32) {
-                const float2 own = cand[warp][i];
+            // in front: a larger value, then the lower expert; no two candidates are equal in both, so the ranks are 0 .. n - 1. Up to 32 (nearly
+            // always) are compared from the lanes' registers by value, and by expert only where ranks meet.
+            if (n <= 32) {
+                const float2 own = lane < n ? tok.cand[lane] : make_float2(-INFINITY, 0.f);
+                int rank = 0;
+#pragma unroll 4
+                for (int q = 0; q < n; ++q) rank += __shfl_sync(full, own.x, q) > own.x;
+                if (__reduce_or_sync(full, lane < n ? 1u << rank : 0u) != 0xffffffffu >> (32 - n)) {  // n >= k >= 1
+                    unsigned same = __match_any_sync(full, __float_as_uint(own.x + 0.f)) & ~(1u << lane);  // -0 is 0
+                    for (same = lane < n ? same : 0u; same != 0; same &= same - 1) rank += __float_as_int(tok.cand[__ffs(same) - 1].y) < __float_as_int(own.y);
+                }
+                if (lane < n && rank <= a.k) sorted[warp][rank] = own;
+            }
+            for (int i = n <= 32 ? n : lane; i < n; i += 32) {
+                const float2 own = tok.cand[i];
                 int rank = 0;
 #pragma unroll 4
                 for (int q = 0; q < n; ++q) {
-                    const float2 o = cand[warp][q];
+                    const float2 o = tok.cand[q];
                     rank += o.x > own.x || (o.x == own.x && __float_as_int(o.y) < __float_as_int(own.y));
                 }
                 if (rank <= a.k) sorted[warp][rank] = own;
@@ -408,22 +425,30 @@ __global__ void __launch_bounds__(kWarps * 32) router_scored_kernel(const T *log
             const float value = sorted[warp][lane].x, next = sorted[warp][lane + 1].x;
             near = !(value - next > base + 0x1p-22f * (fabsf(value) + fabsf(next)));
         }
+        if (__any_sync(full, near)) {  // by the bound for the largest scores; these two may be small ones
+            const float inv = 1.0f / sum;
+            auto off = [&](float2 at) {
+                const float l = ld_act(row, __float_as_int(at.y));
+                return (a.score == kSigmoid ? 0x1p-20f * fast_sigmoid(l) : 0x1p-16f * (expf(l - top) * inv)) + 0x1p-22f * fabsf(at.x) + 0x1p-120f;
+            };
+            if (near) near = !(sorted[warp][lane].x - sorted[warp][lane + 1].x > off(sorted[warp][lane]) + off(sorted[warp][lane + 1]));
+        }
         if (__any_sync(full, near)) {
             // the candidates once more, in 64 bits
             if (a.score == kSoftmax && sum64 == 0.0) sum64 = softmax_sum_64(row, a.E, top);
 #pragma unroll 1
             for (int i = lane; i < n; i += 32) {
-                const int e = __float_as_int(cand[warp][i].y);
-                exact[warp][i] = score_64(ld_act(row, e), top, sum64, a.score) + (double)a.bias[e];
+                const int e = __float_as_int(tok.cand[i].y);
+                tok.exact[i] = score_64(ld_act(row, e), top, sum64, a.score) + (double)a.bias[e];
             }
             __syncwarp();
 #pragma unroll 1
             for (int i = lane; i < n; i += 32) {
-                const float2 own = cand[warp][i];
-                const double v = exact[warp][i];
+                const float2 own = tok.cand[i];
+                const double v = tok.exact[i];
                 int rank = 0;
 #pragma unroll 1
-                for (int q = 0; q < n; ++q) rank += exact[warp][q] > v || (exact[warp][q] == v && __float_as_int(cand[warp][q].y) < __float_as_int(own.y));
+                for (int q = 0; q < n; ++q) rank += tok.exact[q] > v || (tok.exact[q] == v && __float_as_int(tok.cand[q].y) < __float_as_int(own.y));
                 if (rank <= a.k) sorted[warp][rank] = own;
             }
             __syncwarp();
@@ -516,6 +541,7 @@ int strix_moe_router_scored(const void *logits, int64_t ld, int64_t M, int64_t E
     int gp = 1;
     while (gp < a.G) gp *= 2;
     a.per = a.E / a.G, a.L = 32 / gp;
+    while (1 << a.log_L < a.L) ++a.log_L;
     // runs of four where they fill the lanes of a group evenly and every row starts aligned
     const bool vec = a.per % (4 * a.L) == 0 && ld % 4 == 0 && reinterpret_cast<uintptr_t>(logits) % (4 * act_size(act)) == 0 && aligned16(bias);
     auto st = static_cast<cudaStream_t>(stream);

@@ -78,6 +78,23 @@ def test_route_close_scores_and_ties(score):
         assert torch.equal(ids.cpu(), want)
 
 
+@pytest.mark.parametrize("score", ("softmax", "sigmoid"))
+@pytest.mark.parametrize("E,k,G,tg", ((1024, 16, 4, 1), (1024, 16, 2, 1), (1024, 32, 8, 7), (1008, 16, 16, 1), (1000, 12, 8, 2), (128, 12, 8, 3), (510, 30, 17, 1), (96, 32, 3, 1)))
+def test_route_few_open_experts(score, E, k, G, tg):
+    """About as many picks as lanes that hold open experts, or more; the same with many equal scores and with scores one step apart."""
+    g = gen(E + k + G)
+    M = 150
+    logits = rand(g, M, E) * 1.5 - 1.0
+    logits[50:100] = torch.round(logits[50:100] * 2) / 2
+    logits[100:] = 1.0 + torch.randint(0, 3, (50, E), generator=g, device="cuda") * 2.0**-23
+    for bias in (None, rand(g, E) * 0.05, torch.round(rand(g, E) * 4) * 2.0**-24):
+        for gt in (1, 2):
+            want, cw = route(logits, k, score, bias, G, tg, gt, True, 2.5)
+            ids, coef, _ = run_route(logits, k, score, bias, G, tg, gt, True, 2.5, K.Act.F32)
+            assert torch.equal(ids.cpu(), want)
+            assert ((coef.cpu().double() - cw).abs() <= cw.abs() * 44 * 2.0**-24).all()
+
+
 def test_route_extremes_shared_slot_and_failed_tokens():
     E, k = 48, 5
     logits = torch.zeros((9, E + 4), device="cuda")  # column E is the shared gate; rows E + 4 apart
