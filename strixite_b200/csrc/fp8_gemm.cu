@@ -449,6 +449,12 @@ int check_rows(const char *fn, const uint8_t *xq, const float *xs, int64_t rows,
     return 0;
 }
 
+// The power of two up to 16 that the byte addresses of all rows of y are multiples of.
+int64_t row_start(const void *y, int64_t N, int act) {
+    const uint64_t bits = reinterpret_cast<uintptr_t>(y) | (uint64_t)(N * act_size(act)) | 16;
+    return (int64_t)(bits & (~bits + 1));
+}
+
 int grouped(const char *fn, const uint8_t *xq, const float *xs, const strix_fp8view *w, int64_t E, const void *ws, size_t ws_bytes, int64_t M, int64_t A,
             int64_t rows, void *y, int out_act, cudaStream_t st) {
     SB_TRY(check_view(fn, w));
@@ -466,10 +472,13 @@ int grouped(const char *fn, const uint8_t *xq, const float *xs, const strix_fp8v
     a.NT = (int)((N + kTileM - 1) / kTileM);
     // Below 8 slots an expert on average the narrow form, from there on the wide one. Measured (gate/up [1024, 2048] of 64 / 256 experts, us, narrow
     // and wide): mean 4: 22 and 29 / 75 and 83; mean 8: 26 and 31 / 99 and 89; mean 16: 33 and 33 / 142 and 101. Tiles of 32 or 64 slots in the narrow
-    // form were never the fastest.
+    // form were never the fastest. The narrow one, too, while it has no more than one (slot tile, weight tile) pair for each SM: 43 slots of 5
+    // experts [207, 592]: 4.5 and 10.5; 1024 of 8 [256, 512], 144 pairs: 5.9 and 8.1; beyond, 256 of 8 [1024, 2048], 192 pairs: 12.6 and 12.3.
+    // And up to three where rows of y start off a 16-byte boundary, which costs the wide form more: 2055 of 8 [281, 128], 408 pairs: 7.6 and 12.3;
+    // 2895 of 4 [310, 400], 552 pairs: 13.5 and 11.3.
     const int64_t tiles = std::min(S, E + S / 16);  // at most: every bucket may end in a partial tile
     SB_CHECK(tiles <= 0x7fffffff / a.NT, fn, ": ", S, " slots of N = ", N, " outputs are too many tiles");
-    if (S < 8 * E) return launch<16, true>(fn, w->q, w->N, xq, rows, w->K, a, tiles, st);
+    if (S < 8 * E || tiles * a.NT <= sm_count() * (row_start(y, N, out_act) < 16 ? 3 : 1)) return launch<16, true>(fn, w->q, w->N, xq, rows, w->K, a, tiles, st);
     return wide_grouped(fn, w->q, w->N, xq, rows, w->K, a, st);
 }
 
@@ -506,10 +515,11 @@ int strix_linear_fp8(const uint8_t *xq, const float *xs, const strix_fp8view *w,
     SB_TRY(check_rows(fn, xq, xs, M, w->K, y, M * w->N * act_size(out_act), out_act));
     // Tiles of 16 rows while K can be split four ways over the SMs, of 32 while there is an SM for each, else the wide form. Measured
     // ([N, K], M: us with 16 / 32 / wide): [1024, 2048], 64: 5.2 / 5.5 / 11.7, 128: 6.8 / 5.8 / 12.1, 512: 12.9 / 10.3 / 12.5, 1024: 20.9 / 15.9 / 12.7;
-    // [4096, 4096], 16: 7.7 / 8.1 / 18.0, 32: 9.6 / 8.9 / 18.5, 128: 20.7 / 14.3 / 19.9, 192: 28.5 / 23.2 / 19.8.
+    // [4096, 4096], 16: 7.7 / 8.1 / 18.0, 32: 9.6 / 8.9 / 18.5, 128: 20.7 / 14.3 / 19.9, 192: 28.5 / 23.2 / 19.8. Two tiles of
+    // 32 for each SM where rows of y start at odd 16-bit elements: [1001, 1024], 1024: 10.9 and 13.8, 1500: 14.8 and 13.9.
     const int64_t sms = sm_count();
     if (tiles(16) * a.NT * 4 <= sms) return launch<16, false>(fn, w->q, w->N, xq, M, w->K, a, tiles(16), st);
-    if (tiles(32) * a.NT <= sms) return launch<32, false>(fn, w->q, w->N, xq, M, w->K, a, tiles(32), st);
+    if (tiles(32) * a.NT <= sms * (row_start(y, w->N, out_act) < 4 ? 2 : 1)) return launch<32, false>(fn, w->q, w->N, xq, M, w->K, a, tiles(32), st);
     return wide_dense(fn, w->q, w->N, xq, M, w->K, a, st);
 }
 

@@ -360,6 +360,8 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
             const int n_rows = t.n, n_base = t.n0 + h * kHalf;
             const int64_t out_row = row;
             fetch(p + step);
+            const int live_rows = min(32, n_rows - (warp & 3) * 32);  // of this warp
+            if (live_rows <= 0) continue;
             // y: 64 bytes of every row at a time through the strip; then 4 lanes write a row's 64 bytes, 8 rows an instruction
             const int es = a.out_f32 ? 4 : 2;
             const uint64_t at = reinterpret_cast<uint64_t>(a.y) | (uint64_t)a.N * es;  // what every row's start is a multiple of
@@ -371,7 +373,7 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
                     for (int i = 0; i < 4; ++i) {
                         const int rr = i * 8 + (lane >> 2), n = n_base + col + (lane & 3) * (16 / es);
                         const int64_t orow = __shfl_sync(0xffffffffu, out_row, rr);
-                        const bool live = (warp & 3) * 32 + rr < n_rows;
+                        const bool live = rr < live_rows;
                         const uint4 q = *reinterpret_cast<const uint4 *>(strip + rr * kStripPitch + (lane & 3) * 16);
                         uint8_t *dst = static_cast<uint8_t *>(a.y) + (orow * a.N + n) * es;
                         if (live && n < a.N) *reinterpret_cast<uint4 *>(dst) = q;
@@ -379,16 +381,25 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
                 } else {
                     // rows that start anywhere: neighbouring lanes write neighbouring words (16 a row, two rows an instruction) or halves.
                     // 2293 x 656 against 2112 (vectors), 2116 (words), 2115 (halves) rows: 13.2, 18.5, 26.5 us; each lane its own row: 43 us.
-                    const int per = 64 / unit, mine = lane & (per - 1), n = n_base + col + mine * unit / es;
-#pragma unroll 8
-                    for (int i = 0; i < per; ++i) {
-                        const int rr = unit == 4 ? i * 2 + (lane >> 4) : i;
-                        const int64_t orow = __shfl_sync(0xffffffffu, out_row, rr);
-                        if ((warp & 3) * 32 + rr >= n_rows || n >= a.N) continue;
-                        uint8_t *dst = static_cast<uint8_t *>(a.y) + (orow * a.N + n) * es;
-                        const uint8_t *src = strip + rr * kStripPitch + mine * unit;
-                        if (unit == 4) *reinterpret_cast<uint32_t *>(dst) = *reinterpret_cast<const uint32_t *>(src);
-                        else *reinterpret_cast<uint16_t *>(dst) = *reinterpret_cast<const uint16_t *>(src);
+                    const int per = 64 / unit, mine = lane & (per - 1), n = n_base + col + mine * unit / es, times = unit == 4 ? (live_rows + 1) / 2 : live_rows;
+                    const uint8_t *src = strip + mine * unit;
+                    uint8_t *dst = static_cast<uint8_t *>(a.y) + (int64_t)n * es;
+                    for (int i = 0; i < times; i += 4) {
+                        uint8_t *to[4];
+                        uint32_t v[4];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const int rr = unit == 4 ? (i + q) * 2 + (lane >> 4) : i + q;
+                            to[q] = dst + __shfl_sync(0xffffffffu, out_row, rr) * a.N * es;
+                            if (rr >= live_rows || n >= a.N) to[q] = nullptr;
+                            v[q] = unit == 4 ? *reinterpret_cast<const uint32_t *>(src + rr * kStripPitch) : *reinterpret_cast<const uint16_t *>(src + rr * kStripPitch);
+                        }
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            if (to[q] == nullptr) continue;
+                            if (unit == 4) *reinterpret_cast<uint32_t *>(to[q]) = v[q];
+                            else *reinterpret_cast<uint16_t *>(to[q]) = (uint16_t)v[q];
+                        }
                     }
                 }
                 __syncwarp();
