@@ -12,7 +12,7 @@ import enum
 import numpy as np
 import torch
 
-from ._lib import Fp8View, QMixView, QView, StrixError, call, lib  # noqa: F401
+from ._lib import Fp8View, QMixView, QView, StrixError, call, last_error, lib  # noqa: F401
 
 
 class Act(enum.IntEnum):  # strixite kernels/norm.hpp:20
@@ -515,6 +515,14 @@ def linear_qw_experts_combine_grouped(h, w, E, ids, coef, ws, ws_bytes, partial,
 # shape has no other sign of it; a tensor of another device than the current one is refused (the launch goes to the current one).
 
 
+_device = torch._C._cuda_getDevice  # torch.cuda.current_device() without its Python
+
+
+def _ok(rc):
+    if rc != 0:
+        raise StrixError(last_error())
+
+
 class Score(enum.IntEnum):
     Softmax = 0
     Sigmoid = 1
@@ -605,7 +613,7 @@ def moe_router_scored(logits, ld, M, E, k, score, bias, n_group, topk_group, gro
     """Score-based routing: `score` 'softmax' or 'sigmoid' (or Score), an optional balance bias [E] for the choice, n_group groups of which
     topk_group stay open (a group's value: its group_top = 1 or 2 largest), k picks, weights renormalised when `renorm`, times route_scale.
     logits: a tensor whose first element is token 0's first logit, rows ld apart; shared_logit as in moe_router."""
-    fn, dev = "moe_router_scored", torch.cuda.current_device()
+    fn, dev = "moe_router_scored", _device()
     how = _SCORES.get(score)
     if how is None:
         raise StrixError("%s: score %r, expected 'softmax' or 'sigmoid'" % (fn, score))
@@ -619,49 +627,49 @@ def moe_router_scored(logits, ld, M, E, k, score, bias, n_group, topk_group, gro
             raise StrixError("%s: %s must be a %s tensor on the current device cuda:%d" % (fn, name, dt[0], dev))
         if t.untyped_storage().nbytes() // t.element_size() - t.storage_offset() < (M - 1) * stride + last:
             raise StrixError("%s: %s ends before the last of %d rows, %d apart" % (fn, name, M, stride))
-    call("strix_moe_router_scored", logits.data_ptr(), ld, M, E, k, how, _t(fn, "bias", bias, _F32, E, dev, True), n_group, topk_group, group_top, 1 if renorm else 0,
+    _ok(lib.strix_moe_router_scored(logits.data_ptr(), ld, M, E, k, how, _t(fn, "bias", bias, _F32, E, dev, True), n_group, topk_group, group_top, 1 if renorm else 0,
          route_scale, None if shared_logit is None else shared_logit.data_ptr(), shared_ld, shared_id, _t(fn, "ids", ids, _I32, M * A, dev),
-         _t(fn, "coef", coef, _F32, M * A, dev), act, _t(fn, "err", err, _I32, 3, dev), _raw(stream, dev))
+         _t(fn, "coef", coef, _F32, M * A, dev), act, _t(fn, "err", err, _I32, 3, dev), _raw(stream, dev)))
 
 
 def residual_rmsnorm_fp8(x, y, w, M, d, eps, x_out, h, q, scale, act, centered=False, stream=None):
     """x_out = x + y (both None: x alone; x_out may be x or y), h = RMSnorm(x_out) * (w, or 1 + w when centered), q / scale: h as FP8 rows.
     h, or q and scale, may be None."""
-    fn, dev = "residual_rmsnorm_fp8", torch.cuda.current_device()
+    fn, dev = "residual_rmsnorm_fp8", _device()
     dt, n = _act_dtypes(fn, act), M * d
-    call("strix_residual_rmsnorm_fp8", _t(fn, "x", x, dt, n, dev), _t(fn, "y", y, dt, n, dev, True), _t(fn, "w", w, _F32, d, dev), 1 if centered else 0, eps, M, d,
+    _ok(lib.strix_residual_rmsnorm_fp8(_t(fn, "x", x, dt, n, dev), _t(fn, "y", y, dt, n, dev, True), _t(fn, "w", w, _F32, d, dev), 1 if centered else 0, eps, M, d,
          _t(fn, "x_out", x_out, dt, n, dev, True), _t(fn, "h", h, dt, n, dev, True), _t(fn, "q", q, _F8, n, dev, True),
-         _t(fn, "scale", scale, _F32, M * fp8_blocks(d), dev, True), act, _raw(stream, dev))
+         _t(fn, "scale", scale, _F32, M * fp8_blocks(d), dev, True), act, _raw(stream, dev)))
 
 
 def swiglu_fp8(gu, q, scale, rows, I, act, stream=None):
     """swiglu of merged [gate | up] rows [rows, 2I] with the result as FP8 rows q [rows, I], scale [rows, blocks(I)]."""
-    fn, dev = "swiglu_fp8", torch.cuda.current_device()
-    call("strix_swiglu_fp8", _t(fn, "gu", gu, _act_dtypes(fn, act), rows * 2 * I, dev), _t(fn, "q", q, _F8, rows * I, dev),
-         _t(fn, "scale", scale, _F32, rows * fp8_blocks(I), dev), rows, I, act, _raw(stream, dev))
+    fn, dev = "swiglu_fp8", _device()
+    _ok(lib.strix_swiglu_fp8(_t(fn, "gu", gu, _act_dtypes(fn, act), rows * 2 * I, dev), _t(fn, "q", q, _F8, rows * I, dev),
+         _t(fn, "scale", scale, _F32, rows * fp8_blocks(I), dev), rows, I, act, _raw(stream, dev)))
 
 
 def linear_fp8(xq, xs, w, y, M, out_act, stream=None):
     """y[M, N] = the FP8 rows (xq [M, K], xs [M, blocks(K)]) times an Fp8Weight [N, K] transposed, FP32 or BF16."""
-    fn, dev = "linear_fp8", torch.cuda.current_device()
+    fn, dev = "linear_fp8", _device()
     v = _fp8w(fn, w, 1, dev)
-    call("strix_linear_fp8", _t(fn, "xq", xq, _F8, M * w.K, dev), _t(fn, "xs", xs, _F32, M * w.KB, dev), v, _t(fn, "y", y, _act_dtypes(fn, out_act), M * w.N, dev), M,
-         out_act, _raw(stream, dev))
+    _ok(lib.strix_linear_fp8(_t(fn, "xq", xq, _F8, M * w.K, dev), _t(fn, "xs", xs, _F32, M * w.KB, dev), v, _t(fn, "y", y, _act_dtypes(fn, out_act), M * w.N, dev), M,
+         out_act, _raw(stream, dev)))
 
 
 def linear_fp8_experts_gather_grouped(xq, xs, w, E, ws, ws_bytes, M, A, y, out_act, stream=None):
     """y[slot, :] = expert ids[slot] of the stack times FP8 row slot / A, over the workspace of moe_group_routes(ids, M, A, E, ...)."""
-    fn, dev = "linear_fp8_experts_gather_grouped", torch.cuda.current_device()
+    fn, dev = "linear_fp8_experts_gather_grouped", _device()
     v = _fp8w(fn, w, E, dev)
-    call("strix_linear_fp8_experts_gather_grouped", _t(fn, "xq", xq, _F8, M * w.K, dev), _t(fn, "xs", xs, _F32, M * w.KB, dev), v, E, _any_bytes(fn, "ws", ws, ws_bytes, dev),
-         ws_bytes, M, A, _t(fn, "y", y, _act_dtypes(fn, out_act), M * A * (w.N // E), dev), out_act, _raw(stream, dev))
+    _ok(lib.strix_linear_fp8_experts_gather_grouped(_t(fn, "xq", xq, _F8, M * w.K, dev), _t(fn, "xs", xs, _F32, M * w.KB, dev), v, E, _any_bytes(fn, "ws", ws, ws_bytes, dev),
+         ws_bytes, M, A, _t(fn, "y", y, _act_dtypes(fn, out_act), M * A * (w.N // E), dev), out_act, _raw(stream, dev)))
 
 
 def linear_fp8_experts_combine_grouped(hq, hs, w, E, ids, coef, ws, ws_bytes, partial, M, A, y, act, stream=None):
     """y[m, :] = sum over a of coef[m, a] * (expert ids[m, a] of the stack times FP8 row m * A + a); partial: M * A * N floats."""
-    fn, dev = "linear_fp8_experts_combine_grouped", torch.cuda.current_device()
+    fn, dev = "linear_fp8_experts_combine_grouped", _device()
     v = _fp8w(fn, w, E, dev)
     S, N = M * A, w.N // E
-    call("strix_linear_fp8_experts_combine_grouped", _t(fn, "hq", hq, _F8, S * w.K, dev), _t(fn, "hs", hs, _F32, S * w.KB, dev), v, E, _t(fn, "ids", ids, _I32, S, dev),
+    _ok(lib.strix_linear_fp8_experts_combine_grouped(_t(fn, "hq", hq, _F8, S * w.K, dev), _t(fn, "hs", hs, _F32, S * w.KB, dev), v, E, _t(fn, "ids", ids, _I32, S, dev),
          _t(fn, "coef", coef, _F32, S, dev), _any_bytes(fn, "ws", ws, ws_bytes, dev), ws_bytes, _t(fn, "partial", partial, _F32, S * N, dev), M, A,
-         _t(fn, "y", y, _act_dtypes(fn, act), M * N, dev), act, _raw(stream, dev))
+         _t(fn, "y", y, _act_dtypes(fn, act), M * N, dev), act, _raw(stream, dev)))
