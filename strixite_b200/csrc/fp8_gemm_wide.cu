@@ -10,8 +10,12 @@
 // bounds the one-CTA form. GROUP = 1 (the experts' slots, gathered by row): an expert has seldom more than 128 rows.
 //
 // Roles: warps 0-3 / 4-7 promote column half 0 / 1 (each half has two accumulators, so the tensor cores run up to three half blocks
-// ahead), warp 8 issues TMA, warps 9 and 10 the MMAs of half 0 and 1 (those of CTA 0 for both CTAs), warps 11-13 gather rows of x. The sums leave through a 64-byte-wide staging strip per warp so that a
-// store covers whole sectors of a row.
+// ahead), warp 8 issues TMA, warps 9 and 10 the MMAs of half 0 and 1 (those of CTA 0 for both CTAs), warps 11-13 gather rows of x. The
+// sums leave through a 64-byte-wide staging strip per warp so that a store covers whole sectors of a row.
+//
+// Measured: 16384 x 4096 x 4096 246 us, 2.23 PFLOP/s, tensor pipe 61 % active; 4096 tokens x 10 of 512 experts [1024, 2048] 247 us, 4.8 TB/s.
+// What bounds both is the chain of a block: its MMAs' commit, the promotion, the accumulator's release, ~750 clocks for 512 of MMA with
+// tensor memory full (the grouped feed alone takes 181 to 190 us).
 // Every mbarrier wait is bounded: on expiry the CTA raises the abort counter, waits for its copies, frees its tensor memory, returns.
 #include <algorithm>
 

@@ -102,8 +102,8 @@ __device__ __forceinline__ void cluster_meet() { asm volatile("barrier.cluster.a
 // its slots per bucket in its own row of `cnt`, the per-bucket prefix over the warps (and over the blocks in front, read from their
 // shared memory) turns the counts into the warp's first position in each bucket, and the warp then places its slots in slot order (ranks inside a
 // 32-slot step by __match_any_sync). So a bucket lists its slots ascending, whatever the scheduling: the permutation is a pure
-// function of ids. Bound by the latency of the steps of a segment: 40960 slots over 513 buckets took 53 us in one block, 8 blocks
-// cut the steps to an eighth.
+// function of ids. Bound by the latency of the steps of a segment: 40960 slots over 513 buckets took 55 us in one block, 8 blocks
+// cut the steps to an eighth (16 us); from 2048 slots on that pays for the cluster's two meetings.
 template <bool CLUSTER>
 __global__ void __launch_bounds__(kRouteThreads)
     route_kernel(const int32_t *ids, int S, int E, int Tmax, int WTmax, int32_t *ws, uint32_t *err) {
