@@ -116,9 +116,9 @@ __global__ void __launch_bounds__(kRouteThreads)
     int *wtile0 = tile0 + B + 1;          // [B + 1] first 64-slot tile
     __shared__ int first_bad;
     __shared__ uint64_t warp_tot[kRouteWarps], total;
-    __shared__ int block_count[kMaxBuckets];
+    __shared__ int block_count[CLUSTER ? kMaxBuckets : 1], block_start[CLUSTER ? kMaxBuckets : 1];  // this block's share of a bucket
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int rank = CLUSTER ? (int)blockIdx.x : 0, blocks = CLUSTER ? (int)gridDim.x : 1;  // the grid is one cluster
+    const int rank = CLUSTER ? (int)blockIdx.x : 0, blocks = CLUSTER ? kRouteBlocks : 1;  // the grid is one cluster
     const int seg = ((S + kRouteWarps * blocks - 1) / (kRouteWarps * blocks) + 31) & ~31;
     const int s_begin = min(S, (rank * kRouteWarps + warp) * seg), s_end = min(S, s_begin + seg);
     const int left = S - rank * kRouteWarps * seg, live_warps = left <= 0 ? 0 : min(kRouteWarps, (left + seg - 1) / seg);  // with slots of their own
@@ -141,10 +141,15 @@ __global__ void __launch_bounds__(kRouteThreads)
     __syncthreads();
     int count = 0;
     if (t < B) {
-        for (int w = 0; w < live_warps; ++w) {
-            const int c = cnt[w * B + t];
-            cnt[w * B + t] = count;  // this warp's first rank inside the block's share of the bucket
-            count += c;
+        for (int w0 = 0; w0 < live_warps; w0 += 8) {  // eight counts in flight
+            int c[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) c[j] = w0 + j < live_warps ? cnt[(w0 + j) * B + t] : 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (w0 + j < live_warps) cnt[(w0 + j) * B + t] = count;  // the warp's first rank inside the block's share of the bucket
+                count += c[j];
+            }
         }
     }
     int before = 0;  // slots of bucket t in the blocks in front
@@ -152,12 +157,12 @@ __global__ void __launch_bounds__(kRouteThreads)
         if (t < B) block_count[t] = count;
         cluster_meet();
         if (t < B) {
+            int c[kRouteBlocks];
+#pragma unroll
+            for (int r = 0; r < kRouteBlocks; ++r) c[r] = (int)peer_u32(&block_count[t], r);
             count = 0;
-            for (int r = 0; r < blocks; ++r) {
-                const int c = (int)peer_u32(&block_count[t], r);
-                before += r < rank ? c : 0;
-                count += c;
-            }
+#pragma unroll
+            for (int r = 0; r < kRouteBlocks; ++r) before += r < rank ? c[r] : 0, count += c[r];
         }
         if (rank == 0 && t == 0)
             for (int r = 1; r < blocks; ++r) first_bad = min(first_bad, (int)peer_u32(&first_bad, r));
@@ -171,7 +176,7 @@ __global__ void __launch_bounds__(kRouteThreads)
     int32_t *wtile_bucket = tile_start + Tmax, *wtile_start = wtile_bucket + WTmax;
     if (t < B) {
         start[t] = st, tile0[t] = tl, wtile0[t] = wt;
-        for (int w = 0; w < live_warps; ++w) cnt[w * B + t] += st + before;  // from here on: the warp's next position in the bucket
+        if constexpr (CLUSTER) block_start[t] = st + before;
         if (rank == 0) offsets[t] = st;
     }
     if (t == 0) {
@@ -200,7 +205,7 @@ __global__ void __launch_bounds__(kRouteThreads)
         if (live) b = (id < 0 || id >= E) ? E : id;
         const unsigned same = __match_any_sync(0xffffffffu, b);
         const int place = __popc(same & ((1u << lane) - 1u));
-        if (live) slots[cnt[warp * B + b] + place] = s;
+        if (live) slots[(CLUSTER ? block_start : start)[b] + cnt[warp * B + b] + place] = s;
         __syncwarp();
         if (live && place == 0) cnt[warp * B + b] += __popc(same);
         __syncwarp();
