@@ -7,7 +7,9 @@
 //
 // GROUP = 2 (dense): a cluster of two CTAs works on 256 rows x 256 columns with cta_group::2 instructions. Each CTA loads its 128 rows of
 // x and half of the weight rows, 32 KB a block of K instead of 48: the feed from L2 (about 58 bytes a clock and SM, measured) is what
-// bounds the one-CTA form. GROUP = 1 (the experts' slots, gathered by row): an expert has seldom more than 128 rows.
+// bounds the one-CTA form. SPLIT: two such pairs share the K blocks of a tile, and each adds up one half of the columns (few tiles, long
+// K: the chain of one tile's blocks is the time). GROUP = 1 (the experts' slots, gathered by row): an expert has seldom more than 128
+// rows.
 //
 // Roles: warps 0-3 / 4-7 promote column half 0 / 1 (each half has two accumulators, so the tensor cores run up to three half blocks
 // ahead), warp 8 issues TMA, warps 9 and 10 the MMAs of half 0 and 1 (those of CTA 0 for both CTAs), warps 11-13 gather rows of x. The
@@ -80,12 +82,12 @@ __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t da, uint64_t d
             : "memory");
     }
 }
-// Arrival on `bar` of this CTA (GROUP 1) or of both CTAs (GROUP 2) when the MMAs issued so far have completed.
+// Arrival on `bar` of this CTA (GROUP 1) or of both CTAs (GROUP 2; their bits in the cluster) when the MMAs issued so far have completed.
 template <int GROUP>
-__device__ __forceinline__ void commit(uint64_t *bar) {
+__device__ __forceinline__ void commit(uint64_t *bar, uint16_t ctas) {
     if constexpr (GROUP == 1) umma_commit(bar);
     else
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"(ctas)
                      : "memory");
 }
 // A box into this CTA's shared memory, counted on the barrier at cluster address `bar` (the leader's).
@@ -116,7 +118,7 @@ struct Tile {
     int wrow, n0, ws_row, halves, first, n;
 };
 
-template <int GROUP, bool GROUPED>
+template <int GROUP, bool GROUPED, bool SPLIT>
 __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
     fp8_wide_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const GemmArgs a) {
     using C = Cfg<GROUP>;
@@ -127,7 +129,10 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     let_next_begin();
     if (warp == kTmaWarp && elect_one()) prefetch_map(&w_map), prefetch_map(&x_map);
-    const uint32_t rank = GROUP == 2 ? cluster_rank() : 0;
+    const uint32_t in_cluster = GROUP == 2 ? cluster_rank() : 0, rank = in_cluster & 1u, leader = in_cluster & ~1u;  // a pair is ranks 2i, 2i + 1
+    constexpr int kCtas = GROUP * (SPLIT ? 2 : 1);  // that share a tile
+    const int part = SPLIT ? (int)in_cluster >> 1 : 0, kb0 = SPLIT ? a.KB * part / 2 : 0, kb1 = SPLIT ? a.KB * (part + 1) / 2 : a.KB;
+    const uint16_t both_ctas = (uint16_t)(3u << leader);
     if (tid == 0) {
         for (int i = 0; i < C::Stages; ++i) mbar_init(&ctl.full[i], 1), mbar_init(&ctl.empty[i], 2);  // empty: both halves' MMAs
         for (int i = 0; i < 4; ++i) mbar_init(&ctl.acc_full[i / 2][i % 2], 1), mbar_init(&ctl.acc_empty[i / 2][i % 2], 4 * GROUP);
@@ -161,7 +166,7 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
     tc_fence_after();
     const uint32_t tmem = ctl.tmem_base;
     volatile int *abort_flag = &ctl.abort_flag;
-    const int n_tiles = refused ? 0 : x_tiles * a.NT, step = gridDim.x / GROUP;
+    const int n_tiles = refused ? 0 : x_tiles * a.NT, step = gridDim.x / kCtas;
 
     auto tile_of = [&](int p) {  // warp-uniform
         const int xt = p / a.NT, nt = p - xt * a.NT;
@@ -190,7 +195,7 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
         const int quad = (warp - kGatherWarp) + kGatherWarps * lane;  // gathering: rows 4 * quad .. of the tile
         uint32_t it = 0;
         bool ok = true;
-        for (int p = blockIdx.x / GROUP; p < n_tiles && ok; p += step) {
+        for (int p = blockIdx.x / kCtas; p < n_tiles && ok; p += step) {
             const Tile t = tile_of(p);
             int rows[4] = {0, 0, 0, 0};
             uint32_t bytes = (uint32_t)C::StageBytes * GROUP;
@@ -204,7 +209,7 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
                 if (warp >= kGatherWarp)
                     for (int j = 0; j < 4; ++j) rows[j] = rt.slots[t.first + min(quad * 4 + j, t.n - 1)] / a.div;
             }
-            for (int kb = 0; kb < a.KB; ++kb, ++it) {
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
                 const int s = it % C::Stages;
                 ok = __all_sync(0xffffffffu, mbar_wait(&ctl.empty[s], ((it / C::Stages) & 1u) ^ 1u, abort_flag));
                 if (!ok) break;
@@ -216,7 +221,7 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
                         // the leader's barrier counts both CTAs' bytes; this CTA's weight rows are the rank-th 64 of each half, so that a
                         // half's instruction (64 rows from each CTA) covers 128 neighbouring rows
                         if (rank == 0) mbar_expect_tx(&ctl.full[s], bytes);
-                        const uint32_t bar = peer_addr(&ctl.full[s], 0);
+                        const uint32_t bar = peer_addr(&ctl.full[s], leader);
                         tma_load_pair(dst, &x_map, kb * kBK, t.first, bar);
                         tma_load_pair(dst + C::ATile, &w_map, kb * kBK, t.wrow + (int)rank * 64, bar);
                         tma_load_pair(dst + C::ATile + 64 * kBK, &w_map, kb * kBK, t.wrow + kHalf + (int)rank * 64, bar);
@@ -246,9 +251,9 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
             const uint32_t idesc = idesc_e4m3(kRows * GROUP, kHalf);
             uint32_t it = 0, done = 0;
             bool ok = true, full = false, free = true;  // fresh accumulators are free
-            for (int p = blockIdx.x / GROUP; p < n_tiles && ok; p += step) {
+            for (int p = blockIdx.x / kCtas; p < n_tiles && ok; p += step) {
                 const Tile t = tile_of(p);
-                for (int kb = 0; kb < a.KB; ++kb) {
+                for (int kb = kb0; kb < kb1; ++kb) {
                     const int s = it % C::Stages;
                     if (!full) ok = mbar_wait(&ctl.full[s], (it / C::Stages) & 1u, abort_flag);
                     if (!ok) break;
@@ -265,11 +270,11 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
                         ++done;
                         free = mbar_test(&ctl.acc_empty[h][done & 1u], ((done >> 1) & 1u) ^ 1u);
                         full = mbar_test(&ctl.full[it % C::Stages], (it / C::Stages) & 1u);
-                        commit<GROUP>(&ctl.acc_full[h][b]);
-                        commit<GROUP>(&ctl.empty[s]);
+                        commit<GROUP>(&ctl.acc_full[h][b], both_ctas);
+                        commit<GROUP>(&ctl.empty[s], both_ctas);
                     } else {
                         full = false;
-                        commit<GROUP>(&ctl.empty[s]);  // nothing of this half reads the stage
+                        commit<GROUP>(&ctl.empty[s], both_ctas);  // nothing of this half reads the stage
                     }
                 }
             }
@@ -281,9 +286,9 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
         const int h = warp >> 2, r = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + h * kHalf;
         uint8_t *strip = strips + warp * kStrip;
-        const uint32_t empty_at = peer_addr(&ctl.acc_empty[0][0], 0);  // the leader's
+        const uint32_t empty_at = peer_addr(&ctl.acc_empty[0][0], leader);
         uint32_t done = 0;
-        bool ok = true;
+        bool ok = true, met = false;
         // What a tile starts with - its rows and first scales, up to three dependent loads - is fetched before the store of the tile in
         // front of it.
         Tile t{};
@@ -307,10 +312,10 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
             wp = a.ws + (int64_t)(t.ws_row + h) * a.KB;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                if (i < a.KB) sx[i] = xp != nullptr ? xp[i] : 0.f, sw[i] = wp[i];
+                if (kb0 + i < kb1) sx[i] = xp != nullptr ? xp[kb0 + i] : 0.f, sw[i] = wp[kb0 + i];
         };
-        fetch(blockIdx.x / GROUP);
-        for (int p = blockIdx.x / GROUP; p < n_tiles; p += step) {
+        fetch(blockIdx.x / kCtas);
+        for (int p = blockIdx.x / kCtas; p < n_tiles; p += step) {
             if (h >= t.halves) {
                 fetch(p + step);
                 continue;
@@ -329,10 +334,10 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
             if (!ok) break;
             tc_fence_after();
             tmem_ld32(lanes + (done & 1u) * 2 * kHalf, v0);
-            for (int kb = 0; kb < a.KB; ++kb) {
+            for (int kb = kb0; kb < kb1; ++kb) {
                 const float s = sx[0] * sw[0];
                 sx[0] = sx[1], sw[0] = sw[1];
-                if (kb + 2 < a.KB) sx[1] = xp != nullptr ? xp[kb + 2] : 0.f, sw[1] = wp[kb + 2];
+                if (kb + 2 < kb1) sx[1] = xp != nullptr ? xp[kb + 2] : 0.f, sw[1] = wp[kb + 2];
                 const uint32_t b = done & 1u, from = lanes + b * 2 * kHalf;
                 ++done;
                 tmem_ld_wait();
@@ -343,7 +348,7 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
                 add(v1, 1, s);
                 tmem_ld_wait();
                 tmem_ld32(from + 96, v1);
-                const bool more = kb + 1 < a.KB, ready = more && mbar_test(&ctl.acc_full[h][done & 1u], (done >> 1) & 1u);
+                const bool more = kb + 1 < kb1, ready = more && mbar_test(&ctl.acc_full[h][done & 1u], (done >> 1) & 1u);
                 add(v0, 2, s);
                 tmem_ld_wait();  // everything is in registers: the accumulator is free
                 tc_fence_before();
@@ -361,6 +366,27 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
                 add(v1, 3, s);
             }
             if (!ok) break;
+            if constexpr (SPLIT) {
+                // Half h of the columns belongs to the pair of part h. The other pair's sums come into the ring, which both are done with.
+                cluster_sync();
+                met = true;
+                float4 *sums = reinterpret_cast<float4 *>(base) + r;  // [kHalf / 4][kRows]
+                if (h != part) {
+                    const uint32_t to = peer_addr(sums, in_cluster ^ 2u);
+#pragma unroll
+                    for (int j = 0; j < kHalf / 4; ++j)
+                        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + j * kRows * 16), "f"(acc[2 * j].x), "f"(acc[2 * j].y), "f"(acc[2 * j + 1].x),
+                                     "f"(acc[2 * j + 1].y)
+                                     : "memory");
+                }
+                cluster_sync();
+                if (h != part) continue;
+#pragma unroll
+                for (int j = 0; j < kHalf / 4; ++j) {
+                    const float4 o = sums[j * kRows];
+                    acc[2 * j].x += o.x, acc[2 * j].y += o.y, acc[2 * j + 1].x += o.z, acc[2 * j + 1].y += o.w;
+                }
+            }
             const int n_rows = t.n, n_base = t.n0 + h * kHalf;
             const int64_t out_row = row;
             fetch(p + step);
@@ -431,9 +457,11 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
                 }
             }
         }
+        if (SPLIT && !met) cluster_sync(), cluster_sync();  // a half without columns, or an abandoned wait
     }
 
     __syncwarp();
+    if (SPLIT && warp >= kPromoWarps) cluster_sync(), cluster_sync();  // the ring is free (the TMA warp has waited); the sums are across
     tc_fence_before();
     if constexpr (GROUP == 2) cluster_sync();  // nobody's barriers or shared memory go while the peer signals or reads them
     __syncthreads();
@@ -445,22 +473,24 @@ __global__ void __launch_bounds__(kThreads<GROUPED>, 1)
     }
 }
 
-template <int GROUP, bool GROUPED>
+template <int GROUP, bool GROUPED, bool SPLIT>
 int launch(const char *fn, const uint8_t *w, int64_t w_rows, const uint8_t *x, int64_t x_rows, int64_t K, GemmArgs a, int64_t tiles, cudaStream_t st) {
     static thread_local int prepared = -1;
     constexpr size_t smem = smem_bytes<GROUP>();
     int dev = 0;
     SB_CUDA(cudaGetDevice(&dev), fn);
     if (prepared != dev) {
-        SB_CUDA(cudaFuncSetAttribute(fp8_wide_kernel<GROUP, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), fn);
+        SB_CUDA(cudaFuncSetAttribute(fp8_wide_kernel<GROUP, GROUPED, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), fn);
         prepared = dev;
     }
     CUtensorMap wm, xm;
     SB_TRY(make_map(fn, &wm, w, w_rows, K, GROUP == 2 ? 64 : kColTile));
     SB_TRY(make_map(fn, &xm, x, x_rows, K, GROUPED ? 1 : kRows));
     a.NT = (a.N + kColTile - 1) / kColTile;
-    const int64_t all = tiles * a.NT, room = sm_count() / GROUP;
-    SB_CUDA((launch_after(fp8_wide_kernel<GROUP, GROUPED>, dim3((unsigned)(std::min(all, room) * GROUP)), dim3(kThreads<GROUPED>), smem, st, GROUP, wm, xm, a)), fn,
+    const int64_t all = tiles * a.NT;
+    constexpr int kCtas = GROUP * (SPLIT ? 2 : 1);
+    const int64_t clusters = SPLIT ? all : std::min(all, (int64_t)sm_count() / GROUP);  // split: one tile each
+    SB_CUDA((launch_after(fp8_wide_kernel<GROUP, GROUPED, SPLIT>, dim3((unsigned)(clusters * kCtas)), dim3(kThreads<GROUPED>), smem, st, kCtas, wm, xm, a)), fn,
             " (wide) N=", a.N, " K=", K);
     return 0;
 }
@@ -471,11 +501,16 @@ namespace sb {
 namespace fp8 {
 
 int wide_dense(const char *fn, const uint8_t *w, int64_t w_rows, const uint8_t *x, int64_t x_rows, int64_t K, const GemmArgs &a, cudaStream_t st) {
-    return launch<2, false>(fn, w, w_rows, x, x_rows, K, a, ((int64_t)a.M + 2 * kRows - 1) / (2 * kRows), st);
+    const int64_t tiles = ((int64_t)a.M + 2 * kRows - 1) / (2 * kRows);
+    // K over two pairs where that many clusters of four run at once (33 on 148 SMs: 34 of them took twice the time of 33) and K is long
+    // enough to pay for bringing the sums together: [4096, 7168], 256 rows 27.1 -> 19.2 us; [4096, 4096], 512: 19.0 -> 15.7; [8192, 2048], 256:
+    // 12.6 -> 12.7; [4096, 1024], 400: 9.0 -> 10.1.
+    if (a.KB >= 20 && tiles * ((a.N + kColTile - 1) / kColTile) * 9 <= sm_count() * 2) return launch<2, false, true>(fn, w, w_rows, x, x_rows, K, a, tiles, st);
+    return launch<2, false, false>(fn, w, w_rows, x, x_rows, K, a, tiles, st);
 }
 
 int wide_grouped(const char *fn, const uint8_t *w, int64_t w_rows, const uint8_t *x, int64_t x_rows, int64_t K, const GemmArgs &a, cudaStream_t st) {
-    return launch<1, true>(fn, w, w_rows, x, x_rows, K, a, std::min(a.S, a.E + a.S / kRows), st);
+    return launch<1, true, false>(fn, w, w_rows, x, x_rows, K, a, std::min(a.S, a.E + a.S / kRows), st);
 }
 
 unsigned int wide_aborts() {

@@ -225,7 +225,7 @@ def test_swiglu_fp8_nan_stays_in_its_block():
 # ---- the dense product -----------------------------------------------------------------------------------------------
 
 
-@pytest.mark.parametrize("M,N,Kd", [(1, 128, 128), (1, 1, 16), (1, 2048, 4096), (6, 1024, 2048), (16, 100, 144), (17, 129, 1040), (33, 640, 2560), (64, 4096, 512),
+@pytest.mark.parametrize("M,N,Kd", [(600, 1000, 2704), (2400, 300, 2576), (384, 4096, 4096), (1025, 517, 2448), (1, 128, 128), (1, 1, 16), (1, 2048, 4096), (6, 1024, 2048), (16, 100, 144), (17, 129, 1040), (33, 640, 2560), (64, 4096, 512),
                                     (65, 257, 272), (128, 384, 8192), (129, 512, 640), (300, 1000, 1040), (1000, 136, 256), (513, 2048, 1024), (256, 4096, 128)])
 def test_linear_fp8(M, N, Kd):
     g = gen(M + N + Kd)
