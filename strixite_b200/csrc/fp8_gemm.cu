@@ -473,13 +473,13 @@ int grouped(const char *fn, const uint8_t *xq, const float *xs, const strix_fp8v
     a.NT = (int)((N + kTileM - 1) / kTileM);
     // Below 8 slots an expert on average the narrow form, from there on the wide one. Measured (gate/up [1024, 2048] of 64 / 256 experts, us, narrow
     // and wide): mean 4: 22 and 29 / 75 and 83; mean 8: 26 and 31 / 99 and 89; mean 16: 33 and 33 / 142 and 101. Tiles of 32 or 64 slots in the narrow
-    // form were never the fastest. The narrow one, too, while it has no more than one (slot tile, weight tile) pair for each SM: 43 slots of 5
-    // experts [207, 592]: 4.5 and 10.5; 1024 of 8 [256, 512], 144 pairs: 5.9 and 8.1; beyond, 256 of 8 [1024, 2048], 192 pairs: 12.6 and 12.3.
-    // And up to three where rows of y start off a 16-byte boundary, which costs the wide form more: 2055 of 8 [281, 128], 408 pairs: 7.6 and 12.3;
-    // 2895 of 4 [310, 400], 552 pairs: 13.5 and 11.3.
+    // form were never the fastest. The narrow one, too, while it has no more than four (slot tile, weight tile) pairs for three SMs: 43 slots of 5
+    // experts [207, 592]: 4.5 and 10.5; 1024 of 8 [256, 512], 144 pairs: 5.9 and 8.1; 1024 of 32 [256, 2048], 192 pairs: 13.0 and 15.2; beyond,
+    // 512 of 32 [512, 1024], 256 pairs: 9.3 and 8.7. Up to three for each SM where rows of y start off a 16-byte boundary, which costs the wide
+    // form more: 2055 of 8 [281, 128], 408 pairs: 7.6 and 12.3; 2895 of 4 [310, 400], 552 pairs: 13.5 and 11.3.
     const int64_t tiles = std::min(S, E + S / 16);  // at most: every bucket may end in a partial tile
     SB_CHECK(tiles <= 0x7fffffff / a.NT, fn, ": ", S, " slots of N = ", N, " outputs are too many tiles");
-    if (S < 8 * E || tiles * a.NT <= sm_count() * (row_start(y, N, out_act) < 16 ? 3 : 1)) return launch<16, true>(fn, w->q, w->N, xq, rows, w->K, a, tiles, st);
+    if (S < 8 * E || tiles * a.NT * 3 <= (int64_t)sm_count() * (row_start(y, N, out_act) < 16 ? 9 : 4)) return launch<16, true>(fn, w->q, w->N, xq, rows, w->K, a, tiles, st);
     return wide_grouped(fn, w->q, w->N, xq, rows, w->K, a, st);
 }
 

@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(256)
     wait_for_previous();
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= M * N) return;
-    const int64_t m = i / N, n = i - m * N;
+    const int64_t m = M * N <= 0xffffffffll ? (int64_t)((uint32_t)i / (uint32_t)N) : i / N, n = i - m * N;
     bool ok = true;
     float v = 0.f;
     for (int64_t a = 0; a < A; ++a) {
@@ -586,6 +586,12 @@ int combine_reduce(const char *fn, const void *partial, const int32_t *ids, cons
     } else {
         const unsigned blocks = (unsigned)((M * N + 255) / 256);
         const float *pf = static_cast<const float *>(partial);
+        if (early) {
+            SB_CUDA((act == kF32 ? launch_after(combine_reduce_kernel<float>, dim3(blocks), dim3(256), 0, st, 1, pf, ids, coef, M, A, E, N, (float *)y)
+                                 : launch_after(combine_reduce_kernel<uint16_t>, dim3(blocks), dim3(256), 0, st, 1, pf, ids, coef, M, A, E, N, (uint16_t *)y)),
+                    fn, " reduce ", act_name(act), " M=", M, " A=", A, " N=", N);
+            return 0;
+        }
         if (act == kF32) combine_reduce_kernel<float><<<blocks, 256, 0, st>>>(pf, ids, coef, M, A, E, N, (float *)y);
         else combine_reduce_kernel<uint16_t><<<blocks, 256, 0, st>>>(pf, ids, coef, M, A, E, N, (uint16_t *)y);
     }
