@@ -425,13 +425,15 @@ __global__ void __launch_bounds__(kWarps * 32, NV <= 8 ? 7 : 0) router_scored_ke
             const float value = sorted[warp][lane].x, next = sorted[warp][lane + 1].x;
             near = !(value - next > base + 0x1p-22f * (fabsf(value) + fabsf(next)));
         }
-        if (__any_sync(full, near)) {  // by the bound for the largest scores; these two may be small ones
+        if (__any_sync(full, near)) {
+            // That was the bound for the largest scores; two neighbours among the picks may be small ones, and their own errors tell. (Behind the last
+            // pick stand all that are left, with any score: there the bound stays.)
             const float inv = 1.0f / sum;
             auto off = [&](float2 at) {
                 const float l = ld_act(row, __float_as_int(at.y));
                 return (a.score == kSigmoid ? 0x1p-20f * fast_sigmoid(l) : 0x1p-16f * (expf(l - top) * inv)) + 0x1p-22f * fabsf(at.x) + 0x1p-120f;
             };
-            if (near) near = !(sorted[warp][lane].x - sorted[warp][lane + 1].x > off(sorted[warp][lane]) + off(sorted[warp][lane + 1]));
+            if (near && lane + 1 < a.k) near = !(sorted[warp][lane].x - sorted[warp][lane + 1].x > off(sorted[warp][lane]) + off(sorted[warp][lane + 1]));
         }
         if (__any_sync(full, near)) {
             // the candidates once more, in 64 bits
