@@ -625,7 +625,8 @@ def moe_router_scored(logits, ld, M, E, k, score, bias, n_group, topk_group, gro
             continue
         if t is None or t.get_device() != dev or t.dtype not in dt:
             raise StrixError("%s: %s must be a %s tensor on the current device cuda:%d" % (fn, name, dt[0], dev))
-        if t.untyped_storage().nbytes() // t.element_size() - t.storage_offset() < (M - 1) * stride + last:
+        need = (M - 1) * stride + last
+        if not (t.is_contiguous() and t.numel() >= need) and t.untyped_storage().nbytes() // t.element_size() - t.storage_offset() < need:
             raise StrixError("%s: %s ends before the last of %d rows, %d apart" % (fn, name, M, stride))
     _ok(lib.strix_moe_router_scored(logits.data_ptr(), ld, M, E, k, how, _t(fn, "bias", bias, _F32, E, dev, True), n_group, topk_group, group_top, 1 if renorm else 0,
          route_scale, None if shared_logit is None else shared_logit.data_ptr(), shared_ld, shared_id, _t(fn, "ids", ids, _I32, M * A, dev),
