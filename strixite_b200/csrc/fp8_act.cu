@@ -118,38 +118,36 @@ struct RowOf {
 };
 
 // Eight lanes per (row, 128-column block) of h = silu(gate) * up, 16 elements a thread. Gate and up stay FP32 until the one rounding
-// to e4m3. FP32 rows are bound by memory (40960 x 512: 28.6 us, 6.6 TB/s), BF16 rows by the instructions issued (21.9 us, 4.8 TB/s; with
-// 8 elements a thread, whose index, maximum and scale cost as much as those of 16: 25.1 us, and with scalar arithmetic 26.5).
-constexpr int kSwigluThreads = 256, kSwigluUnits = kSwigluThreads / 8;  // of a block
+// to e4m3. FP32 rows are bound by memory (40960 x 512: 28.5 us, 6.6 TB/s), BF16 rows by the instructions issued (20.0 us, 5.3 TB/s; with
+// 8 elements a thread, whose index, maximum and scale cost as much as those of 16: 25.1 us, and with scalar arithmetic 26.5). Small
+// blocks, as many as there is work: 256 threads and blocks that stay for several units: 21.9 us.
+constexpr int kSwigluThreads = 128, kSwigluUnits = kSwigluThreads / 8;  // of a block
 template <typename T>
-__global__ void __launch_bounds__(kSwigluThreads, 4) swiglu_fp8_kernel(const T *gu, uint8_t *q, float *scale, int64_t rows, int I, int blocks, RowOf row_of) {
+__global__ void __launch_bounds__(kSwigluThreads, 8) swiglu_fp8_kernel(const T *gu, uint8_t *q, float *scale, int64_t units, int I, int blocks, RowOf row_of) {
     let_next_begin();
     wait_for_previous();
-    const int64_t units = rows * blocks, stride = (int64_t)gridDim.x * kSwigluUnits;
     const int t = threadIdx.x & 7;
-    for (int64_t u0 = (int64_t)blockIdx.x * kSwigluUnits; u0 < units; u0 += stride) {
-        const int64_t u = u0 + threadIdx.x / 8;
-        const int64_t row = row_of.mul != 0 ? (int64_t)((uint64_t)(uint32_t)u * row_of.mul >> row_of.shift) : u / blocks;
-        const int b = (int)(u - row * blocks), c = b * kFp8Block + t * 16;
-        const bool live = u < units && c < I;  // I % 16 == 0
-        Block8 h[2];
-        float top = 0.f;
-        if (live) {
-            const T *gate = gu + row * 2 * I + c, *up = gate + I;
-            float g[2][8], v[2][8];
-            load8(gate, g[0]), load8(gate + 8, g[1]);
-            load8(up, v[0]), load8(up + 8, v[1]);
-            swiglu8(g[0], v[0], h[0]), swiglu8(g[1], v[1], h[1]);
-            top = max_abs(max_abs8(h[0].hi), max_abs8(h[1].hi));
-        }
-        top = lanes_max<8>(top);
-        if (live) {
-            float s;
-            uint2 codes[2];
-            fp8_pack(h, top, 1.0f, s, codes);
-            *reinterpret_cast<uint4 *>(q + row * I + c) = make_uint4(codes[0].x, codes[0].y, codes[1].x, codes[1].y);
-            if (t == 0) scale[u] = s;
-        }
+    const int64_t u = (int64_t)blockIdx.x * kSwigluUnits + threadIdx.x / 8;
+    const int64_t row = row_of.mul != 0 ? (int64_t)((uint64_t)(uint32_t)u * row_of.mul >> row_of.shift) : u / blocks;
+    const int b = (int)(u - row * blocks), c = b * kFp8Block + t * 16;
+    const bool live = u < units && c < I;  // I % 16 == 0
+    Block8 h[2];
+    float top = 0.f;
+    if (live) {
+        const T *gate = gu + row * 2 * I + c, *up = gate + I;
+        float g[2][8], v[2][8];
+        load8(gate, g[0]), load8(gate + 8, g[1]);
+        load8(up, v[0]), load8(up + 8, v[1]);
+        swiglu8(g[0], v[0], h[0]), swiglu8(g[1], v[1], h[1]);
+        top = max_abs(max_abs8(h[0].hi), max_abs8(h[1].hi));
+    }
+    top = lanes_max<8>(top);
+    if (live) {
+        float s;
+        uint2 codes[2];
+        fp8_pack(h, top, 1.0f, s, codes);
+        *reinterpret_cast<uint4 *>(q + row * I + c) = make_uint4(codes[0].x, codes[0].y, codes[1].x, codes[1].y);
+        if (t == 0) scale[u] = s;
     }
 }
 
@@ -205,18 +203,19 @@ int strix_swiglu_fp8(const void *gu, uint8_t *q, float *scale, int64_t rows, int
     SB_CHECK(apart(q, qb, gu, gb) && apart(scale, sb_, gu, gb) && apart(q, qb, scale, sb_), fn, ": q [", (const void *)q, "], scale [", (const void *)scale,
              "] and gu [", gu, "] overlap");
     const int blocks = (int)fp8_blocks(I);
-    const int64_t units = rows * blocks, want = (units + kSwigluUnits - 1) / kSwigluUnits, cap = (int64_t)sm_count() * 32;
-    const unsigned grid = (unsigned)(want < cap ? want : cap);
+    const int64_t units = rows * blocks;  // at most 2^35
+    const unsigned grid = (unsigned)((units + kSwigluUnits - 1) / kSwigluUnits);
+    SB_CHECK((units + kSwigluUnits - 1) / kSwigluUnits <= 0x7fffffff, fn, ": ", rows, " rows of ", blocks, " blocks are too many");
     auto st = static_cast<cudaStream_t>(stream);
     RowOf row_of{0, 0};
-    if (units + cap * kSwigluUnits < (1ll << 31)) {
+    if (units + kSwigluUnits < (1ll << 31)) {
         int log = 0;
         while ((1 << log) < blocks) ++log;
         row_of.shift = 31 + log;
         row_of.mul = (uint32_t)(((1ull << row_of.shift) + blocks - 1) / blocks);
     }
-    SB_CUDA((act == kF32 ? launch_after(swiglu_fp8_kernel<float>, dim3(grid), dim3(kSwigluThreads), 0, st, 1, (const float *)gu, q, scale, rows, (int)I, blocks, row_of)
-                         : launch_after(swiglu_fp8_kernel<uint16_t>, dim3(grid), dim3(kSwigluThreads), 0, st, 1, (const uint16_t *)gu, q, scale, rows, (int)I, blocks, row_of)),
+    SB_CUDA((act == kF32 ? launch_after(swiglu_fp8_kernel<float>, dim3(grid), dim3(kSwigluThreads), 0, st, 1, (const float *)gu, q, scale, units, (int)I, blocks, row_of)
+                         : launch_after(swiglu_fp8_kernel<uint16_t>, dim3(grid), dim3(kSwigluThreads), 0, st, 1, (const uint16_t *)gu, q, scale, units, (int)I, blocks, row_of)),
             fn, " ", act_name(act), " rows=", rows, " I=", I);
     return 0;
 }
