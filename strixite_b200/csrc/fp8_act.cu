@@ -118,12 +118,12 @@ struct RowOf {
 };
 
 // Eight lanes per (row, 128-column block) of h = silu(gate) * up, 16 elements a thread. Gate and up stay FP32 until the one rounding
-// to e4m3. FP32 rows are bound by memory (40960 x 512: 28.5 us, 6.6 TB/s), BF16 rows by the instructions issued (20.0 us, 5.3 TB/s; with
+// to e4m3. FP32 rows are bound by memory (40960 x 512: 28.5 us, 6.6 TB/s), BF16 rows by the instructions issued (19.4 us, 5.4 TB/s; with
 // 8 elements a thread, whose index, maximum and scale cost as much as those of 16: 25.1 us, and with scalar arithmetic 26.5). Small
-// blocks, as many as there is work: 256 threads and blocks that stay for several units: 21.9 us.
+// blocks, as many as there is work: 256 threads and blocks that stay for several units: 21.9 us; with 8 blocks an SM for BF16: 20.0.
 constexpr int kSwigluThreads = 128, kSwigluUnits = kSwigluThreads / 8;  // of a block
 template <typename T>
-__global__ void __launch_bounds__(kSwigluThreads, 8) swiglu_fp8_kernel(const T *gu, uint8_t *q, float *scale, int64_t units, int I, int blocks, RowOf row_of) {
+__global__ void __launch_bounds__(kSwigluThreads, sizeof(T) == 2 ? 10 : 8) swiglu_fp8_kernel(const T *gu, uint8_t *q, float *scale, int64_t units, int I, int blocks, RowOf row_of) {
     let_next_begin();
     wait_for_previous();
     const int t = threadIdx.x & 7;
