@@ -20,7 +20,7 @@ namespace {
 
 using namespace sb;
 
-constexpr int kWarps = 4;        // tokens per block
+constexpr int kWarps = 2;        // tokens per block (16384 x 512 with 1, 2, 4, 8: 23.3, 22.5, 23.5, 23.2 us; 4097 x 160: 7.0, 5.3, 5.3, 9.8)
 constexpr int kMaxCand = 256;    // candidates a token may have in the FP32 path
 constexpr int64_t kMaxExperts = 1024, kMaxTopK = 32, kMaxGroups = 32;
 enum Score : int { kSoftmax = 0, kSigmoid = 1 };
@@ -162,7 +162,7 @@ __device__ __forceinline__ float4 load4(const uint16_t *p) {
 // The choice: the k-th largest lane maximum bounds the k-th largest value from below, what reaches it are the candidates (about 1.3 k of
 // them), they meet in shared memory and each counts those in front of it: no k rounds of warp-wide maxima. Where neighbours in that
 // order are closer than the error, the candidates are valued again in 64 bits (one token in a thousand).
-// Bound by the instructions issued: 16384 x 512 experts, 10 of 4 of 8 groups, 23.4 us, of which the loads are 4.9, scores 2.9, groups
+// Bound by the instructions issued: 16384 x 512 experts, 10 of 4 of 8 groups, 22.5 us, of which the loads are 4.9, scores 2.9, groups
 // 3.5, candidates and their order 7, the last step 4.
 //
 // The FP32 errors that the choice allows for (documented bounds: expf 2 ulp; ex2.approx 2^-22, rcp.approx 2^-23 relative):
@@ -190,7 +190,7 @@ struct PerToken {
 };
 
 template <typename T, int NV, bool VEC>
-__global__ void __launch_bounds__(kWarps * 32, NV <= 8 ? 7 : 0) router_scored_kernel(const T *logits, const T *shared, const RouteArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, NV <= 8 ? 14 : 0) router_scored_kernel(const T *logits, const T *shared, const RouteArgs a) {
     __shared__ PerToken tokens[kWarps];
     __shared__ float2 sorted[kWarps][40];
     const unsigned full = 0xffffffffu;
@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(kWarps * 32, NV <= 8 ? 7 : 0) router_scored_ke
         if (many * 4 < a.k * 5 && many < 32 && a.topk_group * a.per > 32) {
             // Few lanes are open and hold the experts of all: these are dealt anew, to every lane its share, or the bound would let most of them
             // in (16384 tokens: 16 picks of 512 experts in 16 open lanes 68 -> 27 us, of 256 in 8 lanes 185 -> 46; below the rule, 6 of 64 in
-            // 8 lanes, 17.1 -> 17.0, 10 of 256 in 16 lanes 23.4 -> 24.6).
+            // 8 lanes, 17.1 -> 17.0, 10 of 256 in 16 lanes 23.4 -> 24.6 us).
             const int total = min(many * ((a.per + L - 1) >> a.log_L), kMaxCand * 4);  // what is not dealt only lowers the bound
             int at = __popc(lanes & ((1u << lane) - 1));
 #pragma unroll
