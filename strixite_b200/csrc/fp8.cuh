@@ -67,16 +67,16 @@ __device__ __forceinline__ Pair2 fma2(Pair2 a, Pair2 b, Pair2 c) {
 }
 
 // The 8 N values (times `unit`, a factor that the block shares) as e4m3 bytes of v / scale, scale = max(amax * unit, 2^-100) / 448: the largest
-// magnitude gets the largest e4m3 value, and a block of zeros has a scale that divides. A NaN stays one. The quotient is taken against the unrounded block maximum, in which the unit cancels: 448 / amax as two floats, three FMAs a value.
+// magnitude (amax + amax_lo, unrounded) gets the largest e4m3 value, and a block of zeros has a scale that divides. A NaN stays one. The quotient is taken against the unrounded block maximum, in which the unit cancels: 448 / amax as two floats, three FMAs a value.
 template <int N>
-__device__ __forceinline__ void fp8_pack(const Block8 (&v)[N], float amax, float unit, float &scale, uint2 (&codes)[N]) {
+__device__ __forceinline__ void fp8_pack(const Block8 (&v)[N], float amax, float amax_lo, float unit, float &scale, uint2 (&codes)[N]) {
     const float top = amax * unit;
     if (top >= 0x1p-100f && amax > 0x1p-60f && amax < 0x1p60f) {
         const float s = top * (1.0f / 448.0f);
         scale = fmaf(fmaf(-s, 448.0f, top), 1.0f / 448.0f, s);
         float r = fast_rcp(amax);
         r = fmaf(fmaf(-r, amax, 1.0f), r, r);
-        const float inv = 448.0f * r, rest = fmaf(-inv, amax, 448.0f) * r;  // 448 / amax = inv + rest
+        const float inv = 448.0f * r, rest = fmaf(-inv, amax_lo, fmaf(-inv, amax, 448.0f)) * r;  // 448 / (amax + amax_lo) = inv + rest
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             uint32_t h[4];
