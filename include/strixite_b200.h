@@ -289,7 +289,8 @@ int strix_linear_qmix_experts_combine_grouped(const void *h, const strix_qmix_vi
 /* The grouped pair in 8-bit floating point (strix_fp8view stacks of E experts): gather y[slot, :] = W[ids[slot]] * row slot / A of
  * the FP8 rows xq [M, K], xs, in slot order [M * A, N]; combine partial[slot, :] = W[ids[slot]] * FP8 row slot of hq [M * A, K], hs,
  * then y[m, :] = sum over a ascending of coef * partial, one rounding. Slots with an invalid id keep their rows of y (gather) and make
- * their token's row NaN (combine). ws: moe_group_routes of the same ids. partial: M * A * N floats. K % 16 == 0, any N.
+ * their token's row NaN (combine). ws: moe_group_routes of the same ids; with one grouped for other sizes nothing is stored and
+ * strix_workspace_refusal_count goes up. partial: M * A * N floats. K % 16 == 0, any N.
  * No counterpart in the reference. */
 int strix_linear_fp8_experts_gather_grouped(const uint8_t *xq, const float *xs, const strix_fp8view *w, int64_t E, const void *ws,
                                             size_t ws_bytes, int64_t M, int64_t A, void *y, int out_act, void *stream);

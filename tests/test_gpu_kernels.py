@@ -418,3 +418,26 @@ def test_grouped_tensor_cores_bad_id_and_k_check():
     with pytest.raises(StrixError, match="multiple of 64"):
         K.linear_q4_experts_gather_grouped(torch.zeros((M, 96), dtype=torch.bfloat16, device="cuda"), upload_stack(st32), E, ws, nbytes, M, A,
                                            torch.zeros((M, A, 64), dtype=torch.bfloat16, device="cuda"), K.Act.BF16, K.MoeMath.WmmaBf16)
+
+
+def test_grouped_combine_refuses_a_workspace_grouped_for_other_sizes():
+    """The refusal above for the combine entries: the partial sums and y stay as they are."""
+    rng = np.random.default_rng(29)
+    I, d, E, M, A = 128, 64, 20, 12, 4
+    nbytes = K.moe_route_workspace_bytes(16, 4, 16)
+    ids = np.stack([rng.permutation(16)[:4] for _ in range(16)]).astype(np.int32)
+    ws, err = torch.empty(nbytes // 4, dtype=torch.int32, device="cuda"), dev_err()
+    K.moe_group_routes(torch.from_numpy(ids).cuda(), 16, 4, 16, ws, nbytes, err)
+    w = upload_stack(make_stack(rng, E, d, I, 32))
+    idt, coef = torch.from_numpy(ids[:M]).cuda(), torch.ones((M, A), device="cuda")
+    for act in ACTS:
+        h = to_torch_act(randn_act(rng, (M * A, I), act))
+        for math in (K.MoeMath.F32, K.MoeMath.WmmaF16):
+            partial, y = torch.full((M * A, d), 5.0, device="cuda"), torch.full((M, d), 7.0, dtype=K._dtype(act), device="cuda")
+            before = K.workspace_refusal_count()
+            K.linear_q4_experts_combine_grouped(h, w, E, idt, coef, ws, nbytes, partial, M, A, y, act, math)
+            torch.cuda.synchronize()
+            assert bool((y == 7.0).all()) and bool((partial == 5.0).all()) and K.workspace_refusal_count() == before + 1
+            K.linear_q4_experts_combine_grouped_fixed(h, w, E, idt, coef, ws, nbytes, M, A, y, act, math)
+            torch.cuda.synchronize()
+            assert bool((y == 7.0).all()) and K.workspace_refusal_count() == before + 2
