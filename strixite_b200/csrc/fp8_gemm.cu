@@ -536,6 +536,7 @@ int strix_linear_fp8_experts_combine_grouped(const uint8_t *hq, const float *hs,
     SB_CHECK(reinterpret_cast<uintptr_t>(ids) % 4 == 0 && reinterpret_cast<uintptr_t>(coef) % 4 == 0, fn, ": ids ", (const void *)ids, " and coef ",
              (const void *)coef, " must be 4-byte aligned");
     SB_CHECK(act_ok(act), fn, ": unsupported activation dtype ", act);
+    SB_CHECK(reinterpret_cast<uintptr_t>(y) % act_size(act) == 0, fn, ": y ", y, " must be aligned to its elements");
     SB_CHECK(M >= 1 && A >= 1 && A <= 64 && M <= (1 << 20) && M * A <= (1 << 20), fn, ": M = ", M, ", A = ", A, " (A <= 64, M * A <= 2^20)");
     SB_TRY(check_view(fn, w));
     SB_CHECK(E >= 1 && E <= kMaxE && w->N % E == 0, fn, ": weight has ", w->N, " rows for E = ", E, " experts (E must be 1..1023 and divide the rows)");

@@ -161,3 +161,11 @@ def test_weight_object():
                 lambda: Fp8Weight(q, s, experts=3), lambda: Fp8Weight(q, s, experts=0), lambda: Fp8Weight(q.view(-1), s)):
         with pytest.raises(StrixError):
             bad()
+
+
+@pytest.mark.parametrize("act,off", ((0, 2), (0, 1), (1, 1)))
+def test_combine_refuses_an_output_off_its_elements(mem, act, off):
+    v = Fp8View(mem(4).value, mem(5).value, 8 * 64, 256)
+    need = lib.strix_moe_route_workspace_bytes(4, 2, 8)
+    y = C.c_void_p(mem(3).value + off)
+    refused(lib.strix_linear_fp8_experts_combine_grouped(mem(0), mem(1), C.byref(v), 8, mem(6), mem(7), mem(2), need, mem(8), 4, 2, y, act, None), "aligned to its elements")
