@@ -529,6 +529,11 @@ int strix_moe_router_scored(const void *logits, int64_t ld, int64_t M, int64_t E
         SB_CHECK(shared_id >= 0, fn, ": shared_id = ", shared_id, ", expected >= 0 (its expert row block)");
     }
     SB_CHECK(act_ok(act), fn, ": unsupported activation dtype ", act);
+    auto off = [](const void *p, int64_t size) { return reinterpret_cast<uintptr_t>(p) % size != 0; };
+    SB_CHECK(!off(logits, act_size(act)) && !off(shared_logit, act_size(act)), fn, ": logits ", logits, " and shared_logit ", shared_logit,
+             " must be aligned to their elements");
+    SB_CHECK(!off(bias, 4) && !off(ids, 4) && !off(coef, 4) && !off(err, 4), fn, ": bias ", (const void *)bias, ", ids ", (const void *)ids, ", coef ",
+             (const void *)coef, " and err ", (const void *)err, " must be aligned to 4 bytes");
     const int64_t A = k + (shared_logit != nullptr ? 1 : 0), ob = M * A * 4;
     SB_CHECK(apart(ids, ob, coef, ob), fn, ": ids [", (const void *)ids, "] and coef [", (const void *)coef, "] (", ob, " B each) overlap");
     const int64_t lb = ((M - 1) * ld + E) * act_size(act);

@@ -169,3 +169,10 @@ def test_combine_refuses_an_output_off_its_elements(mem, act, off):
     need = lib.strix_moe_route_workspace_bytes(4, 2, 8)
     y = C.c_void_p(mem(3).value + off)
     refused(lib.strix_linear_fp8_experts_combine_grouped(mem(0), mem(1), C.byref(v), 8, mem(6), mem(7), mem(2), need, mem(8), 4, 2, y, act, None), "aligned to its elements")
+
+
+@pytest.mark.parametrize("act,which,off", ((0, "logits", 2), (1, "logits", 1), (0, "shared", 2), (1, "shared", 1), (0, "bias", 2), (0, "ids", 2), (1, "coef", 1), (1, "err", 2)))
+def test_router_scored_refuses_pointers_off_their_elements(mem, act, which, off):
+    p = {n: mem(i) for i, n in enumerate(("logits", "shared", "bias", "ids", "coef", "err"))}
+    p[which] = C.c_void_p(p[which].value + off)
+    refused(lib.strix_moe_router_scored(p["logits"], 64, 4, 64, 8, 1, p["bias"], 8, 4, 2, 1, 1.0, p["shared"], 1, 64, p["ids"], p["coef"], act, p["err"], None), "aligned to")
