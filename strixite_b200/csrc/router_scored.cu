@@ -168,6 +168,8 @@ __device__ __forceinline__ float4 load4(const uint16_t *p) {
 // The FP32 errors that the choice allows for (documented bounds: expf 2 ulp; ex2.approx 2^-22, rcp.approx 2^-23 relative):
 //   sigmoid  e = 2^(-l log2 e): the argument's roundings move e by 1.5 |l| 2^-24, so p by p (1 - p) (2^-22 + 1.5 |l| 2^-24) <= 0.7 * 2^-23; 1 + e
 //            and the reciprocal by 1.5 * 2^-23: 2.2 * 2^-23, for two values 4.4 * 2^-23 < 2^-20
+//            relative to p itself the factor 1 - p no longer helps where l is negative: (7 + 1.5 |l|) 2^-24 < 2^-20 + 2^-23 |l|; for
+//            l > 0, (1 - p) l < 0.28: 7.5 * 2^-24 < 2^-20
 //   softmax  e = expf(l - top): (2 + |x| / 2) 2^-23 of e; the sum of up to 64 a lane and 5 steps: 35 * 2^-23 and the terms' mean, at most
 //            2 + ln(1024) / 2; p by at most 45 * 2^-23 of the largest p, for two values 90 * 2^-23 < 2^-16
 //            relative to p itself: its exponential's error with |x| < 88 and the sum's, below 2^-16 p
@@ -431,7 +433,7 @@ __global__ void __launch_bounds__(kWarps * 32, NV <= 8 ? 14 : 0) router_scored_k
             const float inv = 1.0f / sum;
             auto off = [&](float2 at) {
                 const float l = ld_act(row, __float_as_int(at.y));
-                return (a.score == kSigmoid ? 0x1p-20f * fast_sigmoid(l) : 0x1p-16f * (expf(l - top) * inv)) + 0x1p-22f * fabsf(at.x) + 0x1p-120f;
+                return (a.score == kSigmoid ? (0x1p-20f + 0x1p-23f * fmaxf(-l, 0.f)) * fast_sigmoid(l) : 0x1p-16f * (expf(l - top) * inv)) + 0x1p-22f * fabsf(at.x) + 0x1p-120f;
             };
             if (near && lane + 1 < a.k) near = !(sorted[warp][lane].x - sorted[warp][lane + 1].x > off(sorted[warp][lane]) + off(sorted[warp][lane + 1]));
         }

@@ -3,11 +3,36 @@ rows, tiles and K blocks end off every boundary."""
 import pytest
 import torch
 
-from fp8_ref import rows_fp8, stack_fp8
+from fp8_ref import route, rows_fp8, stack_fp8
 from strixite_b200 import kernels as K
-from test_gpu_fp8 import ACTS, DT, gen, group, rand, some_ids
+from test_gpu_fp8 import ACTS, DT, gen, group, rand, run_route, some_ids
 
 pytestmark = pytest.mark.gpu
+
+
+# ---- routing ---------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("score", ("softmax", "sigmoid"))
+def test_route_small_scores_beside_biases_of_their_size(score):
+    """Two experts whose scores lie far below 1, one with a bias that brings its sum within a few steps of FP32 of the other's: the order of
+    64 bits. As many picks as experts, so that none behind the last pick asks for 64 bits, and one such pair a token, so that no
+    other pair does."""
+    r = torch.Generator().manual_seed(7)
+    wrong = []
+    for _ in range(1000):
+        u = torch.rand(3, generator=r, dtype=torch.float64)
+        a = -(25 + 54 * u[0])
+        l = torch.tensor([a, a - 6 * u[1], 0.0]).float().view(1, 3)[:, : 3 if score == "softmax" else 2]  # softmax: the scores are the exponentials
+        E = l.shape[1]
+        p = torch.sigmoid(l.double()) if score == "sigmoid" else torch.softmax(l.double(), 1)
+        bias = torch.zeros(E)
+        bias[1] = (p[0, 0] - p[0, 1] + (u[2] * 128 - 64) * 2.0**-24 * p[0, 0]).float()
+        want, cw = route(l, E, score, bias, 1, 1, 1, True, 1.0)
+        ids, coef, err = run_route(l.cuda(), E, score, bias.cuda(), 1, 1, 1, True, 1.0, K.Act.F32)
+        if not torch.equal(ids.cpu(), want):
+            wrong.append(float(a))
+    assert not wrong, "%d of 1000 tokens in another order, scores e^%s" % (len(wrong), wrong[:8])
 
 
 # ---- products --------------------------------------------------------------------------------------------------------
