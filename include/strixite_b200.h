@@ -168,8 +168,8 @@ int strix_swiglu_fp8(const void *gu, uint8_t *q, float *scale, int64_t rows, int
 /* The norm in front of the layer with the residual's addition: x_out = x + y rounded to act (y and x_out NULL: x as it is; x_out may be
  * x or y), h = x_out * g / sqrt(mean(x_out^2) + eps) from the stored values, g = w (FP32 [d]) or 1 + w when centered. h [M, d] in the
  * activation dtype (or NULL), and the unrounded h as FP8 rows q, scale as strix_swiglu_fp8 makes them (or both NULL). A NaN makes its
- * whole row NaN; an infinity (or an FP32 sum of squares that overflows to one) makes h 0, and NaN where x_out is infinite; a block with
- * a NaN is NaN in every code and in its scale; a row of zeros with eps 0 is 0 * inf = NaN. d % 16 == 0, d <= 16384. No counterpart in the reference's MoE path. */
+ * whole row NaN; an infinity makes h 0, and NaN where x_out is infinite (finite rows have their norm, also where the squares leave FP32's
+ * range); a block with a NaN is NaN in every code and in its scale; a row of zeros with eps 0 is 0 * inf = NaN. d % 16 == 0, d <= 16384. No counterpart in the reference's MoE path. */
 int strix_residual_rmsnorm_fp8(const void *x, const void *y, const float *w, int centered, float eps, int64_t M, int64_t d,
                                void *x_out, void *h, uint8_t *q, float *scale, int act, void *stream);
 /* strixite kernels/residual.hpp:17 residual_add. */

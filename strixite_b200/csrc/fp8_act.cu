@@ -11,6 +11,18 @@ using namespace sb;
 constexpr int kNormMaxThreads = 256;
 constexpr int kNormMaxVec = 8;  // 8-element pieces a thread can hold: d <= 256 * 8 * 8
 
+// The warps' values (each the same in all lanes of a warp) folded in the order of the warps; what stood in `part` has been read by then.
+template <typename F>
+__device__ __forceinline__ float block_fold(float *part, float v, F f) {
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float all = part[0];
+#pragma unroll 1
+    for (int i = 1; i < (int)blockDim.x / 32; ++i) all = f(all, part[i]);
+    return all;
+}
+
 // One block per row; a thread holds VEC pieces of 8 consecutive elements in registers, so a row is read once whatever its
 // length: x' = x + y rounded to the activation type (what the residual stream keeps), r = 1 / sqrt(mean(x'^2) + eps) from the stored
 // values, h = x' r g. 16 neighbouring threads hold one 128-column block: its largest magnitude is a half-warp reduction.
@@ -57,9 +69,30 @@ __global__ void __launch_bounds__(kNormMaxThreads)
     const float mean = fmaf(total, inv_d, eps);
     float r;
     asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(mean));
-    if (mean > 0x1p-100f && mean < 0x1p100f) r = fmaf(r * 0.5f, fmaf(-mean * r, r, 1.0f), r);
-    else r = 1.0f / sqrtf(mean);
-    const bool plain = !(r > 0x1p-60f && r < 0x1p60f);  // a row near FP32's ends (or with an infinity, a NaN): h first, then its codes
+    if (mean > 0x1p-100f && mean < 0x1p100f) {
+        r = fmaf(r * 0.5f, fmaf(-mean * r, r, 1.0f), r);
+    } else {
+        // The squares may have left FP32's range or lost their low bits below it; the norm itself is an ordinary number. Once more on the row
+        // (and sqrt(eps)) times a power of two that brings the largest to 2^30, or as near as a float gets it: exact (but where h is
+        // below 2^-150), and h stays. (Costs other rows 0.1 us at 1001 x 2560 FP32, nothing measurable at the large sizes.)
+        float top = sqrtf(eps);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) top = max_abs(top, max_abs8(v[i]));
+        top = block_fold(part, lanes_max<32>(top), [](float a, float b) { return max_abs(a, b); });
+        if (top > 0.f && top < INFINITY) {
+            const float s = __int_as_float((min(127, 157 - (__float_as_int(top) >> 23)) + 127) << 23);
+            sq = 0.f;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] *= s, sq = fmaf(v[i][j], v[i][j], sq);
+            total = block_fold(part, warp_sum(sq), [](float a, float b) { return a + b; });
+            r = 1.0f / sqrtf(fmaf(total, inv_d, eps * s * s));
+        } else {
+            r = 1.0f / sqrtf(mean);
+        }
+    }
+    const bool plain = !(r > 0x1p-60f && r < 0x1p60f);  // a row with an infinity or a NaN, or of zeros with eps 0: h first, then its codes
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
         const int c = (threadIdx.x + i * blockDim.x) * 8;

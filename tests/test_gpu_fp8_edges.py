@@ -3,7 +3,7 @@ rows, tiles and K blocks end off every boundary."""
 import pytest
 import torch
 
-from fp8_ref import route, rows_fp8, stack_fp8
+from fp8_ref import FP8, blocks, check_fp8_rows, route, rows_fp8, stack_fp8
 from strixite_b200 import kernels as K
 from test_gpu_fp8 import ACTS, DT, gen, group, rand, run_route, some_ids
 
@@ -33,6 +33,50 @@ def test_route_small_scores_beside_biases_of_their_size(score):
         if not torch.equal(ids.cpu(), want):
             wrong.append(float(a))
     assert not wrong, "%d of 1000 tokens in another order, scores e^%s" % (len(wrong), wrong[:8])
+
+
+# ---- norm and SwiGLU -------------------------------------------------------------------------------------------------
+
+# Sum of squares, root and products as in the norm's own test, and eps scaled twice (two roundings of its share of the mean, halved by the root).
+NORM_REL = (77 / 2 + 7) * 2.0**-24
+
+
+def check_norm(x, eps, act, d):
+    M = x.shape[0]
+    w = rand(gen(d), d) * 0.1 + 1
+    f = x.double()
+    h64 = f / torch.sqrt(f.pow(2).mean(1, keepdim=True) + eps) * w.double()
+    h, q, s = torch.empty_like(x), torch.empty((M, d), dtype=FP8, device="cuda"), torch.empty((M, blocks(d)), device="cuda")
+    K.residual_rmsnorm_fp8(x, None, w, M, d, eps, None, h, q, s, act)
+    tol = h64.abs() * (NORM_REL + (2.0**-8 if act == K.Act.BF16 else 0)) + 1e-37
+    for m in range(M):
+        assert ((h[m].double() - h64[m]).abs() <= tol[m]).all(), "row %d is off by up to %g of itself" % (m, ((h[m].double() - h64[m]).abs() / h64[m].abs()).max())
+    check_fp8_rows(q, s, h64, NORM_REL)
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("d", (16, 512, 2560, 8192))
+def test_rmsnorm_fp8_rows_near_the_ends_of_fp32(act, d):
+    """Rows whose squares leave FP32's range, or its normal range, on either side: their norm is an ordinary number."""
+    g = gen(d)
+    powers = (0, -45, -62, -64, -70, -90, -115, 45, 58, 62, 64, 90, 120)
+    x = torch.stack([rand(g, d) * 2.0**p for p in powers]).to(DT[act])
+    check_norm(x, 0.0, act, d)
+    tiny = x[1:7].contiguous()
+    for eps in (2.0**-90, 2.0**-128, 2.0**-140, 2.0**-149):  # above, near and below the squares' mean
+        check_norm(tiny, eps, act, d)
+    check_norm(x[6:].contiguous(), 1e-6, act, d)
+    check_norm(x, 1e30, act, d)
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_rmsnorm_fp8_one_value_far_above_the_rest(act):
+    d = 1024
+    x = rand(gen(1), 4, d).to(DT[act])
+    x[1, 700], x[2, 5] = 2.0**70, -(2.0**100)
+    x[3] *= 2.0**-60
+    x[3, 3] = 2.0**-20
+    check_norm(x, 0.0, act, d)
 
 
 # ---- products --------------------------------------------------------------------------------------------------------
