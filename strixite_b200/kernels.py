@@ -55,7 +55,9 @@ def _s(stream):
     return C.c_void_p(_raw(stream, torch.cuda.current_device()))
 
 
-_current_raw = torch._C._cuda_getCurrentRawStream  # the stream's handle without a Stream object: 0.1 instead of 1 us a call
+# The stream's handle without a Stream object, the device's number without its Python: 0.1 instead of 1 us a call. A torch without CUDA has neither.
+_current_raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _raw(stream, device):
@@ -513,9 +515,6 @@ def linear_qw_experts_combine_grouped(h, w, E, ids, coef, ws, ws_bytes, partial,
 # ---- 8-bit floating point (e4m3, a scale per block of 128) ------------------------------------------------------------
 # No counterpart in the reference. These wrappers look at dtype, size and device of every tensor, because a byte matrix of the wrong
 # shape has no other sign of it; a tensor of another device than the current one is refused (the launch goes to the current one).
-
-
-_device = torch._C._cuda_getDevice  # torch.cuda.current_device() without its Python
 
 
 def _ok(rc):

@@ -176,3 +176,19 @@ def test_router_scored_refuses_pointers_off_their_elements(mem, act, which, off)
     p = {n: mem(i) for i, n in enumerate(("logits", "shared", "bias", "ids", "coef", "err"))}
     p[which] = C.c_void_p(p[which].value + off)
     refused(lib.strix_moe_router_scored(p["logits"], 64, 4, 64, 8, 1, p["bias"], 8, 4, 2, 1, 1.0, p["shared"], 1, 64, p["ids"], p["coef"], act, p["err"], None), "aligned to")
+
+
+def test_the_package_imports_where_torch_has_no_cuda_calls():
+    """A torch built without CUDA lacks these names; the quantizers, views and refusals work there."""
+    import os
+    import subprocess
+    import sys
+
+    code = ("import torch\n"
+            "for n in ('_cuda_getCurrentRawStream', '_cuda_getDevice'):\n"
+            "    if hasattr(torch._C, n): delattr(torch._C, n)\n"
+            "from strixite_b200 import Fp8Weight, kernels as K\n"
+            "w = Fp8Weight(torch.zeros((128, 128), dtype=torch.float8_e4m3fn), torch.ones((1, 1)))\n"
+            "assert w.nbytes() == 128 * 128 + 4 and K.moe_route_workspace_bytes(4, 2, 8) > 0\n")
+    r = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
