@@ -42,6 +42,7 @@ inline int fail_cuda(const char *file, int line, const char *func, cudaError_t e
     const char *base = file;
     for (const char *p = file; *p; ++p)
         if (*p == '/') base = p + 1;
+    (void)cudaGetLastError();  // reported here: it must not be found by the next launch's check (SB_LAUNCH_OK)
     last_error() = cat(func, " (", base, ":", line, "): CUDA error ", cudaGetErrorName(e), " (", cudaGetErrorString(e), "): ", msg);
     return STRIX_ERR_CUDA;
 }

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from fp8_ref import FP8, blocks, check_fp8_rows, route, rows_fp8, stack_fp8
+from strixite_b200 import StrixError
 from strixite_b200 import kernels as K
 from test_gpu_fp8 import ACTS, DT, gen, group, rand, run_route, some_ids
 
@@ -96,3 +97,36 @@ def test_combine_refuses_a_workspace_of_other_sizes(act, M, A, E, N):
     before = K.workspace_refusal_count()
     K.linear_fp8_experts_combine_grouped(hq, hs, K.Fp8Weight(wq, wsc, experts=E), E, ids, coef, ws, n, partial, M, A, y, act)
     assert K.workspace_refusal_count() == before + 1 and (partial == 5.0).all() and (y == 7.0).all()
+
+
+# ---- errors ----------------------------------------------------------------------------------------------------------
+
+
+def test_a_refused_launch_does_not_fail_the_next_call():
+    """A launch that the runtime refuses (the legacy stream while a stream that synchronises with it is captured) is the error of its own call
+    alone."""
+    rt = pytest.importorskip("cuda.bindings.runtime")
+    M, A, E = 4, 2, 8
+    ids = torch.zeros((M, A), dtype=torch.int32, device="cuda")
+    n = K.moe_route_workspace_bytes(M, A, E)
+    ws, err = torch.empty(n, dtype=torch.uint8, device="cuda"), K.new_err()
+    gu, h = torch.ones((4, 512), device="cuda"), torch.empty((4, 256), device="cuda")
+    q, s = torch.empty((4, 256), dtype=FP8, device="cuda"), torch.empty((4, 2), device="cuda")
+    calls = (lambda: K.moe_group_routes(ids, M, A, E, ws, n, err), lambda: K.swiglu_fp8(gu, q, s, 4, 256, K.Act.F32), lambda: K.swiglu(gu, h, 4, 256, K.Act.F32))
+    for call in calls:
+        call()  # set up
+    torch.cuda.synchronize()
+    assert torch.cuda.current_stream().cuda_stream == 0
+    for refused in calls:
+        rc, stream = rt.cudaStreamCreate()
+        assert int(rc) == 0
+        rc, = rt.cudaStreamBeginCapture(stream, rt.cudaStreamCaptureMode.cudaStreamCaptureModeRelaxed)
+        assert int(rc) == 0
+        with pytest.raises(StrixError, match="cudaErrorStreamCapture"):
+            refused()
+        rt.cudaStreamEndCapture(stream)
+        rt.cudaGetLastError()
+        rt.cudaStreamDestroy(stream)
+        for call in calls:
+            call()
+    torch.cuda.synchronize()
