@@ -549,7 +549,7 @@ int strix_linear_fp8_experts_combine_grouped(const uint8_t *hq, const float *hs,
              ": y overlaps the rows or their scales");
     auto st = static_cast<cudaStream_t>(stream);
     SB_TRY(grouped(fn, hq, hs, w, E, ws, ws_bytes, M, A, M * A, partial, kF32, st));
-    return sb::combine_reduce(fn, partial, ids, coef, M, A, E, N, y, act, st, nullptr, false, true, static_cast<const int32_t *>(ws));
+    return sb::combine_reduce(fn, partial, ids, coef, M, A, E, N, y, act, st, nullptr, false, static_cast<const int32_t *>(ws));
 }
 
 }  // extern "C"

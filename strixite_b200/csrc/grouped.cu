@@ -389,20 +389,32 @@ __global__ void __launch_bounds__(256)
     }
 }
 
-// Whether the product in front of a reduction has stored its partial sums: it stores none where the workspace `ws` was grouped for other
-// sizes (ws_is_for, which counts the refusal there), and then y is left as it is too. Null: no workspace belongs to the sums.
-__device__ __forceinline__ bool has_partials(const int32_t *ws, int64_t S, int64_t E) { return ws == nullptr || (ws[1] == S && ws[2] == E); }
+// The words of a workspace that say what it was grouped for. A product stores no partial sums where they are others than the call's
+// (ws_is_for, which counts the refusal there), and the reduction behind it then leaves y as it is too. Fetched in front of the sums'
+// loads and looked at behind them, so that the reduction does not wait for them.
+struct Header {
+    int32_t S, E;
+    __device__ __forceinline__ explicit Header(const int32_t *ws) {
+        asm volatile("ld.global.b32 %0, [%1+4];" : "=r"(S) : "l"(ws));
+        asm volatile("ld.global.b32 %0, [%1+8];" : "=r"(E) : "l"(ws));
+    }
+    __device__ __forceinline__ bool is_for(int64_t s, int64_t e) const { return S == s && E == e; }
+};
+struct NoHeader {  // no workspace belongs to the sums
+    __device__ __forceinline__ explicit NoHeader(const int32_t *) {}
+    __device__ __forceinline__ bool is_for(int64_t, int64_t) const { return true; }
+};
 
 // y[m, n] = sum_a fma(coef[m, a], partial[m * A + a, n], v), a ascending, one rounding; a token with any invalid id
 // gets a NaN row whatever its partials hold.
-template <typename T>
+template <typename T, typename Head>
 __global__ void __launch_bounds__(256)
     combine_reduce_kernel(const float *partial, const int32_t *ids, const float *coef, int64_t M, int64_t A, int64_t E,
                           int64_t N, T *y, const int32_t *ws) {
     wait_for_previous();
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= M * N) return;
-    const bool live = has_partials(ws, M * A, E);
+    const Head head(ws);
     const int64_t m = M * N <= 0xffffffffll ? (int64_t)((uint32_t)i / (uint32_t)N) : i / N, n = i - m * N;
     bool ok = true;
     float v = 0.f;
@@ -411,7 +423,7 @@ __global__ void __launch_bounds__(256)
         ok = ok && id >= 0 && id < E;
         v = fmaf(coef[m * A + a], partial[(m * A + a) * N + n], v);
     }
-    if (live) st_act(y, i, ok ? v : qnan());
+    if (head.is_for(M * A, E)) st_act(y, i, ok ? v : qnan());
 }
 
 // The same on four consecutive outputs per thread: 16-byte loads of the partial rows, four of them in flight per step.
@@ -429,14 +441,14 @@ __device__ __forceinline__ float4 ld_partial4(const void *partial, int64_t elem)
 }
 
 // FEW: too few threads to hide a round trip to memory behind others, so up to 16 slots' loads are under way at once.
-template <typename T, bool H, bool FEW = false>
+template <typename T, bool H, typename Head, bool FEW = false>
 __global__ void __launch_bounds__(256)
     combine_reduce4_kernel(const void *partial, const int64_t *pos, const int32_t *ids, const float *coef, int64_t M, int64_t A, int64_t E,
                            int64_t N, T *y, const int32_t *ws) {
     wait_for_previous();
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, N4 = N / 4;
     if (i >= M * N4) return;
-    const bool live = has_partials(ws, M * A, E);
+    const Head head(ws);
     const int64_t m = i / N4, n = (i - m * N4) * 4;
     bool ok = true;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -489,7 +501,7 @@ __global__ void __launch_bounds__(256)
         ok = ok && id >= 0 && id < E;
         v.x = fmaf(c, p.x, v.x), v.y = fmaf(c, p.y, v.y), v.z = fmaf(c, p.z, v.z), v.w = fmaf(c, p.w, v.w);
     }
-    if (!live) return;
+    if (!head.is_for(M * A, E)) return;
     const float q = qnan();
     st_act(y, m * N + n, ok ? v.x : q), st_act(y, m * N + n + 1, ok ? v.y : q), st_act(y, m * N + n + 2, ok ? v.z : q), st_act(y, m * N + n + 3, ok ? v.w : q);
 }
@@ -580,46 +592,46 @@ int combine_grouped(const char *fn, const void *h, const StackView &w, int64_t E
         SB_LAUNCH_OK(fn, " ", act_name(act), " M=", M, " A=", A, " E=", E, " N=", w.N, " K=", w.K, " G=", w.G);
     }
     const unsigned blocks = (unsigned)((M * w.N + 255) / 256);
-    if (act == kF32) combine_reduce_kernel<float><<<blocks, 256, 0, st>>>(partial, ids, coef, M, A, E, w.N, (float *)y, wsi);
-    else combine_reduce_kernel<uint16_t><<<blocks, 256, 0, st>>>(partial, ids, coef, M, A, E, w.N, (uint16_t *)y, wsi);
+    if (act == kF32) combine_reduce_kernel<float, Header><<<blocks, 256, 0, st>>>(partial, ids, coef, M, A, E, w.N, (float *)y, wsi);
+    else combine_reduce_kernel<uint16_t, Header><<<blocks, 256, 0, st>>>(partial, ids, coef, M, A, E, w.N, (uint16_t *)y, wsi);
     SB_LAUNCH_OK(fn, " reduce ", act_name(act), " M=", M, " A=", A, " N=", w.N);
     return 0;
 }
 
 int combine_reduce(const char *fn, const void *partial, const int32_t *ids, const float *coef, int64_t M, int64_t A, int64_t E, int64_t N,
-                   void *y, int act, cudaStream_t st, const int64_t *pos, bool half_partial, bool early, const int32_t *ws) {
+                   void *y, int act, cudaStream_t st, const int64_t *pos, bool half_partial, const int32_t *early_ws) {
     const bool vec = N % 4 == 0 && reinterpret_cast<uintptr_t>(partial) % 16 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
     SB_CHECK((pos == nullptr && !half_partial) || vec, fn, ": the indexed combine and F16 partial sums need N % 4 == 0 and 16-byte aligned buffers");
-    if (early && vec && !half_partial) {
+    if (early_ws != nullptr && vec && !half_partial) {
         const int64_t threads = M * (N / 4);
         const bool few = threads <= (int64_t)sm_count() * 256;  // 6 tokens x 10 x 2048 with the product in front: 19.0 -> 18.2 us
         const dim3 block(few ? 64 : 256), blocks((unsigned)((threads + block.x - 1) / block.x));
-        auto go = [&](auto kernel, auto *out) { return launch_after(kernel, blocks, block, 0, st, 1, partial, pos, ids, coef, M, A, E, N, out, ws); };
-        SB_CUDA((act == kF32 ? go(few ? combine_reduce4_kernel<float, false, true> : combine_reduce4_kernel<float, false, false>, static_cast<float *>(y))
-                             : go(few ? combine_reduce4_kernel<uint16_t, false, true> : combine_reduce4_kernel<uint16_t, false, false>, static_cast<uint16_t *>(y))),
+        auto go = [&](auto kernel, auto *out) { return launch_after(kernel, blocks, block, 0, st, 1, partial, pos, ids, coef, M, A, E, N, out, early_ws); };
+        SB_CUDA((act == kF32 ? go(few ? combine_reduce4_kernel<float, false, Header, true> : combine_reduce4_kernel<float, false, Header>, static_cast<float *>(y))
+                             : go(few ? combine_reduce4_kernel<uint16_t, false, Header, true> : combine_reduce4_kernel<uint16_t, false, Header>, static_cast<uint16_t *>(y))),
                 fn, " reduce ", act_name(act), " M=", M, " A=", A, " N=", N);
         return 0;
     }
     if (vec) {
         const unsigned blocks = (unsigned)((M * (N / 4) + 255) / 256);
         if (half_partial) {
-            if (act == kF32) combine_reduce4_kernel<float, true><<<blocks, 256, 0, st>>>(partial, pos, ids, coef, M, A, E, N, (float *)y, ws);
-            else combine_reduce4_kernel<uint16_t, true><<<blocks, 256, 0, st>>>(partial, pos, ids, coef, M, A, E, N, (uint16_t *)y, ws);
+            if (act == kF32) combine_reduce4_kernel<float, true, NoHeader><<<blocks, 256, 0, st>>>(partial, pos, ids, coef, M, A, E, N, (float *)y, nullptr);
+            else combine_reduce4_kernel<uint16_t, true, NoHeader><<<blocks, 256, 0, st>>>(partial, pos, ids, coef, M, A, E, N, (uint16_t *)y, nullptr);
         } else {
-            if (act == kF32) combine_reduce4_kernel<float, false><<<blocks, 256, 0, st>>>(partial, pos, ids, coef, M, A, E, N, (float *)y, ws);
-            else combine_reduce4_kernel<uint16_t, false><<<blocks, 256, 0, st>>>(partial, pos, ids, coef, M, A, E, N, (uint16_t *)y, ws);
+            if (act == kF32) combine_reduce4_kernel<float, false, NoHeader><<<blocks, 256, 0, st>>>(partial, pos, ids, coef, M, A, E, N, (float *)y, nullptr);
+            else combine_reduce4_kernel<uint16_t, false, NoHeader><<<blocks, 256, 0, st>>>(partial, pos, ids, coef, M, A, E, N, (uint16_t *)y, nullptr);
         }
     } else {
         const unsigned blocks = (unsigned)((M * N + 255) / 256);
         const float *pf = static_cast<const float *>(partial);
-        if (early) {
-            SB_CUDA((act == kF32 ? launch_after(combine_reduce_kernel<float>, dim3(blocks), dim3(256), 0, st, 1, pf, ids, coef, M, A, E, N, (float *)y, ws)
-                                 : launch_after(combine_reduce_kernel<uint16_t>, dim3(blocks), dim3(256), 0, st, 1, pf, ids, coef, M, A, E, N, (uint16_t *)y, ws)),
+        if (early_ws != nullptr) {
+            SB_CUDA((act == kF32 ? launch_after(combine_reduce_kernel<float, Header>, dim3(blocks), dim3(256), 0, st, 1, pf, ids, coef, M, A, E, N, (float *)y, early_ws)
+                                 : launch_after(combine_reduce_kernel<uint16_t, Header>, dim3(blocks), dim3(256), 0, st, 1, pf, ids, coef, M, A, E, N, (uint16_t *)y, early_ws)),
                     fn, " reduce ", act_name(act), " M=", M, " A=", A, " N=", N);
             return 0;
         }
-        if (act == kF32) combine_reduce_kernel<float><<<blocks, 256, 0, st>>>(pf, ids, coef, M, A, E, N, (float *)y, ws);
-        else combine_reduce_kernel<uint16_t><<<blocks, 256, 0, st>>>(pf, ids, coef, M, A, E, N, (uint16_t *)y, ws);
+        if (act == kF32) combine_reduce_kernel<float, NoHeader><<<blocks, 256, 0, st>>>(pf, ids, coef, M, A, E, N, (float *)y, nullptr);
+        else combine_reduce_kernel<uint16_t, NoHeader><<<blocks, 256, 0, st>>>(pf, ids, coef, M, A, E, N, (uint16_t *)y, nullptr);
     }
     SB_LAUNCH_OK(fn, " reduce ", act_name(act), " M=", M, " A=", A, " N=", N);
     return 0;

@@ -36,10 +36,10 @@ unsigned int prefill_ws_refusals();
 void prefill_cycles(unsigned long long *out, bool reset);
 
 // y[m, :] = sum_a coef[m, a] * partial[m * A + a, :] in ascending a; NaN rows for tokens with an invalid id (grouped.cu).
-// ws: the workspace that the product of the partial sums went by, if any; y is left as it is where that is grouped for other sizes.
-// early: may be set up while the kernel in front of it drains (launch_after; FP32 partials).
+// early_ws: the workspace of the product in front of it, if y is to be left as it is where that was grouped for other sizes; the kernel may
+// then be set up while the product drains (launch_after; FP32 partials).
 // pos: slot (m, a) is row pos[m * A + a] of partial; half_partial: the partial sums are F16 (prefill_experts with half_partial).
 int combine_reduce(const char *fn, const void *partial, const int32_t *ids, const float *coef, int64_t M, int64_t A, int64_t E, int64_t N,
-                   void *y, int act, cudaStream_t st, const int64_t *pos = nullptr, bool half_partial = false, bool early = false, const int32_t *ws = nullptr);
+                   void *y, int act, cudaStream_t st, const int64_t *pos = nullptr, bool half_partial = false, const int32_t *early_ws = nullptr);
 
 }  // namespace sb
