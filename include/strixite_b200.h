@@ -120,8 +120,9 @@ int strix_moe_shared_add_inject(void *y, const void *s, const float *gate_logit,
  * largest (2); the topk_group largest groups stay open and the k largest c among their experts are the picks. Ties go to the lower
  * index; the order is that of the 64-bit values of c (without a bias, of the logits). coef = s of the picks, divided by their sum when renorm (picks whose scores
  * all underflow to zero keep 0), times route_scale. ids, coef [M, A] in descending c, A = k (+ 1 with the shared slot, which is
- * filled as moe_router does). n_group <= 32 divides E <= 1024; k <= min(32, topk_group * E / n_group). A non-finite logit or bias
- * fails the token: ids -1, coef NaN, err = {1, token, expert}. */
+ * filled as moe_router does). n_group <= 32 divides E <= 1024 (as moe_router; moe_group_routes and
+ * the grouped products take up to 1023 experts); k <= min(32, topk_group * E / n_group). A non-finite logit or bias fails the token: ids
+ * -1, coef NaN, err = {1, token, expert}. */
 int strix_moe_router_scored(const void *logits, int64_t ld, int64_t M, int64_t E, int64_t k, int score, const float *bias,
                             int64_t n_group, int64_t topk_group, int64_t group_top, int renorm, float route_scale,
                             const void *shared_logit, int64_t shared_ld, int32_t shared_id, int32_t *ids, float *coef, int act,

@@ -67,7 +67,10 @@ __device__ __forceinline__ Pair2 fma2(Pair2 a, Pair2 b, Pair2 c) {
 }
 
 // The 8 N values (times `unit`, a factor that the block shares) as e4m3 bytes of v / scale, scale = max(amax * unit, 2^-100) / 448: the largest
-// magnitude (amax + amax_lo, unrounded) gets the largest e4m3 value, and a block of zeros has a scale that divides. A NaN stays one. The quotient is taken against the unrounded block maximum, in which the unit cancels: 448 / amax as two floats, three FMAs a value.
+// magnitude gets the largest e4m3 value, and a block of zeros has a scale that divides. A NaN stays one. The quotient is taken against
+// the block's largest in front of the scale's own rounding, in which the unit cancels: 448 / (amax + amax_lo) as two floats, three FMAs
+// a value. Only the norm of FP32 rows passes the largest value's second part; the others leave amax_lo at 0, and a block whose largest
+// was rounded has its codes at a scale that is off by up to 2^-24.
 template <int N>
 __device__ __forceinline__ void fp8_pack(const Block8 (&v)[N], float amax, float amax_lo, float unit, float &scale, uint2 (&codes)[N]) {
     const float top = amax * unit;

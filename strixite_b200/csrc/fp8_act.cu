@@ -27,7 +27,8 @@ __device__ __forceinline__ float block_fold(float *part, float v, F f) {
 // length: x' = x + y rounded to the activation type (what the residual stream keeps), r = 1 / sqrt(mean(x'^2) + eps) from the stored
 // values, h = x' r g. 16 neighbouring threads hold one 128-column block: its largest magnitude is a half-warp reduction.
 // Bound by memory: nothing is read twice, and the row's values never leave the registers (16384 x 2048 BF16 with residual and h: 53.2 us,
-// 5.7 TB/s).
+// 5.7 TB/s). A small batch of FP32 rows is bound by its blocks: 64 registers let 6 of 160 threads run on an SM, and the last 113 of 1001 rows
+// of 2560 are a second wave (6.3 us).
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kNormMaxThreads)
     rmsnorm_fp8_kernel(const T *x, const T *y, const float *w, float w_add, float eps, int d, float inv_d, T *x_out, T *h_out, uint8_t *q, float *scale,
@@ -172,7 +173,7 @@ struct RowOf {
 };
 
 // Eight lanes per (row, 128-column block) of h = silu(gate) * up, 16 elements a thread. Gate and up stay FP32 until the one rounding
-// to e4m3. FP32 rows are bound by memory (40960 x 512: 28.5 us, 6.6 TB/s), BF16 rows by the instructions issued (19.4 us, 5.4 TB/s; with
+// to e4m3. FP32 rows are bound by memory (40960 x 512: 28.5 us, 6.6 TB/s), BF16 rows by the instructions issued (19.5 us, 5.4 TB/s; with
 // 8 elements a thread, whose index, maximum and scale cost as much as those of 16: 25.1 us, and with scalar arithmetic 26.5). Small
 // blocks, as many as there is work: 256 threads and blocks that stay for several units: 21.9 us; with 8 blocks an SM for BF16: 20.0.
 constexpr int kSwigluThreads = 128, kSwigluUnits = kSwigluThreads / 8;  // of a block

@@ -15,7 +15,9 @@
 // ahead), warp 8 issues TMA, warps 9 and 10 the MMAs of half 0 and 1 (those of CTA 0 for both CTAs), warps 11-13 gather rows of x. The
 // sums leave through a 64-byte-wide staging strip per warp so that a store covers whole sectors of a row.
 //
-// Measured: 16384 x 4096 x 4096 246 us, 2.23 PFLOP/s, tensor pipe 61 % active; 4096 tokens x 10 of 512 experts [1024, 2048] 247 us, 4.8 TB/s.
+// Measured at the full clock (1965 MHz): 16384 x 4096 x 4096 245 us, 2.24 PFLOP/s, tensor pipe 61 % active; 4096 tokens x 10 of 512 experts
+// [1024, 2048] 243 us, 4.9 TB/s. Called again and again for more than ~0.1 s both bring the GPU to its power limit: at 1425 to 1475 MHz 287 us
+// (1.92 PFLOP/s) and, with the grouping, 308 us for 262.
 // What bounds both is the chain of a block: its MMAs' commit, the promotion, the accumulator's release, ~750 clocks for 512 of MMA with
 // tensor memory full (the grouped feed alone takes 181 to 190 us).
 // Every mbarrier wait is bounded: on expiry the CTA raises the abort counter, waits for its copies, frees its tensor memory, returns.
@@ -502,9 +504,10 @@ namespace fp8 {
 
 int wide_dense(const char *fn, const uint8_t *w, int64_t w_rows, const uint8_t *x, int64_t x_rows, int64_t K, const GemmArgs &a, cudaStream_t st) {
     const int64_t tiles = ((int64_t)a.M + 2 * kRows - 1) / (2 * kRows);
-    // K over two pairs where that many clusters of four run at once (33 on 148 SMs: 34 of them took twice the time of 33) and K is long
-    // enough to pay for bringing the sums together: [4096, 7168], 256 rows 27.1 -> 19.2 us; [4096, 4096], 512: 19.0 -> 15.7; [8192, 2048], 256:
-    // 12.6 -> 12.7; [4096, 1024], 400: 9.0 -> 10.1.
+    // K over two pairs where that many clusters of four run at once (33 on 148 SMs: 34 of them took twice the time of 33; the rule stops at 32)
+    // and K is long enough to pay for bringing the sums together: [4096, 7168], 256 rows 27.1 -> 19.2 us; [4096, 4096], 512: 18.5 -> 15.5;
+    // [4096, 1024], 400: 9.0 -> 10.1. The sides meet between 12 and 18 blocks of K (without -> with, 12 / 16 / 18 / 20 blocks: [4096, K], 512
+    // rows 10.3 -> 11.0 / 11.9 -> 11.9 / 12.5 -> 12.3 / 13.5 -> 12.8; [8192, K], 256: 10.3 -> 11.0 / 12.2 -> 12.1 / 12.8 -> 12.5 / 13.6 -> 12.9).
     if (a.KB >= 20 && tiles * ((a.N + kColTile - 1) / kColTile) * 9 <= sm_count() * 2) return launch<2, false, true>(fn, w, w_rows, x, x_rows, K, a, tiles, st);
     return launch<2, false, false>(fn, w, w_rows, x, x_rows, K, a, tiles, st);
 }

@@ -162,8 +162,10 @@ __device__ __forceinline__ float4 load4(const uint16_t *p) {
 // The choice: the k-th largest lane maximum bounds the k-th largest value from below, what reaches it are the candidates (about 1.3 k of
 // them), they meet in shared memory and each counts those in front of it: no k rounds of warp-wide maxima. Where neighbours in that
 // order are closer than the error, the candidates are valued again in 64 bits (one token in a thousand).
-// Bound by the instructions issued: 16384 x 512 experts, 10 of 4 of 8 groups, 22.5 us, of which the loads are 4.9, scores 2.9, groups
-// 3.5, candidates and their order 7, the last step 4.
+// Bound by the instructions issued, 1046 a token: 16384 x 512 experts, 10 of 4 of 8 groups, 22.2 us, of which the loads are 4.9, scores 2.9,
+// groups 3.5, candidates and their order 7, the last step 4. Groups that do not fill the vectors load element by element (16384 x 1008 in
+// 16 groups: 78 us), and with as many picks as open lanes the bound is near the least lane maximum, so that most experts are
+// candidates (32 of 256 in one group: 249 us).
 //
 // The FP32 errors that the choice allows for (documented bounds: expf 2 ulp; ex2.approx 2^-22, rcp.approx 2^-23 relative):
 //   sigmoid  e = 2^(-l log2 e): the argument's roundings move e by 1.5 |l| 2^-24, so p by p (1 - p) (2^-22 + 1.5 |l| 2^-24) <= 0.7 * 2^-23; 1 + e
@@ -467,6 +469,8 @@ __global__ void __launch_bounds__(kWarps * 32, NV <= 8 ? 14 : 0) router_scored_k
         const RouteArgs copy = a;  // taking a's own address would move every use of it to local memory (25 -> 34 us at 16384 x 512)
         route_64(row, copy, m);
     } else {
+        // The weights in FP32 from the picks' exact logits: scores, their sum, the quotient and the scale round to 2^-24 each (6.7e-8 off on average
+        // at 16384 x 512; in 64 bits with one rounding it would be 2.7e-8).
         float p = 0.f;
         if (lane < a.k) {
             if (a.score == kSigmoid) {
